@@ -125,6 +125,13 @@ __device__ __forceinline__ void x3_store4(uint16_t* __restrict__ y3, int64_t row
 // call: every entry point that can fill one takes it first thing, so a registration never leaks to a later call
 void styler_take_x3_out(uint16_t** y3, int* parts);
 
+// a * b rounded to fp32: a consumer that adds it cannot contract the product into an fma.  Kernels that have to agree bit for
+// bit on a quantity they use twice (as it is and inside a sum) form it this way.
+__device__ __forceinline__ float mul_rounded(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // v - float(bf16(v)): the low part of the hi + lo split of the bf16x3 arithmetic (exact in fp32)
 __device__ __forceinline__ float bf16_lo_part(float v) { return v - __uint_as_float(f32_to_bf16_bits(v) << 16); }
 

@@ -22,6 +22,18 @@
 // Same expressions in the same order as before: the results are bit-identical to the round-2 kernel.
 enum { LNM_ALL16 = 1, LNM_DOT = 2, LNM_DROP = 4, LNM_INDROP = 8, LNM_LEN = 16, LNM_RELU = 32 };
 
+// Wave-wide sum from the nearest lanes to the farthest (xor 1, 2, 4, 8, 16, 32): the order in which the sixteen-lanes-per-row
+// kernel below adds a row's channels.  A mirror of eight (sixteen) lanes is xor 4 (8) where the quads (halves) already agree.
+__device__ __forceinline__ float wave_sum_up(float v) {
+  v += dpp_f32<0xB1>(v);                               // quad_perm [1,0,3,2]
+  v += dpp_f32<0x4E>(v);                               // quad_perm [2,3,0,1]
+  v += dpp_f32<0x141>(v);                              // row_half_mirror
+  v += dpp_f32<0x140>(v);                              // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
 template <int R, int M, bool Y3 = false>
 __global__ __launch_bounds__(64 * LNB_WAVES) void layernorm_bwd_kernel(
     const float* __restrict__ x, int64_t ldx, const float* __restrict__ dy, int64_t lddy,
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void layernorm_bwd_kernel(
 #pragma unroll
     for (int k = 0; k < R; ++k) mean[k] = v[k].x + v[k].y + v[k].z + v[k].w;
 #pragma unroll
-    for (int k = 0; k < R; ++k) mean[k] = wave_sum(mean[k]);
+    for (int k = 0; k < R; ++k) mean[k] = wave_sum_up(mean[k]);
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       mean[k] *= (1.f / 256.f);
@@ -179,7 +191,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void layernorm_bwd_kernel(
       rstd[k] = h[k].x * h[k].x + h[k].y * h[k].y + h[k].z * h[k].z + h[k].w * h[k].w;
     }
 #pragma unroll
-    for (int k = 0; k < R; ++k) rstd[k] = wave_sum(rstd[k]);
+    for (int k = 0; k < R; ++k) rstd[k] = wave_sum_up(rstd[k]);
     float m1[R], m2[R];
     float4 ex[R];
 #pragma unroll
@@ -195,12 +207,12 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void layernorm_bwd_kernel(
         ag.x += d[k].x * h[k].x; ag.y += d[k].y * h[k].y; ag.z += d[k].z * h[k].z; ag.w += d[k].w * h[k].w;
         ab.x += d[k].x; ab.y += d[k].y; ab.z += d[k].z; ab.w += d[k].w;
       }
-      ex[k] = make_float4(d[k].x * g.x, d[k].y * g.y, d[k].z * g.z, d[k].w * g.w);
+      ex[k] = make_float4(mul_rounded(d[k].x, g.x), mul_rounded(d[k].y, g.y), mul_rounded(d[k].z, g.z), mul_rounded(d[k].w, g.w));
       m1[k] = ex[k].x + ex[k].y + ex[k].z + ex[k].w;
       m2[k] = ex[k].x * h[k].x + ex[k].y * h[k].y + ex[k].z * h[k].z + ex[k].w * h[k].w;
     }
 #pragma unroll
-    for (int k = 0; k < R; ++k) { m1[k] = wave_sum(m1[k]); m2[k] = wave_sum(m2[k]); }
+    for (int k = 0; k < R; ++k) { m1[k] = wave_sum_up(m1[k]); m2[k] = wave_sum_up(m2[k]); }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       if (!live[k]) continue;
@@ -260,8 +272,9 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void layernorm_bwd_kernel(
 // channels 16 l .. 16 l + 15 as two 16-byte loads per tensor -- so a wave works on FOUR rows at once, a reduction is four DPP
 // steps inside a 16-lane DPP row (quad permutes, row_half_mirror, row_mirror: no cross-row traffic at all), and the
 // per-row overhead is shared by four rows: ~75 wave-instructions per row.  Two row groups per iteration are in flight.
-// Same arithmetic per element as the kernel above (fp32, statistics recomputed from the saved sum); the order of the additions
-// inside a reduction differs, i.e. results agree to fp32 rounding, not bit for bit (tests/test_20_hip_backward.py).
+// Same arithmetic per element as the kernel above (fp32, statistics recomputed from the saved sum), and the same order of the
+// additions inside a row's reductions -- four channels in sequence, then neighbouring quads, pairs of quads, ... (wave_sum_up) --
+// so dx agrees bit for bit; the parameter gradients sum over the rows in another order.
 __device__ __forceinline__ float q16_sum(float v) {
   v += dpp_f32<0xB1>(v);                               // quad_perm [1,0,3,2]
   v += dpp_f32<0x4E>(v);                               // quad_perm [2,3,0,1]
@@ -375,22 +388,27 @@ __global__ __launch_bounds__(512) void layernorm_bwd_q16_kernel(
 #pragma unroll
         for (int k = 0; k < 16; ++k) { v[k] = 0.f; d[k] = 0.f; }
       }
-      float sm = 0.f;
+      float h[16], ex[16], p4[4], r4[4];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) sm += v[k];
-      const float mean = q16_sum(sm) * (1.f / 256.f);
-      float h[16], ss = 0.f;
+      for (int j = 0; j < 4; ++j) p4[j] = v[4 * j] + v[4 * j + 1] + v[4 * j + 2] + v[4 * j + 3];
+      const float mean = q16_sum((p4[0] + p4[1]) + (p4[2] + p4[3])) * (1.f / 256.f);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) { h[k] = v[k] - mean; ss += h[k] * h[k]; }
-      const float rstd = 1.0f / sqrtf(q16_sum(ss) * (1.f / 256.f) + 1e-5f);
-      float ex[16], m1 = 0.f, m2 = 0.f;
+      for (int k = 0; k < 16; ++k) h[k] = v[k] - mean;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p4[j] = h[4 * j] * h[4 * j] + h[4 * j + 1] * h[4 * j + 1] + h[4 * j + 2] * h[4 * j + 2] + h[4 * j + 3] * h[4 * j + 3];
+      const float rstd = 1.0f / sqrtf(q16_sum((p4[0] + p4[1]) + (p4[2] + p4[3])) * (1.f / 256.f) + 1e-5f);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         h[k] *= rstd;
-        ex[k] = d[k] * g[k];
-        m1 += ex[k];
-        m2 += ex[k] * h[k];
+        ex[k] = mul_rounded(d[k], g[k]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p4[j] = ex[4 * j] + ex[4 * j + 1] + ex[4 * j + 2] + ex[4 * j + 3];
+        r4[j] = ex[4 * j] * h[4 * j] + ex[4 * j + 1] * h[4 * j + 1] + ex[4 * j + 2] * h[4 * j + 2] + ex[4 * j + 3] * h[4 * j + 3];
+      }
+      float m1 = (p4[0] + p4[1]) + (p4[2] + p4[3]), m2 = (r4[0] + r4[1]) + (r4[2] + r4[3]);
       if (gq.live) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) { ag[k] += d[k] * h[k]; ab[k] += d[k]; }
