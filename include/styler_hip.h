@@ -35,6 +35,8 @@ extern "C" {
 #define STYLER_ACT_LOGCLAMP 3 /* log(max(v, 1e-5)): dynamic_range_compression, audio_processing.py:80-86 */
 #define STYLER_ACT_LEAKY 4    /* v > 0 ? v : 0.1 v: LRELU_SLOPE of the vocoder, hifigan/models.py:7,97 */
 #define STYLER_ACT_CRELU 5    /* min(max(v, 0), 20): DeepSpeaker's clipped ReLU, deepspeaker/conv_models.py:83-86 */
+#define STYLER_ACT_SILU 6     /* v / (1 + exp(-v)): styler_groupnorm_act only */
+#define STYLER_ACT_GELU 7     /* 0.5 v (1 + erf(v / sqrt 2)): styler_groupnorm_act only */
 /* OR-ed into `act`: the residual input joins BEFORE scale / shift / activation, y = act(scale * (acc + res) + shift)
  * -- the last call of a convolution that is summed over several GEMM calls (2-D taps of the ResCNN, conv_models.py) */
 #define STYLER_ACT_RES_FIRST 0x100
@@ -891,6 +893,62 @@ int styler_sumsq(const float* g, int64_t n, double* out, void* stream);
 int styler_adam_step(float* p, const float* g, float* m, float* v, int64_t n, const double* sumsq,
                      float max_norm, float lr, float beta1, float beta2, float eps, int step,
                      float grad_scale, void* stream);
+
+/* ---- operators of a decoder block that reads an encoder's states ---------------------------------------------------------
+ * Tensors are fp32 or (bf16 = 1) bf16; parameters, statistics and sums are fp32. */
+
+/* Attention of queries [B, Lq, H, D] over keys / values [B, Lk, G, D] of another sequence, H % G == 0 (head h reads key head
+ * h / (H / G)), D a multiple of 8 up to 128:  out = softmax(scale q k^T over the seen keys) v.  Key j of item b is seen iff
+ * j < len[b] (len may be NULL) and mask[b * maskb + j] == 0 (mask may be NULL); what an unseen key's rows hold is not used.
+ * Queries at or past q_len[b] (may be NULL) and queries that see no key give zeros and lse = -inf.  lse [B, H, Lq] (natural
+ * logarithm of the softmax's denominator, scores included) may be NULL in the forward.  Strides (item, row, head) are in
+ * elements, multiples of 16 bytes, features contiguous, 16-byte aligned bases; out / dq [B, Lq, H, D] and dk / dv
+ * [B, Lk, G, D]: `out` by its strides, the gradients contiguous.  The backward takes the forward's out and lse; unseen keys and
+ * queries past their length get zero gradients.  No atomics: both directions are deterministic.  The workspace
+ * (styler_cross_attention_workspace_bytes, 16-byte aligned) belongs to the call until it has run on its stream. */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  const void* dout;
+  void *dq, *dk, *dv;
+  float* lse;
+  const int64_t *len, *q_len;
+  const uint8_t* mask;
+  int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh; /* q, k, v, out, dout: item, row, head stride */
+  int64_t maskb;
+  int32_t B, Lq, Lk, H, G, D, bf16;
+  float scale;
+} styler_xattn_t;
+int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int bwd);
+int styler_cross_attention(const styler_xattn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
+int styler_cross_attention_bwd(const styler_xattn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rotary positions: y[b, l, h, :] = x[b, l, h, :] with pair i of the first `rot` (even) features turned by pos[b, l] * freqs[i]
+ * and scaled by `gain`; features rot .. D-1 are copied.  Pair i = (2i, 2i+1) (interleaved) or (i, i + rot/2).  inverse = 1 turns
+ * the other way: the gradient dx of dy.  freqs: rot/2 doubles (angle per position); pos_kind 0: pos = l, 1: int64, 2: float, with
+ * item stride posb (0: one row for all).  Strides (item, row, head) in elements, features contiguous; x == y with equal strides is
+ * allowed (in place), any other overlap is not. */
+int styler_rotary(const void* x, int64_t xb, int64_t xl, int64_t xh, void* y, int64_t yb, int64_t yl, int64_t yh,
+                  const double* freqs, const void* pos, int64_t posb, int pos_kind, int B, int L, int H, int D, int rot,
+                  int interleaved, int inverse, float gain, int bf16, void* stream);
+
+/* Group norm over channels-last [B, L, C] with an activation (STYLER_ACT_NONE / RELU / SILU / GELU), C % G == 0: statistics of
+ * group g over the C / G channels of the rows t < len[b] (len may be NULL), biased variance; rows at or past len[b] give zeros.
+ * out = y; stats [B, G, 2] receives mean and 1 / sqrt(var + eps) (may be NULL in the forward).  The backward takes x, dy, stats
+ * and gives dx in `out` and dgamma, dbeta [C].  Strides (item, row) in elements, channels contiguous.  Deterministic. */
+typedef struct {
+  const void *x, *dy;
+  void* out;
+  const float *gamma, *beta;
+  float *stats, *dgamma, *dbeta;
+  const int64_t* len;
+  int64_t xb, xl, db, dl, ob, ol; /* x, dy, out: item, row stride */
+  int32_t B, L, C, G, act, bf16;
+  float eps;
+} styler_gn_t;
+int64_t styler_groupnorm_act_workspace_bytes(int B, int L, int C, int G, int bf16, int bwd);
+int styler_groupnorm_act(const styler_gn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
+int styler_groupnorm_act_bwd(const styler_gn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Self-test: out_swap / out_shfl [groups * 64] receive, for every 64-value group of `in`, the wave-wide sum computed by the
  * library's reduction (v_permlane32/16_swap + DPP) and by the six-step __shfl_xor butterfly; the two must be bit-identical. */

@@ -146,6 +146,13 @@ _SIGS = {
     "styler_ds_rows": [P, P, I, I, I, I, I, I, I, P],
     "styler_ds_crelu_add": [P, P, P, I64, P],
     "styler_l2_normalize_rows": [P, P, I, I, P],
+    "styler_cross_attention_workspace_bytes": [I, I, I, I, I, I, I, I],
+    "styler_cross_attention": [P, P, I64, P],
+    "styler_cross_attention_bwd": [P, P, I64, P],
+    "styler_rotary": [P, I64, I64, I64, P, I64, I64, I64, P, P, I64, I, I, I, I, I, I, I, I, F, I, P],
+    "styler_groupnorm_act_workspace_bytes": [I, I, I, I, I, I],
+    "styler_groupnorm_act": [P, P, I64, P],
+    "styler_groupnorm_act_bwd": [P, P, I64, P],
     "styler_stft_mel_varlen": [P, I64, P, P, P, P, P, P, P, F, F, P, P, P, I, I, I, P],
 }
 
@@ -188,6 +195,18 @@ class CopyDesc(ctypes.Structure):
     _fields_ = [("src", ctypes.c_uint64), ("src2", ctypes.c_uint64), ("dst", ctypes.c_uint64)] + \
                [(k, ctypes.c_int64) for k in ("ss0", "ss1", "ss2", "ds0", "ds1", "ds2", "block_start")] + \
                [(k, ctypes.c_int32) for k in ("d0", "d1", "d2", "flags")]
+
+
+class XattnArgs(ctypes.Structure):
+    _fields_ = [(k, P) for k in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "len", "q_len", "mask")] + \
+               [(k, I64) for k in ("qb", "ql", "qh", "kb", "kl", "kh", "vb", "vl", "vh", "ob", "ol", "oh", "gb", "gl", "gh", "maskb")] + \
+               [(k, ctypes.c_int32) for k in ("B", "Lq", "Lk", "H", "G", "D", "bf16")] + [("scale", F)]
+
+
+class GnArgs(ctypes.Structure):
+    _fields_ = [(k, P) for k in ("x", "dy", "out", "gamma", "beta", "stats", "dgamma", "dbeta", "len")] + \
+               [(k, I64) for k in ("xb", "xl", "db", "dl", "ob", "ol")] + \
+               [(k, ctypes.c_int32) for k in ("B", "L", "C", "G", "act", "bf16")] + [("eps", F)]
 
 
 class LstmBwdDesc(ctypes.Structure):

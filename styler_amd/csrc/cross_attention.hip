@@ -1,0 +1,945 @@
+// Attention between two sequences (queries of one, keys and values of the other), forward and backward, bf16 or fp32.
+//
+//   o[q, h] = sum_j p_j v[j, h / R],  p = softmax_j(scale q[q, h] . k[j, h / R]) over the keys j that are SEEN:
+//   j < len[b] and not mask[b, j].  R = H / G query heads share a key head.  A query past q_len[b] and a query that sees no
+//   key give 0 (lse = -inf).  With P_ij = exp(scale s_ij - lse_i) and delta_i = sum_d do_id o_id:
+//   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - delta_i),  dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
+//   the sums over i running over the R heads of the group as well.
+//
+// Decomposition.  The R heads of a group and the queries are ONE row axis, m = q R + r (M = Lq R rows per item and key head):
+// a single token of a grouped model fills R rows of a tile instead of one.  S^T = K Q^T on 32 x 32 matrix tiles, so a lane owns
+// one row (column li = lane & 31 of S^T) and the 16 accumulator registers are 16 keys of it (keys (r&3) + 8 (r>>2) + 4 (lane>>5)):
+// the softmax is a running maximum and sum per lane plus one exchange with lane ^ 32, and P never leaves its registers -- the
+// product over the keys consumes them in place (bf16: packed in pairs, the other operand through the transposing LDS read;
+// fp32: register r of both half waves IS the k pair of v_mfma_f32_32x32x2_f32).
+//
+// Tiles go memory -> LDS by DMA (buffer_load_dwordx4 ... lds), one tile ahead.  A lane whose key is not seen, or whose feature
+// is past D (heads that are no multiple of the tile width), gives an offset past the descriptor: the DMA writes zeros, so
+// nothing that stands in an unseen row (NaN, infinities) enters a product.  The 16-byte pieces of a row are permuted by the row
+// index (swz): both the row-wise ds_read_b128 and the transposing reads then touch distinct banks.
+#include <type_traits>
+#include "common.h"
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr uint32_t OOB = 0x80000000u;                  // past every descriptor's num_records
+constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
+
+struct XArgs {
+  const void *q, *k, *v, *o, *dout;                    // dout / o: backward
+  void *out, *dq, *dk, *dv;
+  float* lse;                                          // [B, H, Lq]
+  float* delta;                                        // [B, H, Lq] (backward workspace)
+  float* part;                                         // partial results of a split launch
+  const int64_t *len, *qlen;
+  const uint8_t* mask;
+  int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh;   // strides (elements): item, row, head; g: dout
+  int64_t maskb;
+  int B, Lq, Lk, H, G, R, D, nrt, splits;
+  float scale;
+};
+
+__device__ __forceinline__ int clamp_len(const int64_t* len, int b, int L) {
+  if (!len) return L;
+  const int64_t n = len[b];
+  return n < 0 ? 0 : (n > L ? L : (int)n);
+}
+
+// Launch slot -> logical block: workgroups go to the eight XCDs round robin, and blocks that read the same keys are
+// neighbours in the logical order -- an XCD (and its L2) gets consecutive ones.
+__device__ __forceinline__ int xcd_block(int total) {
+  const int n = blockIdx.x;
+  const int v = (n & 7) * (int)(gridDim.x >> 3) + (n >> 3);
+  return v < total ? v : -1;
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<uint16_t> { static constexpr bool bf16 = true; };
+template <> struct Elem<float> { static constexpr bool bf16 = false; };
+
+// ---- LDS tiles: rows of DT elements, RB bytes ---------------------------------------------------------------------------------
+// The 16-byte piece c of row r stands at piece c ^ swz(r).  256 bytes are the 64 banks once: rows narrower than that share a
+// bank line, so the row index is divided by the rows per line first; its bits enter reversed, so that the four consecutive rows
+// of a transposing read differ in the high piece bits (its 32 lanes read four neighbouring pieces of each of the four rows).
+template <int RB> struct Swz {
+  static constexpr int NCH = RB / 16 < 16 ? RB / 16 : 16, RPL = RB < 256 ? 256 / RB : 1;
+  static constexpr int BITS = NCH == 16 ? 4 : (NCH == 8 ? 3 : (NCH == 4 ? 2 : 1));
+  __device__ static constexpr uint32_t of(uint32_t row) {
+    uint32_t x = row / RPL, r = 0;
+    for (int i = 0; i < BITS; ++i) r |= ((x >> i) & 1u) << (BITS - 1 - i);
+    return r;
+  }
+};
+
+// Fill ROWS rows (a multiple of 32) of a tile: 1 KB per instruction, dealt to the WAVES waves.  off(row) = byte offset of a
+// tile row from the descriptor's base, seen(row) = its row may be read.
+template <int RB, int ROWS, int WAVES, typename Seen>
+__device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* base, int64_t ldbytes, int dbytes, int wave, int lane,
+                                         Seen seen) {
+  constexpr int RPI = 1024 / RB, N = ROWS * RB / 1024;       // rows per instruction, instructions
+  static_assert(N % WAVES == 0 || N < WAVES, "");
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+  const int lrow = lane / (RB / 16);
+  const uint32_t piece = lane % (RB / 16);
+#pragma unroll
+  for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
+    const int ins = i * WAVES + wave;
+    if (N % WAVES != 0 && ins >= N) break;
+    const int row = ins * RPI + lrow;
+    const uint32_t c = (piece ^ Swz<RB>::of(row)) * 16;
+    const uint32_t off = (c < (uint32_t)dbytes && seen(row)) ? (uint32_t)(row * (int)ldbytes) + c : OOB;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + lds + ins * 1024), 16, off, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void wait_tiles() {         // this wave's DMA has landed and its LDS reads are done; then all waves'
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// ---- matrix products ----------------------------------------------------------------------------------------------------------
+// Frag: a lane's own row (32 rows of a wave), the half of its features that its half wave (lh) feeds to the product over d.
+template <typename T, int DT> struct Frag;
+template <int DT> struct Frag<uint16_t, DT> { bf16x8 v[DT / 16]; };
+template <int DT> struct Frag<float, DT> { float4 v[DT / 8]; };
+
+template <typename T, int DT>
+__device__ __forceinline__ void load_frag(Frag<T, DT>& f, const T* row, int D, int lh, bool ok) {
+  constexpr int E = 16 / sizeof(T);                          // elements per 16-byte piece; lane lh takes the pieces 2 i + lh
+#pragma unroll
+  for (int i = 0; i < DT / E / 2; ++i) {
+    const int d = (2 * i + lh) * E;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (ok && d < D) u = *reinterpret_cast<const uint4*>(row + d);
+    f.v[i] = *reinterpret_cast<const typename std::remove_reference<decltype(f.v[0])>::type*>(&u);
+  }
+}
+template <int DT> __device__ __forceinline__ float frag_dot(const Frag<uint16_t, DT>& a, const Frag<uint16_t, DT>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < DT / 16; ++i) {
+    const uint4 x = *reinterpret_cast<const uint4*>(&a.v[i]), y = *reinterpret_cast<const uint4*>(&b.v[i]);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), s);
+      s = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), s);
+    }
+  }
+  return s;
+}
+template <int DT> __device__ __forceinline__ float frag_dot(const Frag<float, DT>& a, const Frag<float, DT>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < DT / 8; ++i)
+    s = fmaf(a.v[i].x, b.v[i].x, fmaf(a.v[i].y, b.v[i].y, fmaf(a.v[i].z, b.v[i].z, fmaf(a.v[i].w, b.v[i].w, s))));
+  return s;
+}
+
+__device__ __forceinline__ void zero16(f32x16& a) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) a[r] = 0.f;
+}
+
+// s[32 tile rows][32 lane rows] += tile(rows blk * 32 ..) . frag
+template <typename T, int DT>
+__device__ __forceinline__ void mma_rows(f32x16& s, const char* tile, int blk, const Frag<T, DT>& f, int li, int lh) {
+  constexpr int RB = DT * sizeof(T);
+  const char* row = tile + (blk * 32 + li) * RB;
+  const uint32_t x = (lh ^ Swz<RB>::of(li)) * 16;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i) {
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + (x ^ (i * 32)));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, f.v[i], s, 0, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < DT / 8; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(row + (x ^ (i * 32)));
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, f.v[i].x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, f.v[i].y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, f.v[i].z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, f.v[i].w, s, 0, 0, 0);
+    }
+  }
+}
+
+__device__ __forceinline__ bf16x8 pack8(const f32x16& a, int s2) {
+  uint4 v = make_uint4(cvt_pk_bf16_rne(a[s2 * 8 + 0], a[s2 * 8 + 1]), cvt_pk_bf16_rne(a[s2 * 8 + 2], a[s2 * 8 + 3]),
+                       cvt_pk_bf16_rne(a[s2 * 8 + 4], a[s2 * 8 + 5]), cvt_pk_bf16_rne(a[s2 * 8 + 6], a[s2 * 8 + 7]));
+  return *reinterpret_cast<bf16x8*>(&v);
+}
+
+// acc[dt][32 features][32 lane rows] += tile(rows blk * 32 ..)^T . p      (p: accumulator registers of a 32 x 32 product; bf16:
+// rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain)
+template <typename T, int DT>
+__device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* tile, int blk, const f32x16& p, int lane) {
+  constexpr int RB = DT * sizeof(T);
+  const int li = lane & 31, lh = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    const int tq = lane & 15, tc = (lane >> 4) & 1, r0 = lh * 4 + (tq >> 2);
+    const uint32_t x = ((tc * 2 + ((tq & 3) >> 1)) ^ Swz<RB>::of(r0)) * 16 + (tq & 1) * 8;
+    const char* base = tile + (blk * 32 + r0) * RB;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const bf16x8 pb = pack8(p, s2);
+#pragma unroll
+      for (int dt = 0; dt < DT / 32; ++dt) {
+        // rows r0 + 16 s2 and r0 + 16 s2 + 8: the swizzle of r0 + 16 s2 is that of r0 where a tile row has 8 or 16 pieces (a
+        // period of 16 rows); with 4 pieces the period is 16 too
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(base + s2 * 16 * RB + (x ^ (dt * 64)))));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(base + (s2 * 16 + 8) * RB + (x ^ (dt * 64) ^ (Swz<RB>::of(8) * 16)))));
+        const uint2 ua = *reinterpret_cast<const uint2*>(&a), ub = *reinterpret_cast<const uint2*>(&b);
+        uint4 u = make_uint4(ua.x, ua.y, ub.x, ub.y);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<bf16x8*>(&u), pb, acc[dt], 0, 0, 0);
+      }
+    }
+  } else {
+    const uint32_t x = ((li >> 2) ^ Swz<RB>::of(lh * 4)) * 16 + (li & 3) * 4;
+    const char* base = tile + (blk * 32 + lh * 4) * RB;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = (r & 3) + 8 * (r >> 2);
+#pragma unroll
+      for (int dt = 0; dt < DT / 32; ++dt) {
+        const float a = *reinterpret_cast<const float*>(base + row * RB + (x ^ (dt * 128) ^ (Swz<RB>::of(row) * 16)));
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// a lane's row of acc (features dt * 32 + 8 g + 4 lh + 0..3) times c -> memory
+template <typename T, int DT>
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DT / 32], int D, int lh, float c) {
+#pragma unroll
+  for (int dt = 0; dt < DT / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = dt * 32 + g * 8 + lh * 4;
+      if (d >= D) continue;
+      const float x = acc[dt][g * 4] * c, y = acc[dt][g * 4 + 1] * c, z = acc[dt][g * 4 + 2] * c, w = acc[dt][g * 4 + 3] * c;
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + d) = make_uint2(cvt_pk_bf16_rne(x, y), cvt_pk_bf16_rne(z, w));
+      else *reinterpret_cast<float4*>(row + d) = make_float4(x, y, z, w);
+    }
+}
+template <typename T, int DT>
+__device__ __forceinline__ void store_zero(T* row, int D, int lh) {
+#pragma unroll
+  for (int i = 0; i < DT / 8; ++i) {
+    const int d = i * 8 + lh * 4;
+    if (d < D) {
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + d) = make_uint2(0, 0);
+      else *reinterpret_cast<float4*>(row + d) = make_float4(0, 0, 0, 0);
+    }
+  }
+}
+
+// The seen keys of a tile as bit words, 32 keys each (uniform over the wave).  Without a mask they follow from the length; with
+// one, lane i holds the mask bytes of keys i and (tiles of 128) 64 + i, fetched one tile before they are needed.
+template <int KT> struct KeyWords {
+  uint32_t w[KT / 32];
+  __device__ __forceinline__ bool none() const {
+    uint32_t x = 0;
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) x |= w[i];
+    return x == 0;
+  }
+};
+template <int KT> struct MaskBytes { uint8_t b[(KT + 63) / 64]; };
+template <int KT>
+__device__ __forceinline__ void mask_fetch(MaskBytes<KT>& m, const uint8_t* mask, int k0, int klen, int lane) {
+#pragma unroll
+  for (int i = 0; i < (KT + 63) / 64; ++i) {
+    const int key = k0 + i * 64 + lane;
+    m.b[i] = mask && key < klen ? mask[key] : 0;
+  }
+}
+template <int KT>
+__device__ __forceinline__ KeyWords<KT> key_words(const MaskBytes<KT>& m, bool has_mask, int k0, int klen, int lane) {
+  KeyWords<KT> r;
+  if (!has_mask && k0 + KT <= klen) {
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) r.w[i] = 0xffffffffu;
+    return r;
+  }
+#pragma unroll
+  for (int i = 0; i < (KT + 63) / 64; ++i) {
+    const uint64_t w = __builtin_amdgcn_ballot_w64(k0 + i * 64 + lane < klen && m.b[i] == 0);
+    r.w[2 * i] = (uint32_t)w;
+    if (2 * i + 1 < KT / 32) r.w[2 * i + 1] = (uint32_t)(w >> 32);
+  }
+  return r;
+}
+template <int KT> __device__ __forceinline__ bool word_bit(const KeyWords<KT>& k, int row) {
+  uint32_t w = k.w[0];
+#pragma unroll
+  for (int i = 1; i < KT / 32; ++i) w = (row >> 5) == i ? k.w[i] : w;
+  return (w >> (row & 31)) & 1u;
+}
+
+// rows of keys per tile (shared-tile kernels) such that two tiles of K and V stay within 64 KB where two blocks per CU pay
+template <typename T, int DT> constexpr int key_tile() { return DT * sizeof(T) >= 512 ? 32 : 64; }
+
+// a block's share of the key tiles: split s of S takes tiles [s n / S, (s + 1) n / S) of the n that the item has
+__device__ __forceinline__ void tile_range(int n, int s, int S, int& t0, int& t1) {
+  t0 = (int)((int64_t)n * s / S);
+  t1 = (int)((int64_t)n * (s + 1) / S);
+}
+
+// ------------------------------------------------------------------------------------------------------------- forward
+// FEW = false: a block owns 128 rows (32 per wave) and walks key tiles that its waves share.
+// FEW = true (M <= 32): all waves hold the same 32 rows and a wave takes 32 of the tile's 128 keys -- every wave works where
+// a block of rows would leave three idle; the four partial softmaxes are joined through LDS.
+template <typename T, int DT, bool FEW>
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fwd_kernel(XArgs a) {
+  constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
+  constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
+  constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * NBUF * TILE + (FEW ? 1024 : 0)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  if (v < 0) return;
+  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int M = a.Lq * a.R;
+  const int klen = clamp_len(a.len, b, a.Lk), Mv = clamp_len(a.qlen, b, a.Lq) * a.R;
+  const int m0 = rt * (FEW ? 32 : 128), m = m0 + (FEW ? 0 : wave * 32) + li;
+  const int qi = m / a.R, head = g * a.R + m % a.R;
+  const bool live = m < Mv;
+  T* orow = reinterpret_cast<T*>(a.out) + b * a.ob + qi * a.ol + head * a.oh;
+  const int64_t prow = (int64_t)bg * M + m, prows = (int64_t)a.B * a.G * M;
+  float* pml = a.part ? a.part + prows * a.splits * a.D + (sp * prows + prow) * 2 : nullptr;
+  int t0, t1;
+  tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
+  if (m0 >= Mv || t0 >= t1) {                            // no live row, or no key in this share
+    if (FEW ? wave == 0 : true)
+      if (m < M) {
+        if (a.splits > 1) { if (lh == 0) { pml[0] = -INFINITY; pml[1] = 0.f; } }
+        else {
+          store_zero<T, DT>(orow, a.D, lh);
+          if (a.lse && lh == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = -INFINITY;
+        }
+      }
+    return;
+  }
+  const T* kbase = reinterpret_cast<const T*>(a.k) + b * a.kb + g * a.kh;
+  const T* vbase = reinterpret_cast<const T*>(a.v) + b * a.vb + g * a.vh;
+  const uint8_t* mask = a.mask ? a.mask + b * a.maskb : nullptr;
+  const int dbytes = a.D * (int)sizeof(T);
+  const int64_t klb = a.kl * (int64_t)sizeof(T), vlb = a.vl * (int64_t)sizeof(T);
+
+  MaskBytes<KT> mb;
+  mask_fetch(mb, mask, t0 * KT, klen, lane);
+  KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
+  auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
+    auto seen = [&](int row) { return word_bit(kw, row); };
+    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, dbytes, wave, lane, seen);
+    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, dbytes, wave, lane, seen);
+  };
+  fill(t0, 0, cur);
+  Frag<T, DT> qf;
+  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
+  mask_fetch(mb, mask, (t0 + 1) * KT, klen, lane);
+
+  f32x16 o[DT / 32];
+#pragma unroll
+  for (int i = 0; i < DT / 32; ++i) zero16(o[i]);
+  const float SC = a.scale * LOG2E;                      // scores in the log2 domain: p = exp2(SC s - SC m)
+  float mx = -INFINITY, l = 0.f;
+  wait_tiles();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = NBUF == 2 ? (t - t0) & 1 : 0;
+    if (t + 1 < t1) {
+      nxt = key_words(mb, mask != nullptr, (t + 1) * KT, klen, lane);
+      if (NBUF == 2) {
+        fill(t + 1, buf ^ 1, nxt);
+        mask_fetch(mb, mask, (t + 2) * KT, klen, lane);
+      }
+    }
+    if (!cur.none()) {
+      const char* tk = smem + buf * 2 * TILE;
+      const char* tv = tk + TILE;
+      f32x16 s[NB];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        const int blk = FEW ? wave : kb;
+        zero16(s[kb]);
+        mma_rows<T, DT>(s[kb], tk, blk, qf, li, lh);
+        uint32_t w = cur.w[FEW ? 0 : kb];
+        if (FEW) {
+#pragma unroll
+          for (int i = 1; i < KT / 32; ++i) w = wave == i ? cur.w[i] : w;
+        }
+        if (w != 0xffffffffu) {
+          const uint32_t wl = w >> (4 * lh);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] = (wl >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[kb][r] : -INFINITY;
+        }
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      // The maximum moves only when a tile exceeds it by more than 8 in the log2 domain (p <= 256 is harmless; o and l
+      // carry the same maximum): the rescaling of o leaves the common path.
+      const bool move = mt * SC > mx * SC + 8.f;
+      if (__builtin_amdgcn_ballot_w64(move) != 0) {
+        const float mn = move ? mt : mx;
+        const float al = mn == mx ? 1.f : __builtin_amdgcn_exp2f((mx - mn) * SC);
+        mx = mn;
+        l *= al;
+#pragma unroll
+        for (int i = 0; i < DT / 32; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= al;
+      }
+      const float off = mx == -INFINITY ? 0.f : -mx * SC;
+      float ls = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], SC, off));
+          ls += s[kb][r];
+        }
+      l += ls + __shfl_xor(ls, 32, 64);
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT>(o, tv, FEW ? wave : kb, s[kb], lane);
+    }
+    if (NBUF == 1 && t + 1 < t1) {
+      wait_tiles();                                      // every wave has read the tile: it may be overwritten
+      fill(t + 1, 0, nxt);
+      mask_fetch(mb, mask, (t + 2) * KT, klen, lane);
+    }
+    wait_tiles();
+    cur = nxt;
+  }
+  if (!live) {                                           // a row past the queries: as one that sees no key
+    mx = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT / 32; ++i) zero16(o[i]);
+  }
+  const float m2 = mx == -INFINITY ? -INFINITY : mx * SC;      // log2 domain
+  if constexpr (!FEW) {
+    if (m >= M) return;
+    if (a.splits > 1) {
+      store_row<float, DT>(a.part + (sp * prows + prow) * a.D, o, a.D, lh, 1.f);
+      if (lh == 0) { pml[0] = m2; pml[1] = l; }
+    } else {
+      store_row<T, DT>(orow, o, a.D, lh, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+      if (a.lse && lh == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
+    }
+  } else {
+    // join the four waves: ml[wave][32] = (max, sum), then o scaled to the common maximum, summed in wave order
+    float* ml = reinterpret_cast<float*>(smem + 2 * NBUF * TILE);
+    if (lh == 0) { ml[(wave * 32 + li) * 2] = m2; ml[(wave * 32 + li) * 2 + 1] = l; }
+    wait_tiles();
+    float mm = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + li) * 2]);
+    const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) lt += ml[(w * 32 + li) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + li) * 2] - base);
+    const float c = __builtin_amdgcn_exp2f(m2 - base);
+    // rows of DT + 4 floats: a half wave's 32 rows start 4 banks apart
+    float* so = reinterpret_cast<float*>(smem);
+    constexpr int LDO = DT + 4;
+    static_assert(32 * LDO * 4 <= 2 * NBUF * TILE, "");
+    for (int w = 0; w < 4; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int dt = 0; dt < DT / 32; ++dt)
+#pragma unroll
+          for (int gq = 0; gq < 4; ++gq) {
+            float4* p = reinterpret_cast<float4*>(so + li * LDO + dt * 32 + gq * 8 + lh * 4);
+            float4 x = make_float4(o[dt][gq * 4] * c, o[dt][gq * 4 + 1] * c, o[dt][gq * 4 + 2] * c, o[dt][gq * 4 + 3] * c);
+            if (w) { const float4 y = *p; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
+            *p = x;
+          }
+      }
+      wait_tiles();
+    }
+    if (wave == 0 && lh == 0 && m < M) {
+      if (a.splits > 1) { pml[0] = mm; pml[1] = lt; }
+      else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = lt == 0.f ? -INFINITY : (mm + log2f(lt)) * LN2;
+    }
+    if (wave == 0 && lh == 0) ml[li] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+    wait_tiles();
+    for (int i = tid; i < 32 * (DT / 4); i += 256) {
+      const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
+      if (mr >= M || d >= a.D) continue;
+      const float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
+      if (a.splits > 1) {
+        *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
+      } else {
+        const float cl = ml[r];
+        T* p = reinterpret_cast<T*>(a.out) + b * a.ob + (mr / a.R) * a.ol + (g * a.R + mr % a.R) * a.oh + d;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x.x * cl, x.y * cl), cvt_pk_bf16_rne(x.z * cl, x.w * cl));
+        else *reinterpret_cast<float4*>(p) = make_float4(x.x * cl, x.y * cl, x.z * cl, x.w * cl);
+      }
+    }
+  }
+}
+
+// Join the splits of a forward launch: a wave per row.  Splits are added in order; an empty split has max = -inf, sum = 0 and its
+// partial row is not read (it is not written either).
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int M = a.Lq * a.R;
+  const int64_t rows = (int64_t)a.B * a.G * M, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int bg = (int)(row / M), m = (int)(row % M), g = bg % a.G, b = bg / a.G, qi = m / a.R, head = g * a.R + m % a.R;
+  const float* ml = a.part + rows * a.splits * a.D;
+  float mm = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) mm = fmaxf(mm, ml[(s * rows + row) * 2]);
+  mm = wave_max(mm);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float l = 0.f, x = 0.f, y = 0.f;
+  const int d = lane * 2;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 q = *reinterpret_cast<const float2*>(ml + (s * rows + row) * 2);
+    const float c = __builtin_amdgcn_exp2f(q.x - base);
+    l += c * q.y;
+    if (q.x != -INFINITY && d < a.D) {
+      const float2 p = *reinterpret_cast<const float2*>(a.part + (s * rows + row) * a.D + d);
+      x = fmaf(c, p.x, x);
+      y = fmaf(c, p.y, y);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (d < a.D) {
+    T* p = reinterpret_cast<T*>(a.out) + b * a.ob + qi * a.ol + head * a.oh + d;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = cvt_pk_bf16_rne(x * inv, y * inv);
+    else *reinterpret_cast<float2*>(p) = make_float2(x * inv, y * inv);
+  }
+  if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (mm + log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------------------- dQ (and delta)
+// Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
+template <typename T, int DT, bool FEW>
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq_kernel(XArgs a) {
+  constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
+  constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
+  constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * NBUF * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  if (v < 0) return;
+  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int M = a.Lq * a.R;
+  const int klen = clamp_len(a.len, b, a.Lk), Mv = clamp_len(a.qlen, b, a.Lq) * a.R;
+  const int m0 = rt * (FEW ? 32 : 128), m = m0 + (FEW ? 0 : wave * 32) + li;
+  const int qi = m / a.R, head = g * a.R + m % a.R;
+  const bool live = m < Mv;
+  T* dqrow = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + qi) * a.H + head) * a.D;
+  const int64_t prow = (int64_t)bg * M + m, prows = (int64_t)a.B * a.G * M;
+  const int64_t srow = ((int64_t)b * a.H + head) * a.Lq + qi;
+  Frag<T, DT> qf, dof;
+  float dl = 0.f, lse2 = INFINITY;
+  load_frag<T, DT>(dof, reinterpret_cast<const T*>(a.dout) + b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
+  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.o) + b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
+  dl = frag_dot<DT>(qf, dof);
+  dl += __shfl_xor(dl, 32, 64);
+  if (live) {
+    const float x = a.lse[srow];
+    lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
+  }
+  if (sp == 0 && m < M && lh == 0 && (!FEW || wave == 0)) a.delta[srow] = dl;
+  int t0, t1;
+  tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
+  if (m0 >= Mv || t0 >= t1) {
+    if (m < M && (!FEW || wave == 0)) {
+      if (a.splits > 1) store_zero<float, DT>(a.part + (sp * prows + prow) * a.D, a.D, lh);
+      else store_zero<T, DT>(dqrow, a.D, lh);
+    }
+    return;
+  }
+  const T* kbase = reinterpret_cast<const T*>(a.k) + b * a.kb + g * a.kh;
+  const T* vbase = reinterpret_cast<const T*>(a.v) + b * a.vb + g * a.vh;
+  const uint8_t* mask = a.mask ? a.mask + b * a.maskb : nullptr;
+  const int dbytes = a.D * (int)sizeof(T);
+  const int64_t klb = a.kl * (int64_t)sizeof(T), vlb = a.vl * (int64_t)sizeof(T);
+  MaskBytes<KT> mb;
+  mask_fetch(mb, mask, t0 * KT, klen, lane);
+  KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
+  auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
+    auto seen = [&](int row) { return word_bit(kw, row); };
+    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, dbytes, wave, lane, seen);
+    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, dbytes, wave, lane, seen);
+  };
+  fill(t0, 0, cur);
+  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
+  mask_fetch(mb, mask, (t0 + 1) * KT, klen, lane);
+  f32x16 dq[DT / 32];
+#pragma unroll
+  for (int i = 0; i < DT / 32; ++i) zero16(dq[i]);
+  const float SC = a.scale * LOG2E;
+  wait_tiles();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = NBUF == 2 ? (t - t0) & 1 : 0;
+    if (t + 1 < t1) {
+      nxt = key_words(mb, mask != nullptr, (t + 1) * KT, klen, lane);
+      if (NBUF == 2) {
+        fill(t + 1, buf ^ 1, nxt);
+        mask_fetch(mb, mask, (t + 2) * KT, klen, lane);
+      }
+    }
+    const char* tk = smem + buf * 2 * TILE;
+    const char* tv = tk + TILE;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+      const int blk = FEW ? wave : kb;
+      uint32_t w = cur.w[FEW ? 0 : kb];
+      if (FEW) {
+#pragma unroll
+        for (int i = 1; i < KT / 32; ++i) w = wave == i ? cur.w[i] : w;
+      }
+      if (w == 0) continue;
+      f32x16 s, dp;
+      zero16(s);
+      zero16(dp);
+      mma_rows<T, DT>(s, tk, blk, qf, li, lh);
+      mma_rows<T, DT>(dp, tv, blk, dof, li, lh);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * (dp[r] - dl);
+      if (w != 0xffffffffu) {
+        const uint32_t wl = w >> (4 * lh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (wl >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[r] : 0.f;
+      }
+      mma_cols<T, DT>(dq, tk, blk, s, lane);
+    }
+    if (NBUF == 1 && t + 1 < t1) {
+      wait_tiles();
+      fill(t + 1, 0, nxt);
+      mask_fetch(mb, mask, (t + 2) * KT, klen, lane);
+    }
+    wait_tiles();
+    cur = nxt;
+  }
+  if constexpr (!FEW) {
+    if (m >= M) return;
+    if (a.splits > 1) store_row<float, DT>(a.part + (sp * prows + prow) * a.D, dq, a.D, lh, a.scale);
+    else store_row<T, DT>(dqrow, dq, a.D, lh, a.scale);
+  } else {
+    float* so = reinterpret_cast<float*>(smem);
+    constexpr int LDO = DT + 4;
+    static_assert(32 * LDO * 4 <= 2 * NBUF * TILE, "");
+    for (int w = 0; w < 4; ++w) {                        // sums of the four waves, in wave order
+      if (wave == w) {
+#pragma unroll
+        for (int dt = 0; dt < DT / 32; ++dt)
+#pragma unroll
+          for (int gq = 0; gq < 4; ++gq) {
+            float4* p = reinterpret_cast<float4*>(so + li * LDO + dt * 32 + gq * 8 + lh * 4);
+            float4 x = make_float4(dq[dt][gq * 4], dq[dt][gq * 4 + 1], dq[dt][gq * 4 + 2], dq[dt][gq * 4 + 3]);
+            if (w) { const float4 y = *p; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
+            *p = x;
+          }
+      }
+      wait_tiles();
+    }
+    for (int i = tid; i < 32 * (DT / 4); i += 256) {
+      const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
+      if (mr >= M || d >= a.D) continue;
+      float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
+      x.x *= a.scale; x.y *= a.scale; x.z *= a.scale; x.w *= a.scale;
+      if (a.splits > 1) *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
+      else {
+        T* p = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + mr / a.R) * a.H + g * a.R + mr % a.R) * a.D + d;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x.x, x.y), cvt_pk_bf16_rne(x.z, x.w));
+        else *reinterpret_cast<float4*>(p) = x;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- dK, dV
+// A block owns 128 keys (32 per wave, a lane one key: its K and V rows stay in registers) and walks tiles of query rows, head
+// after head of the group.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen
+// key computes stays in its own lane; zeros are stored for it.
+template <typename T, int DT> constexpr int row_tile() { return DT * sizeof(T) >= 256 ? 32 : 64; }
+template <typename T, int DT>
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dkv_kernel(XArgs a) {
+  constexpr int RB = DT * sizeof(T), RT = row_tile<T, DT>(), TILE = RT * RB;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  if (v < 0) return;
+  const int kt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int klen = clamp_len(a.len, b, a.Lk), qv = clamp_len(a.qlen, b, a.Lq);
+  const int key = kt * 128 + wave * 32 + li;
+  const bool seen = key < klen && !(a.mask && a.mask[b * a.maskb + key]);
+  const int64_t krow = ((int64_t)b * a.Lk + key) * a.G + g, krows = (int64_t)a.B * a.Lk * a.G;
+  const int nt = (qv + RT - 1) / RT, total = nt * a.R;
+  int t0, t1;
+  tile_range(total, sp, a.splits, t0, t1);
+  if (kt * 128 >= klen || t0 >= t1) {
+    if (key < a.Lk) {
+      if (a.splits > 1) {
+        store_zero<float, DT>(a.part + (sp * 2 * krows + krow) * a.D, a.D, lh);
+        store_zero<float, DT>(a.part + ((sp * 2 + 1) * krows + krow) * a.D, a.D, lh);
+      } else {
+        store_zero<T, DT>(reinterpret_cast<T*>(a.dk) + krow * a.D, a.D, lh);
+        store_zero<T, DT>(reinterpret_cast<T*>(a.dv) + krow * a.D, a.D, lh);
+      }
+    }
+    return;
+  }
+  const int dbytes = a.D * (int)sizeof(T);
+  const int64_t qlb = a.ql * (int64_t)sizeof(T), glb = a.gl * (int64_t)sizeof(T);
+  float* stat = reinterpret_cast<float*>(smem + 4 * TILE);         // [buf][lse2 | delta][RT]
+  float sreg = 0.f;
+  auto fill = [&](int t, int buf) {
+    const int r = t / nt, q0 = (t - r * nt) * RT, head = g * a.R + r;
+    auto ok = [&](int row) { return q0 + row < qv; };
+    dma_tile<RB, RT, 4>(smem, buf * 2 * TILE, reinterpret_cast<const T*>(a.q) + b * a.qb + (int64_t)q0 * a.ql + head * a.qh, qlb, dbytes, wave, lane, ok);
+    dma_tile<RB, RT, 4>(smem, buf * 2 * TILE + TILE, reinterpret_cast<const T*>(a.dout) + b * a.gb + (int64_t)q0 * a.gl + head * a.gh, glb, dbytes, wave, lane, ok);
+    if (tid < 2 * RT) {
+      const int q = q0 + tid % RT;
+      const int64_t s = ((int64_t)b * a.H + head) * a.Lq + q;
+      sreg = tid < RT ? INFINITY : 0.f;                             // rows past the queries: P = exp2(s - inf) = 0
+      if (q < qv) {
+        sreg = tid < RT ? a.lse[s] * LOG2E : a.delta[s];
+        if (tid < RT && sreg == -INFINITY) sreg = INFINITY;
+      }
+    }
+  };
+  auto put_stat = [&](int buf) { if (tid < 2 * RT) stat[buf * 2 * RT + tid] = sreg; };
+  fill(t0, 0);
+  Frag<T, DT> kf, vf;
+  load_frag<T, DT>(kf, reinterpret_cast<const T*>(a.k) + b * a.kb + (int64_t)key * a.kl + g * a.kh, a.D, lh, seen);
+  load_frag<T, DT>(vf, reinterpret_cast<const T*>(a.v) + b * a.vb + (int64_t)key * a.vl + g * a.vh, a.D, lh, seen);
+  f32x16 dk[DT / 32], dv[DT / 32];
+#pragma unroll
+  for (int i = 0; i < DT / 32; ++i) { zero16(dk[i]); zero16(dv[i]); }
+  const float SC = a.scale * LOG2E;
+  put_stat(0);
+  wait_tiles();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) fill(t + 1, buf ^ 1);
+    const char* tq = smem + buf * 2 * TILE;
+    const char* tg = tq + TILE;
+    const float* st = stat + buf * 2 * RT;
+#pragma unroll
+    for (int blk = 0; blk < RT / 32; ++blk) {
+      f32x16 s, dp;
+      zero16(s);
+      zero16(dp);
+      mma_rows<T, DT>(s, tq, blk, kf, li, lh);
+      mma_rows<T, DT>(dp, tg, blk, vf, li, lh);
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const float4 L = *reinterpret_cast<const float4*>(st + blk * 32 + gq * 8 + lh * 4);
+        const float4 E = *reinterpret_cast<const float4*>(st + RT + blk * 32 + gq * 8 + lh * 4);
+        const float ls[4] = {L.x, L.y, L.z, L.w}, de[4] = {E.x, E.y, E.z, E.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = gq * 4 + e;
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -ls[e]));
+          dp[r] = s[r] * (dp[r] - de[e]);
+        }
+      }
+      mma_cols<T, DT>(dv, tg, blk, s, lane);
+      mma_cols<T, DT>(dk, tq, blk, dp, lane);
+    }
+    if (t + 1 < t1) put_stat(buf ^ 1);
+    wait_tiles();
+  }
+  if (key >= a.Lk) return;
+  if (a.splits > 1) {
+    float* pk = a.part + (sp * 2 * krows + krow) * a.D;
+    float* pv = a.part + ((sp * 2 + 1) * krows + krow) * a.D;
+    if (seen) { store_row<float, DT>(pk, dk, a.D, lh, a.scale); store_row<float, DT>(pv, dv, a.D, lh, 1.f); }
+    else { store_zero<float, DT>(pk, a.D, lh); store_zero<float, DT>(pv, a.D, lh); }
+  } else {
+    T* pk = reinterpret_cast<T*>(a.dk) + krow * a.D;
+    T* pv = reinterpret_cast<T*>(a.dv) + krow * a.D;
+    if (seen) { store_row<T, DT>(pk, dk, a.D, lh, a.scale); store_row<T, DT>(pv, dv, a.D, lh, 1.f); }
+    else { store_zero<T, DT>(pk, a.D, lh); store_zero<T, DT>(pv, a.D, lh); }
+  }
+}
+
+// Sum the splits of a gradient in order.  dq partials are in (item, key head, q, r) row order, dk / dv partials in output order.
+template <typename T, bool DQ>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a) {
+  const int d4 = a.D / 4, M = a.Lq * a.R;
+  const int64_t rows = DQ ? (int64_t)a.B * a.G * M : 2 * (int64_t)a.B * a.Lk * a.G;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * d4) return;
+  const int64_t row = i / d4;
+  const int d = (int)(i % d4) * 4;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 y = *reinterpret_cast<const float4*>(a.part + (s * rows + row) * a.D + d);
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
+  T* p;
+  if (DQ) {
+    const int bg = (int)(row / M), m = (int)(row % M), g = bg % a.G, b = bg / a.G;
+    p = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + m / a.R) * a.H + g * a.R + m % a.R) * a.D + d;
+  } else {
+    const int64_t half = rows / 2;
+    p = (row < half ? reinterpret_cast<T*>(a.dk) + row * a.D : reinterpret_cast<T*>(a.dv) + (row - half) * a.D) + d;
+  }
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x.x, x.y), cvt_pk_bf16_rne(x.z, x.w));
+  else *reinterpret_cast<float4*>(p) = x;
+}
+
+constexpr int MAX_SPLITS = 64;
+// How many shares of a long axis (n tiles) give the launch about `want` blocks, each with at least `least` tiles.
+int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
+  int64_t s = (want + blocks - 1) / blocks;
+  const int64_t most = n / least;
+  if (s > most) s = most;
+  if (s > MAX_SPLITS) s = MAX_SPLITS;
+  return s < 1 ? 1 : (int)s;
+}
+struct Plan { bool few; int nrt, fwd, dq, nkt, dkv; };
+Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
+  Plan p;
+  const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
+  const int rb = (D <= 32 ? 32 : D <= 64 ? 64 : 128) * (bf16 ? 2 : 4);
+  p.few = M <= 32;
+  p.nrt = (int)(p.few ? 1 : (M + 127) / 128);
+  const int KT = p.few ? 128 : (rb >= 512 ? 32 : 64);
+  const int64_t kt = (Lk + KT - 1) / KT;
+  p.fwd = split_count(BG * p.nrt, kt, 512, 2);
+  p.dq = split_count(BG * p.nrt, kt, 512, 4);
+  p.nkt = (Lk + 127) / 128;
+  const int RT = rb >= 256 ? 32 : 64;
+  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), 512, 8);
+  return p;
+}
+
+dim3 grid8(int64_t blocks) { return dim3((unsigned)((blocks + 7) / 8 * 8)); }
+
+template <typename T, int DT>
+void launch_fwd(const XArgs& a, bool few, hipStream_t st) {
+  const dim3 g = grid8((int64_t)a.nrt * a.splits * a.G * a.B);
+  if (few) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, true>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, false>), g, dim3(256), 0, st, a);
+}
+template <typename T, int DT>
+void launch_dq(const XArgs& a, bool few, hipStream_t st) {
+  const dim3 g = grid8((int64_t)a.nrt * a.splits * a.G * a.B);
+  if (few) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, true>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, false>), g, dim3(256), 0, st, a);
+}
+template <typename T, int DT>
+void launch_dkv(const XArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((xattn_dkv_kernel<T, DT>), grid8((int64_t)a.nrt * a.splits * a.G * a.B), dim3(256), 0, st, a);
+}
+#define BY_WIDTH(T, CALL)              \
+  do {                                 \
+    if (a.D <= 32) { CALL(T, 32); }    \
+    else if (a.D <= 64) { CALL(T, 64); } \
+    else { CALL(T, 128); }             \
+  } while (0)
+
+int check(const styler_xattn_t* x, bool bwd) {
+  if (!x || !x->q || !x->k || !x->v || !x->out) return STYLER_EINVAL;
+  if (x->B < 1 || x->Lq < 1 || x->Lk < 1 || x->H < 1 || x->G < 1 || x->H % x->G || x->D < 8 || x->D > 128 || x->D % 8) return STYLER_EINVAL;
+  if (!(x->scale > 0.f) || x->scale > 3e38f) return STYLER_EINVAL;
+  if ((int64_t)x->Lq * (x->H / x->G) > (1 << 30) || (int64_t)x->Lk > (1 << 30)) return STYLER_EINVAL;
+  const int es = x->bf16 ? 2 : 4, e16 = 16 / es;
+  const int64_t st[] = {x->qb, x->ql, x->qh, x->kb, x->kl, x->kh, x->vb, x->vl, x->vh, x->ob, x->ol, x->oh, x->gb, x->gl, x->gh};
+  for (int i = 0; i < (bwd ? 15 : 12); ++i)
+    if (st[i] < 0 || st[i] % e16) return STYLER_EALIGN;
+  // a tile's rows (128 at most) are addressed with 32-bit byte offsets from the tile's base
+  const int64_t rows[] = {x->ql, x->kl, x->vl, bwd ? x->gl : 0};
+  for (int64_t r : rows) if (r * es >= (1 << 23)) return STYLER_EINVAL;
+  const void* p[] = {x->q, x->k, x->v, x->out, bwd ? x->dout : nullptr, bwd ? x->dq : nullptr, bwd ? x->dk : nullptr, bwd ? x->dv : nullptr};
+  for (const void* q : p) if ((uintptr_t)q & 15) return STYLER_EALIGN;
+  if (bwd && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse)) return STYLER_EINVAL;
+  const Plan pl = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  const int64_t bg = (int64_t)x->B * x->G;
+  if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0x7ffffff0 || bg * pl.nkt * pl.dkv > 0x7ffffff0) return STYLER_EINVAL;
+  return 0;
+}
+XArgs args(const styler_xattn_t* x) {
+  XArgs a = {};
+  a.q = x->q; a.k = x->k; a.v = x->v; a.o = x->out; a.out = x->out; a.dout = x->dout; a.dq = x->dq; a.dk = x->dk; a.dv = x->dv;
+  a.lse = x->lse; a.len = x->len; a.qlen = x->q_len; a.mask = x->mask; a.maskb = x->maskb;
+  a.qb = x->qb; a.ql = x->ql; a.qh = x->qh; a.kb = x->kb; a.kl = x->kl; a.kh = x->kh; a.vb = x->vb; a.vl = x->vl; a.vh = x->vh;
+  a.ob = x->ob; a.ol = x->ol; a.oh = x->oh; a.gb = x->gb; a.gl = x->gl; a.gh = x->gh;
+  a.B = x->B; a.Lq = x->Lq; a.Lk = x->Lk; a.H = x->H; a.G = x->G; a.R = x->H / x->G; a.D = x->D; a.scale = x->scale;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int bwd) {
+  if (B < 1 || Lq < 1 || Lk < 1 || G < 1 || H < G || H % G || D < 8 || D > 128) return 0;
+  const Plan p = make_plan(B, Lq, Lk, H, G, D, bf16);
+  const int64_t qrows = (int64_t)B * H * Lq, krows = (int64_t)B * G * Lk;
+  if (!bwd) return p.fwd > 1 ? 4 * p.fwd * qrows * (D + 2) : 0;
+  int64_t part = p.dq > 1 ? p.dq * qrows * D : 0;
+  const int64_t kv = p.dkv > 1 ? 2 * p.dkv * krows * D : 0;
+  if (kv > part) part = kv;                              // the two gradients' launches follow each other: one buffer
+  return 4 * (part + (qrows + 3) / 4 * 4);
+}
+
+extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check(x, false)) return rc;
+  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, 0);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return STYLER_EINVAL;
+  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  hipStream_t st = (hipStream_t)stream;
+  XArgs a = args(x);
+  a.nrt = p.nrt; a.splits = p.fwd; a.part = p.fwd > 1 ? (float*)workspace : nullptr;
+#define FWD(T, W) launch_fwd<T, W>(a, p.few, st)
+  if (x->bf16) BY_WIDTH(uint16_t, FWD); else BY_WIDTH(float, FWD);
+#undef FWD
+  if (p.fwd > 1) {
+    const unsigned blocks = (unsigned)(((int64_t)x->B * x->H * x->Lq + 3) / 4);
+    if (x->bf16) hipLaunchKernelGGL((xattn_join_kernel<uint16_t>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((xattn_join_kernel<float>), dim3(blocks), dim3(256), 0, st, a);
+  }
+  return launch_status();
+}
+
+extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check(x, true)) return rc;
+  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, 1);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return STYLER_EINVAL;
+  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  hipStream_t st = (hipStream_t)stream;
+  XArgs a = args(x);
+  const int64_t qrows = (int64_t)x->B * x->H * x->Lq, krows = (int64_t)x->B * x->G * x->Lk;
+  a.delta = (float*)workspace;
+  a.part = (float*)workspace + (qrows + 3) / 4 * 4;
+  a.nrt = p.nrt; a.splits = p.dq;
+#define DQ(T, W) launch_dq<T, W>(a, p.few, st)
+  if (x->bf16) BY_WIDTH(uint16_t, DQ); else BY_WIDTH(float, DQ);
+#undef DQ
+  if (p.dq > 1) {
+    const unsigned blocks = (unsigned)((qrows * (x->D / 4) + 255) / 256);
+    if (x->bf16) hipLaunchKernelGGL((xattn_sum_kernel<uint16_t, true>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((xattn_sum_kernel<float, true>), dim3(blocks), dim3(256), 0, st, a);
+  }
+  a.nrt = p.nkt; a.splits = p.dkv;
+#define DKV(T, W) launch_dkv<T, W>(a, st)
+  if (x->bf16) BY_WIDTH(uint16_t, DKV); else BY_WIDTH(float, DKV);
+#undef DKV
+  if (p.dkv > 1) {
+    const unsigned blocks = (unsigned)((2 * krows * (x->D / 4) + 255) / 256);
+    if (x->bf16) hipLaunchKernelGGL((xattn_sum_kernel<uint16_t, false>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((xattn_sum_kernel<float, false>), dim3(blocks), dim3(256), 0, st, a);
+  }
+  return launch_status();
+}

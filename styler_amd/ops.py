@@ -4,14 +4,18 @@ PyTorch supplies device memory (caching allocator), the current HIP stream and n
 function here hands raw device pointers + sizes to libstyler_hip.so.  Activations are fp32
 channels-last [B, L, C]; a channel slice `x[..., a:b]` of a wider buffer is a legal argument (the row
 stride travels as `ld`), which is how torch.cat / torch.split copies of the reference disappear."""
+import contextlib
+import ctypes
+import math
 import os
 
 import torch
 
-from ._lib import lib
+from ._lib import GnArgs, XattnArgs, lib
 
 ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
 ACT_LEAKY = 4                      # leaky_relu(0.1), the vocoder's LRELU_SLOPE
+ACT_SILU, ACT_GELU = 6, 7          # groupnorm_act only (GELU: the erf form)
 PREC_F32, PREC_BF16 = 0, 1
 PREC_BF16X3 = 2                    # host-level arithmetic: fp32-class products as three bf16 MFMA products (split3 / lo_part)
 
@@ -1860,3 +1864,282 @@ def adam_step(p, g, m, v, sumsq_buf, max_norm, lr, beta1, beta2, eps, step, grad
     _chk(lib.styler_adam_step(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), _ptr(sumsq_buf),
                               float(max_norm), float(lr), float(beta1), float(beta2), float(eps), int(step),
                               float(grad_scale), _stream()), "styler_adam_step")
+
+
+# ---- operators of a decoder block that reads an encoder's states: group norm + activation, rotary positions, cross attention --------
+# fp32 or bf16 tensors with their own strides; what a kernel cannot read in place (features not contiguous, rows not on 16 bytes) is
+# copied first.  They run on the current stream of the tensors' device, whichever device is current.
+_ON_CURRENT = contextlib.nullcontext()
+
+
+def _refuse(name, what):
+    raise StylerHipError(f"{name}: {what}")
+
+
+def _on(t):
+    """Makes t's device the current one for the launches and allocations inside."""
+    return _ON_CURRENT if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _like(name, t, what, shape, dtype, device):
+    """`t` is a tensor of this shape, type and device."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        _refuse(name, f"{what} must be {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _vector(name, t, what, n, dtype, device):
+    return None if t is None else _like(name, t, what, (n,), dtype, device).contiguous()
+
+
+def _main_type(name, t):
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        _refuse(name, f"float32 or bfloat16 expected, got {t.dtype}")
+    return 1 if t.dtype == torch.bfloat16 else 0
+
+
+def _on_gpu(name, t):
+    if not t.is_cuda:
+        _refuse(name, "there is no CPU form")
+
+
+def _stride(t, i):
+    return t.stride(i) if t.shape[i] > 1 else 0
+
+
+def _heads(t):
+    """[B, L, H, D] as the attention kernels read it: features contiguous, rows on 16 bytes, a tile's rows within 2^31 bytes."""
+    es = t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and _stride(t, 1) * es < 1 << 23 and \
+            all(_stride(t, i) * es % 16 == 0 for i in range(3)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale):
+    bf16 = _main_type(name, q)
+    if q.dim() != 4 or k.dim() != 4:
+        _refuse(name, "q [B, Lq, H, D] and k, v [B, Lk, G, D] expected")
+    B, Lq, H, D = q.shape
+    Lk, G = k.shape[1], k.shape[2]
+    _like(name, k, "k", (B, Lk, G, D), q.dtype, q.device)
+    _like(name, v, "v", (B, Lk, G, D), q.dtype, q.device)
+    if G < 1 or H < 1 or H % G:
+        _refuse(name, f"the query heads ({H}) must be a multiple of the key heads ({G})")
+    if D % 8 or not 8 <= D <= 128:
+        _refuse(name, f"head width {D}: a multiple of 8 up to 128 expected")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        _refuse(name, f"scale {scale}: a positive finite number expected")
+    lens = _vector(name, lens, "lens", B, torch.int64, q.device)
+    q_lens = _vector(name, q_lens, "q_lens", B, torch.int64, q.device)
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.device != q.device or mask.dim() != 2 or mask.shape[0] not in (1, B) or mask.shape[1] != Lk:
+            _refuse(name, f"mask must be bool [{B} or 1, {Lk}] on {q.device} (True: a key that is not seen)")
+        if Lk > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+    _like(name, out, "out", (B, Lq, H, D), q.dtype, q.device)
+    if lse is not None and not _like(name, lse, "lse", (B, H, Lq), torch.float32, q.device).is_contiguous():
+        _refuse(name, "lse must be contiguous")
+    _on_gpu(name, q)
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    a = XattnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, _ptr(lse), _ptr(lens),
+                  _ptr(q_lens), _ptr(mask),
+                  _stride(q, 0), _stride(q, 1), _stride(q, 2), _stride(k, 0), _stride(k, 1), _stride(k, 2),
+                  _stride(v, 0), _stride(v, 1), _stride(v, 2), _stride(out, 0), _stride(out, 1), _stride(out, 2), 0, 0, 0,
+                  0 if mask is None or mask.shape[0] == 1 else mask.stride(0), B, Lq, Lk, H, G, D, bf16, scale)
+    return a, (q, k, v, lens, q_lens, mask)              # (the second: what must outlive the launch's enqueueing)
+
+
+def _workspace(n, device):
+    return torch.empty(n, device=device, dtype=torch.uint8) if n else None
+
+
+def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, out=None, lse=None):
+    """softmax(scale q k^T) v of queries q [B, Lq, H, D] over the keys and values k, v [B, Lk, G, D] of another sequence; head h
+    reads key head h // (H // G).  fp32 or bf16 (all alike), D a multiple of 8 up to 128, scale 1 / sqrt(D) unless given.
+
+    lens int64 [B]: keys at or past it are not seen; mask bool [B or 1, Lk]: True = not seen.  What stands in rows that are not
+    seen is never used.  q_lens int64 [B]: queries at or past it, like queries that see no key, give zeros and lse = -inf.
+    lse (optional, fp32 [B, H, Lq]) receives the logarithm of the softmax's denominator, which cross_attention_bwd needs."""
+    name = "cross_attention"
+    if q.dim() != 4:
+        _refuse(name, "q [B, Lq, H, D] expected")
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    elif out.dim() != 4 or out.stride(3) != 1 or _heads(out) is not out or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(4)):
+        _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
+    a, keep = _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale)
+    if out.numel() == 0 or a.Lk == 0:
+        if lse is not None:
+            lse.fill_(-math.inf)
+        return out.zero_()
+    with _on(q):
+        n = lib.styler_cross_attention_workspace_bytes(a.B, a.Lq, a.Lk, a.H, a.G, a.D, a.bf16, 0)
+        ws = _workspace(n, q.device)
+        _chk(lib.styler_cross_attention(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_cross_attention")
+    return out
+
+
+def cross_attention_bwd(q, k, v, out, dout, lse, lens=None, *, q_lens=None, mask=None, scale=None):
+    """-> (dq, dk, dv) of cross_attention from its out and lse and the gradient dout of out.  The gradients are contiguous, in the
+    inputs' type; dk and dv sum over the query heads that share a key head.  Zero for keys that are not seen and for queries past
+    q_lens.  Deterministic."""
+    name = "cross_attention_bwd"
+    if lse is None:
+        _refuse(name, "the forward's lse is needed")
+    if out.dim() != 4 or q.dim() != 4:
+        _refuse(name, "q and out [B, Lq, H, D] expected")
+    _like(name, dout, "dout", q.shape, q.dtype, q.device)
+    out, dout, lse = _heads(out), _heads(dout), lse.contiguous()
+    a, keep = _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale)
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.gb, a.gl, a.gh = _stride(dout, 0), _stride(dout, 1), _stride(dout, 2)
+    with _on(q):
+        n = lib.styler_cross_attention_workspace_bytes(a.B, a.Lq, a.Lk, a.H, a.G, a.D, a.bf16, 1)
+        ws = _workspace(n, q.device)
+        _chk(lib.styler_cross_attention_bwd(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_cross_attention_bwd")
+    return dq, dk, dv
+
+
+def rotary_freqs(dim, device, *, base=10000.0, scaling=None, factor=1.0, orig_len=None, low=1.0, high=4.0):
+    """The angles per position of the dim / 2 pairs of `rotary`, float64 [dim / 2]: base^(-2 i / dim), for long contexts scaled by
+    scaling = "linear": every angle / factor (positions interpolated); "base": the base raised by factor^(dim / (dim - 2)) (the
+    slowest pair / factor, the fastest kept); "bands": pairs that turn less than `low` times over orig_len / factor, those that turn
+    more than `high` times kept, linear in between."""
+    name = "rotary_freqs"
+    if dim < 2 or dim % 2:
+        _refuse(name, f"dim {dim}: an even number expected")
+    if not (base > 1.0 and factor > 0.0 and math.isfinite(base) and math.isfinite(factor)):
+        _refuse(name, f"base {base} > 1 and factor {factor} > 0 expected")
+    if scaling not in (None, "linear", "base", "bands"):
+        _refuse(name, f"scaling {scaling!r}: None, 'linear', 'base' or 'bands' expected")
+    if scaling == "bands" and (orig_len is None or orig_len < 1 or not 0.0 <= low < high):
+        _refuse(name, "'bands' needs orig_len and 0 <= low < high")
+    if scaling == "base" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "bands":
+        keep = ((orig_len * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = (1 - keep) * f / factor + keep * f
+    return f.to(device)
+
+
+def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, out=None):
+    """x [B, L, H, D] (fp32 or bf16, any strides: the query and key heads of a fused projection's rows) with the first
+    2 len(freqs) features of every head turned by pos * freqs (rotary_freqs), times gain; the features behind them pass through.
+    Pair i is (2 i, 2 i + 1) if interleaved, else (i, i + len(freqs)).  pos: int64 or fp32 (fractional positions), [L] or
+    [B or 1, L]; None: 0 .. L - 1.  Angles are formed in 64 bits.  inverse: the opposite turn, i.e. dx from dy.
+    out (optional): the result's tensor; out=x works in place, any other overlap with x does not."""
+    name = "rotary"
+    bf16 = _main_type(name, x)
+    if x.dim() != 4:
+        _refuse(name, "x [B, L, H, D] expected")
+    B, L, H, D = x.shape
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != x.device or not 2 <= 2 * freqs.numel() <= D:
+        _refuse(name, f"freqs must be float64 [up to {D // 2}] on {x.device}")
+    freqs = freqs.contiguous()
+    kind, posb = 0, 0
+    if pos is not None:
+        if pos.dtype not in (torch.int64, torch.float32) or pos.device != x.device or pos.dim() not in (1, 2) or \
+                pos.shape[-1] != L or (pos.dim() == 2 and pos.shape[0] not in (1, B)):
+            _refuse(name, f"pos must be int64 or float32 [{L}] or [{B} or 1, {L}] on {x.device}")
+        if L > 1 and pos.stride(-1) != 1:
+            pos = pos.contiguous()
+        kind = 1 if pos.dtype == torch.int64 else 2
+        posb = pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else 0
+    if not math.isfinite(gain):
+        _refuse(name, f"gain {gain}: a finite number expected")
+    if out is not None:
+        _like(name, out, "out", x.shape, x.dtype, x.device)
+        if out.stride(3) != 1 or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(3)):
+            _refuse(name, "out must have contiguous features and distinct rows")
+    _on_gpu(name, x)
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if x.numel() == 0:
+        return out
+    with _on(x):
+        _chk(lib.styler_rotary(x.data_ptr(), _stride(x, 0), _stride(x, 1), _stride(x, 2), out.data_ptr(), _stride(out, 0),
+                               _stride(out, 1), _stride(out, 2), freqs.data_ptr(), _ptr(pos), posb, kind, B, L, H, D,
+                               2 * freqs.numel(), 1 if interleaved else 0, 1 if inverse else 0, float(gain), bf16, _stream()),
+             "styler_rotary")
+    return out
+
+
+def _gn_args(name, x, gamma, beta, groups, act, eps, lens, stats):
+    bf16 = _main_type(name, x)
+    if x.dim() != 3:
+        _refuse(name, "x [B, L, C] expected")
+    B, L, C = x.shape
+    if groups < 1 or C < 1 or C % groups:
+        _refuse(name, f"{C} channels do not divide into {groups} groups")
+    if act not in (ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU):
+        _refuse(name, f"activation {act}: ACT_NONE, ACT_RELU, ACT_SILU or ACT_GELU expected")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        _refuse(name, f"eps {eps}: a number >= 0 expected")
+    gamma = _vector(name, gamma, "gamma", C, torch.float32, x.device)
+    beta = _vector(name, beta, "beta", C, torch.float32, x.device)
+    lens = _vector(name, lens, "lens", B, torch.int64, x.device)
+    if stats is not None and not _like(name, stats, "stats", (B, groups, 2), torch.float32, x.device).is_contiguous():
+        _refuse(name, "stats must be contiguous")
+    _on_gpu(name, x)
+    if x.stride(2) != 1 and C > 1:
+        x = x.contiguous()
+    a = GnArgs(x.data_ptr(), None, None, gamma.data_ptr(), beta.data_ptr(), _ptr(stats), None, None, _ptr(lens),
+               _stride(x, 0), _stride(x, 1), 0, 0, 0, 0, B, L, C, groups, act, bf16, eps)
+    return a, (x, gamma, beta, lens)
+
+
+def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, out=None, stats=None):
+    """act(GroupNorm(x)) over channels-last x [B, L, C] (fp32 or bf16), `groups` groups of C / groups channels, gamma and beta fp32
+    [C], act one of ACT_NONE / ACT_RELU / ACT_SILU / ACT_GELU.  lens int64 [B]: the statistics cover the rows before it, rows at or
+    past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
+    groupnorm_act_bwd.  out (optional) may be x."""
+    name = "groupnorm_act"
+    a, keep = _gn_args(name, x, gamma, beta, groups, act, eps, lens, stats)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    else:
+        _like(name, out, "out", x.shape, x.dtype, x.device)
+        if (a.C > 1 and out.stride(2) != 1) or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(2)):
+            _refuse(name, "out must have contiguous channels and distinct rows")
+    if out.numel() == 0:
+        return out
+    a.out, a.ob, a.ol = out.data_ptr(), _stride(out, 0), _stride(out, 1)
+    with _on(x):
+        n = lib.styler_groupnorm_act_workspace_bytes(a.B, a.L, a.C, a.G, a.bf16, 0)
+        ws = _workspace(n, x.device)
+        _chk(lib.styler_groupnorm_act(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_groupnorm_act")
+    return out
+
+
+def groupnorm_act_bwd(x, dy, gamma, beta, stats, groups, act=ACT_SILU, *, lens=None):
+    """-> (dx, dgamma, dbeta) of groupnorm_act from the stats it wrote and the gradient dy of its output: dx contiguous in x's type,
+    zero at and past lens; dgamma, dbeta fp32 [C].  Deterministic."""
+    name = "groupnorm_act_bwd"
+    if stats is None:
+        _refuse(name, "the forward's stats are needed")
+    a, keep = _gn_args(name, x, gamma, beta, groups, act, 0.0, lens, stats)
+    dy = _like(name, dy, "dy", x.shape, x.dtype, x.device)
+    if dy.stride(2) != 1 and a.C > 1:
+        dy = dy.contiguous()
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    dgamma, dbeta = torch.empty(a.C, device=x.device), torch.empty(a.C, device=x.device)
+    if dx.numel() == 0:
+        return dx, dgamma.zero_(), dbeta.zero_()
+    a.dy, a.out, a.dgamma, a.dbeta = dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr()
+    a.db, a.dl, a.ob, a.ol = _stride(dy, 0), _stride(dy, 1), _stride(dx, 0), _stride(dx, 1)
+    with _on(x):
+        n = lib.styler_groupnorm_act_workspace_bytes(a.B, a.L, a.C, a.G, a.bf16, 1)
+        ws = _workspace(n, x.device)
+        _chk(lib.styler_groupnorm_act_bwd(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_groupnorm_act_bwd")
+    return dx, dgamma, dbeta
