@@ -23,6 +23,7 @@
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr uint32_t OOB = 0x80000000u;                  // past every descriptor's num_records
 constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
@@ -37,7 +38,7 @@ struct XArgs {
   const uint8_t* mask;
   int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh;   // strides (elements): item, row, head; g: dout
   int64_t maskb;
-  int B, Lq, Lk, H, G, R, D, nrt, splits;
+  int B, Lq, Lk, H, G, R, D, nrt, splits, chunk;
   float scale;
 };
 
@@ -47,17 +48,14 @@ __device__ __forceinline__ int clamp_len(const int64_t* len, int b, int L) {
   return n < 0 ? 0 : (n > L ? L : (int)n);
 }
 
-// Launch slot -> logical block: workgroups go to the eight XCDs round robin, and blocks that read the same keys are
-// neighbours in the logical order -- an XCD (and its L2) gets consecutive ones.
-__device__ __forceinline__ int xcd_block(int total) {
-  const int n = blockIdx.x;
-  const int v = (n & 7) * (int)(gridDim.x >> 3) + (n >> 3);
+// Launch slot -> logical block.  Workgroups go to the eight XCDs round robin, each with its own L2, and blocks that read the same
+// keys are neighbours in the logical order: runs of `chunk` logical blocks go to one XCD, run after run to the next.  (One eighth
+// of the blocks each would give an XCD whole items: with ragged lengths the XCD of the longest item then worked alone.)
+__device__ __forceinline__ int xcd_block(int total, int chunk) {
+  const int n = blockIdx.x, i = n >> 3;
+  const int v = ((i / chunk) * 8 + (n & 7)) * chunk + i % chunk;
   return v < total ? v : -1;
 }
-
-template <typename T> struct Elem;
-template <> struct Elem<uint16_t> { static constexpr bool bf16 = true; };
-template <> struct Elem<float> { static constexpr bool bf16 = false; };
 
 // ---- LDS tiles: rows of DT elements, RB bytes ---------------------------------------------------------------------------------
 // The 16-byte piece c of row r stands at piece c ^ swz(r).  256 bytes are the 64 banks once: rows narrower than that share a
@@ -73,28 +71,48 @@ template <int RB> struct Swz {
   }
 };
 
-// Fill ROWS rows (a multiple of 32) of a tile: 1 KB per instruction, dealt to the WAVES waves.  off(row) = byte offset of a
-// tile row from the descriptor's base, seen(row) = its row may be read.
-template <int RB, int ROWS, int WAVES, typename Seen>
-__device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* base, int64_t ldbytes, int dbytes, int wave, int lane,
-                                         Seen seen) {
-  constexpr int RPI = 1024 / RB, N = ROWS * RB / 1024;       // rows per instruction, instructions
-  static_assert(N % WAVES == 0 || N < WAVES, "");
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
-  const int lrow = lane / (RB / 16);
-  const uint32_t piece = lane % (RB / 16);
+// Fill ROWS rows (a multiple of 32) of a tile: 1 KB per instruction, instruction i of a wave covers the rows
+// (4 i + wave) RPI .. + RPI.  DmaLane: what a lane adds to the tile's base -- its row of the wave's first instruction and its
+// (permuted) 16-byte piece; the permutation has a period of 16 rows, so it differs between instructions only where four of them
+// cover fewer.  w: the bits of the rows that may be read (32 rows a word).
+template <int RB> struct DmaLane {
+  static constexpr int RPI = 1024 / RB, VAR = RPI * 4 >= 16 ? 1 : 16 / (RPI * 4);
+  uint32_t off[VAR];
+  int row;
+  __device__ __forceinline__ void init(int64_t ldbytes, int dbytes, int wave, int lane) {
+    row = wave * RPI + lane / (RB / 16);
 #pragma unroll
-  for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
-    const int ins = i * WAVES + wave;
-    if (N % WAVES != 0 && ins >= N) break;
-    const int row = ins * RPI + lrow;
-    const uint32_t c = (piece ^ Swz<RB>::of(row)) * 16;
-    const uint32_t off = (c < (uint32_t)dbytes && seen(row)) ? (uint32_t)(row * (int)ldbytes) + c : OOB;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + lds + ins * 1024), 16, off, 0, 0, 0);
+    for (int i = 0; i < VAR; ++i) {
+      const uint32_t c = ((lane % (RB / 16)) ^ Swz<RB>::of(i * 4 * RPI + row)) * 16;
+      off[i] = c < (uint32_t)dbytes ? (uint32_t)(row * (int)ldbytes) + c : OOB;
+    }
+  }
+};
+template <int RB, int ROWS, int NW>
+__device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* base, int64_t ldbytes, const DmaLane<RB>& dl, int wave,
+                                         const uint32_t (&w)[NW]) {
+  constexpr int RPI = DmaLane<RB>::RPI, N = ROWS / (4 * RPI);        // instructions per wave
+  static_assert(N >= 1 && NW == ROWS / 32, "");
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const i32x4 rs = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), 0x7fffffff, 0x00020000};      // raw buffer, 2^31 - 1 bytes
+  const uint32_t l0 = (uint32_t)(uintptr_t)(lds_void*)smem + lds + wave * 1024;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r0 = i * 4 * RPI;                                      // (the word of row r0 + dl.row: 4 RPI divides 32 or is 32 k)
+    uint32_t word = w[r0 / 32];
+    int bit = r0 % 32 + dl.row;
+    if constexpr (4 * RPI > 32) { if (dl.row >= 32) word = w[r0 / 32 + 1]; bit &= 31; }
+    const uint32_t off = (word >> bit) & 1u ? dl.off[i % DmaLane<RB>::VAR] : OOB;
+    // asm: the compiler lets no transposing LDS read start before the DMA it knows of has landed (it cannot tell the buffers
+    // apart), i.e. it would wait for the NEXT tile in the middle of this one.  wait_tiles orders the DMA; the asm has no outputs.
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                 :: "v"(off), "s"(rs), "s"(l0 + i * 4096), "s"(r0 * (int)ldbytes) : "memory");
   }
 }
-__device__ __forceinline__ void wait_tiles() {         // this wave's DMA has landed and its LDS reads are done; then all waves'
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// This wave's DMA has landed and its LDS reads are done; then all waves'.  The builtin, not asm: the compiler has to know that
+// nothing is outstanding, or it waits for everything where a value loaded before the loop is first used in it.
+__device__ __forceinline__ void wait_tiles() {
+  __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0)
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
@@ -277,13 +295,6 @@ __device__ __forceinline__ KeyWords<KT> key_words(const MaskBytes<KT>& m, bool h
   }
   return r;
 }
-template <int KT> __device__ __forceinline__ bool word_bit(const KeyWords<KT>& k, int row) {
-  uint32_t w = k.w[0];
-#pragma unroll
-  for (int i = 1; i < KT / 32; ++i) w = (row >> 5) == i ? k.w[i] : w;
-  return (w >> (row & 31)) & 1u;
-}
-
 // rows of keys per tile (shared-tile kernels) such that two tiles of K and V stay within 64 KB where two blocks per CU pay
 template <typename T, int DT> constexpr int key_tile() { return DT * sizeof(T) >= 512 ? 32 : 64; }
 
@@ -302,9 +313,10 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
   constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
   constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * NBUF * TILE + (FEW ? 1024 : 0)];
+  constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM + (FEW ? 1152 : 0)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
   const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
   const int M = a.Lq * a.R;
@@ -337,10 +349,12 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
   MaskBytes<KT> mb;
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
+  DmaLane<RB> kdl, vdl;
+  kdl.init(klb, dbytes, wave, lane);
+  vdl.init(vlb, dbytes, wave, lane);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
-    auto seen = [&](int row) { return word_bit(kw, row); };
-    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, dbytes, wave, lane, seen);
-    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, dbytes, wave, lane, seen);
+    dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
+    dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
   };
   fill(t0, 0, cur);
   Frag<T, DT> qf;
@@ -440,7 +454,8 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
     }
   } else {
     // join the four waves: ml[wave][32] = (max, sum), then o scaled to the common maximum, summed in wave order
-    float* ml = reinterpret_cast<float*>(smem + 2 * NBUF * TILE);
+    float* ml = reinterpret_cast<float*>(smem + SMEM);
+    float* inv = ml + 256;
     if (lh == 0) { ml[(wave * 32 + li) * 2] = m2; ml[(wave * 32 + li) * 2 + 1] = l; }
     wait_tiles();
     float mm = -INFINITY, lt = 0.f;
@@ -450,38 +465,35 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
 #pragma unroll
     for (int w = 0; w < 4; ++w) lt += ml[(w * 32 + li) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + li) * 2] - base);
     const float c = __builtin_amdgcn_exp2f(m2 - base);
-    // rows of DT + 4 floats: a half wave's 32 rows start 4 banks apart
+    // [wave][32 rows of DT + 4 floats]: the rows of a half wave start 4 banks apart
     float* so = reinterpret_cast<float*>(smem);
     constexpr int LDO = DT + 4;
-    static_assert(32 * LDO * 4 <= 2 * NBUF * TILE, "");
-    for (int w = 0; w < 4; ++w) {
-      if (wave == w) {
+    static_assert(4 * 32 * LDO * 4 <= SMEM, "");
 #pragma unroll
-        for (int dt = 0; dt < DT / 32; ++dt)
+    for (int dt = 0; dt < DT / 32; ++dt)
 #pragma unroll
-          for (int gq = 0; gq < 4; ++gq) {
-            float4* p = reinterpret_cast<float4*>(so + li * LDO + dt * 32 + gq * 8 + lh * 4);
-            float4 x = make_float4(o[dt][gq * 4] * c, o[dt][gq * 4 + 1] * c, o[dt][gq * 4 + 2] * c, o[dt][gq * 4 + 3] * c);
-            if (w) { const float4 y = *p; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
-            *p = x;
-          }
-      }
-      wait_tiles();
-    }
+      for (int gq = 0; gq < 4; ++gq)
+        *reinterpret_cast<float4*>(so + (wave * 32 + li) * LDO + dt * 32 + gq * 8 + lh * 4) =
+            make_float4(o[dt][gq * 4] * c, o[dt][gq * 4 + 1] * c, o[dt][gq * 4 + 2] * c, o[dt][gq * 4 + 3] * c);
     if (wave == 0 && lh == 0 && m < M) {
       if (a.splits > 1) { pml[0] = mm; pml[1] = lt; }
       else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = lt == 0.f ? -INFINITY : (mm + log2f(lt)) * LN2;
     }
-    if (wave == 0 && lh == 0) ml[li] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+    if (wave == 0 && lh == 0) inv[li] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
     wait_tiles();
     for (int i = tid; i < 32 * (DT / 4); i += 256) {
       const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
       if (mr >= M || d >= a.D) continue;
-      const float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
+      float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(so + (w * 32 + r) * LDO + d);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
       if (a.splits > 1) {
         *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
       } else {
-        const float cl = ml[r];
+        const float cl = inv[r];
         T* p = reinterpret_cast<T*>(a.out) + b * a.ob + (mr / a.R) * a.ol + (g * a.R + mr % a.R) * a.oh + d;
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x.x * cl, x.y * cl), cvt_pk_bf16_rne(x.z * cl, x.w * cl));
         else *reinterpret_cast<float4*>(p) = make_float4(x.x * cl, x.y * cl, x.z * cl, x.w * cl);
@@ -490,38 +502,51 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
   }
 }
 
-// Join the splits of a forward launch: a wave per row.  Splits are added in order; an empty split has max = -inf, sum = 0 and its
-// partial row is not read (it is not written either).
-template <typename T>
+// Join the splits of a forward launch: a wave per row.  Lane s holds the (max, sum) of split s; the partial rows are read by
+// W / 4 lanes each, 256 / W splits at a time (W = 32, 64, 128 >= D), and their sums joined across those lane groups.  An empty
+// split has max = -inf, sum = 0, and its partial row is not read (it is not written either).
+constexpr int MAX_SPLITS = 64;
+template <typename T, int W>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
   const int lane = threadIdx.x & 63;
   const int M = a.Lq * a.R;
   const int64_t rows = (int64_t)a.B * a.G * M, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int bg = (int)(row / M), m = (int)(row % M), g = bg % a.G, b = bg / a.G, qi = m / a.R, head = g * a.R + m % a.R;
-  const float* ml = a.part + rows * a.splits * a.D;
-  float mm = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) mm = fmaxf(mm, ml[(s * rows + row) * 2]);
-  mm = wave_max(mm);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  float l = 0.f, x = 0.f, y = 0.f;
-  const int d = lane * 2;
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 q = *reinterpret_cast<const float2*>(ml + (s * rows + row) * 2);
-    const float c = __builtin_amdgcn_exp2f(q.x - base);
-    l += c * q.y;
-    if (q.x != -INFINITY && d < a.D) {
-      const float2 p = *reinterpret_cast<const float2*>(a.part + (s * rows + row) * a.D + d);
-      x = fmaf(c, p.x, x);
-      y = fmaf(c, p.y, y);
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < a.splits) ml = *reinterpret_cast<const float2*>(a.part + rows * a.splits * a.D + (lane * rows + row) * 2);
+  const float mm = wave_max(ml.x), base = mm == -INFINITY ? 0.f : mm;
+  const float c = __builtin_amdgcn_exp2f(ml.x - base);
+  const float l = wave_sum(c * ml.y);
+  constexpr int LPR = W / 4, GR = 64 / LPR, U = 4;
+  const int d = (lane % LPR) * 4, grp = lane / LPR;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < a.splits; s0 += GR * U) {
+    float4 p[U];
+    float w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int sp = s0 + u * GR + grp;
+      w[u] = __shfl(c, sp & 63, 64);
+      p[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const bool full = __shfl(ml.x, sp & 63, 64) != -INFINITY;
+      if (sp < a.splits && full && d < a.D) p[u] = *reinterpret_cast<const float4*>(a.part + (sp * rows + row) * a.D + d);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * GR + grp >= a.splits) w[u] = 0.f;
+      x.x = fmaf(w[u], p[u].x, x.x); x.y = fmaf(w[u], p[u].y, x.y); x.z = fmaf(w[u], p[u].z, x.z); x.w = fmaf(w[u], p[u].w, x.w);
     }
   }
+#pragma unroll
+  for (int o = LPR; o < 64; o <<= 1) {
+    x.x += __shfl_xor(x.x, o, 64); x.y += __shfl_xor(x.y, o, 64); x.z += __shfl_xor(x.z, o, 64); x.w += __shfl_xor(x.w, o, 64);
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (d < a.D) {
+  if (grp == 0 && d < a.D) {
     T* p = reinterpret_cast<T*>(a.out) + b * a.ob + qi * a.ol + head * a.oh + d;
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = cvt_pk_bf16_rne(x * inv, y * inv);
-    else *reinterpret_cast<float2*>(p) = make_float2(x * inv, y * inv);
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x.x * inv, x.y * inv), cvt_pk_bf16_rne(x.z * inv, x.w * inv));
+    else *reinterpret_cast<float4*>(p) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
   }
   if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (mm + log2f(l)) * LN2;
 }
@@ -533,9 +558,10 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
   constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * NBUF * TILE];
+  constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
   const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
   const int M = a.Lq * a.R;
@@ -574,10 +600,12 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   MaskBytes<KT> mb;
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
+  DmaLane<RB> kdl, vdl;
+  kdl.init(klb, dbytes, wave, lane);
+  vdl.init(vlb, dbytes, wave, lane);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
-    auto seen = [&](int row) { return word_bit(kw, row); };
-    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, dbytes, wave, lane, seen);
-    dma_tile<RB, KT, 4>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, dbytes, wave, lane, seen);
+    dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
+    dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
   };
   fill(t0, 0, cur);
   load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
@@ -636,25 +664,23 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   } else {
     float* so = reinterpret_cast<float*>(smem);
     constexpr int LDO = DT + 4;
-    static_assert(32 * LDO * 4 <= 2 * NBUF * TILE, "");
-    for (int w = 0; w < 4; ++w) {                        // sums of the four waves, in wave order
-      if (wave == w) {
+    static_assert(4 * 32 * LDO * 4 <= SMEM, "");
 #pragma unroll
-        for (int dt = 0; dt < DT / 32; ++dt)
+    for (int dt = 0; dt < DT / 32; ++dt)
 #pragma unroll
-          for (int gq = 0; gq < 4; ++gq) {
-            float4* p = reinterpret_cast<float4*>(so + li * LDO + dt * 32 + gq * 8 + lh * 4);
-            float4 x = make_float4(dq[dt][gq * 4], dq[dt][gq * 4 + 1], dq[dt][gq * 4 + 2], dq[dt][gq * 4 + 3]);
-            if (w) { const float4 y = *p; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
-            *p = x;
-          }
-      }
-      wait_tiles();
-    }
+      for (int gq = 0; gq < 4; ++gq)
+        *reinterpret_cast<float4*>(so + (wave * 32 + li) * LDO + dt * 32 + gq * 8 + lh * 4) =
+            make_float4(dq[dt][gq * 4], dq[dt][gq * 4 + 1], dq[dt][gq * 4 + 2], dq[dt][gq * 4 + 3]);
+    wait_tiles();
     for (int i = tid; i < 32 * (DT / 4); i += 256) {
       const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
       if (mr >= M || d >= a.D) continue;
       float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {                      // in wave order
+        const float4 y = *reinterpret_cast<const float4*>(so + (w * 32 + r) * LDO + d);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
       x.x *= a.scale; x.y *= a.scale; x.z *= a.scale; x.w *= a.scale;
       if (a.splits > 1) *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
       else {
@@ -676,7 +702,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dk
   constexpr int RB = DT * sizeof(T), RT = row_tile<T, DT>(), TILE = RT * RB;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-  const int v = xcd_block(a.nrt * a.splits * a.G * a.B);
+  const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
   const int kt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
   const int klen = clamp_len(a.len, b, a.Lk), qv = clamp_len(a.qlen, b, a.Lq);
@@ -702,11 +728,16 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dk
   const int64_t qlb = a.ql * (int64_t)sizeof(T), glb = a.gl * (int64_t)sizeof(T);
   float* stat = reinterpret_cast<float*>(smem + 4 * TILE);         // [buf][lse2 | delta][RT]
   float sreg = 0.f;
+  DmaLane<RB> qdl, gdl;
+  qdl.init(qlb, dbytes, wave, lane);
+  gdl.init(glb, dbytes, wave, lane);
   auto fill = [&](int t, int buf) {
-    const int r = t / nt, q0 = (t - r * nt) * RT, head = g * a.R + r;
-    auto ok = [&](int row) { return q0 + row < qv; };
-    dma_tile<RB, RT, 4>(smem, buf * 2 * TILE, reinterpret_cast<const T*>(a.q) + b * a.qb + (int64_t)q0 * a.ql + head * a.qh, qlb, dbytes, wave, lane, ok);
-    dma_tile<RB, RT, 4>(smem, buf * 2 * TILE + TILE, reinterpret_cast<const T*>(a.dout) + b * a.gb + (int64_t)q0 * a.gl + head * a.gh, glb, dbytes, wave, lane, ok);
+    const int r = t / nt, q0 = (t - r * nt) * RT, head = g * a.R + r, left = qv - q0;
+    uint32_t w[RT / 32];
+#pragma unroll
+    for (int i = 0; i < RT / 32; ++i) w[i] = left >= 32 * (i + 1) ? 0xffffffffu : (left <= 32 * i ? 0u : (1u << (left - 32 * i)) - 1u);
+    dma_tile<RB, RT>(smem, buf * 2 * TILE, reinterpret_cast<const T*>(a.q) + b * a.qb + (int64_t)q0 * a.ql + head * a.qh, qlb, qdl, wave, w);
+    dma_tile<RB, RT>(smem, buf * 2 * TILE + TILE, reinterpret_cast<const T*>(a.dout) + b * a.gb + (int64_t)q0 * a.gl + head * a.gh, glb, gdl, wave, w);
     if (tid < 2 * RT) {
       const int q = q0 + tid % RT;
       const int64_t s = ((int64_t)b * a.H + head) * a.Lq + q;
@@ -800,7 +831,6 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a) {
   else *reinterpret_cast<float4*>(p) = x;
 }
 
-constexpr int MAX_SPLITS = 64;
 // How many shares of a long axis (n tiles) give the launch about `want` blocks, each with at least `least` tiles.
 int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   int64_t s = (want + blocks - 1) / blocks;
@@ -826,23 +856,33 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   return p;
 }
 
-dim3 grid8(int64_t blocks) { return dim3((unsigned)((blocks + 7) / 8 * 8)); }
+// Runs of logical blocks per XCD (see xcd_block): as long as the blocks of one (item, key head), but never fewer than 64 runs
+// -- eight per XCD, so that ragged items even out.
+dim3 grid_for(XArgs& a) {
+  const int64_t per = (int64_t)a.nrt * a.splits, total = per * a.G * a.B;
+  int64_t c = total / 64;
+  if (c > per) c = per;
+  if (c < 1) c = 1;
+  a.chunk = (int)c;
+  return dim3((unsigned)((total + 8 * c - 1) / (8 * c) * 8 * c));
+}
 
 template <typename T, int DT>
-void launch_fwd(const XArgs& a, bool few, hipStream_t st) {
-  const dim3 g = grid8((int64_t)a.nrt * a.splits * a.G * a.B);
+void launch_fwd(XArgs& a, bool few, hipStream_t st) {
+  const dim3 g = grid_for(a);
   if (few) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, true>), g, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, false>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
-void launch_dq(const XArgs& a, bool few, hipStream_t st) {
-  const dim3 g = grid8((int64_t)a.nrt * a.splits * a.G * a.B);
+void launch_dq(XArgs& a, bool few, hipStream_t st) {
+  const dim3 g = grid_for(a);
   if (few) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, true>), g, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, false>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
-void launch_dkv(const XArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((xattn_dkv_kernel<T, DT>), grid8((int64_t)a.nrt * a.splits * a.G * a.B), dim3(256), 0, st, a);
+void launch_dkv(XArgs& a, hipStream_t st) {
+  const dim3 g = grid_for(a);
+  hipLaunchKernelGGL((xattn_dkv_kernel<T, DT>), g, dim3(256), 0, st, a);
 }
 #define BY_WIDTH(T, CALL)              \
   do {                                 \
@@ -868,7 +908,7 @@ int check(const styler_xattn_t* x, bool bwd) {
   if (bwd && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse)) return STYLER_EINVAL;
   const Plan pl = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
   const int64_t bg = (int64_t)x->B * x->G;
-  if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0x7ffffff0 || bg * pl.nkt * pl.dkv > 0x7ffffff0) return STYLER_EINVAL;
+  if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0x60000000 || bg * pl.nkt * pl.dkv > 0x60000000) return STYLER_EINVAL;
   return 0;
 }
 XArgs args(const styler_xattn_t* x) {
@@ -907,8 +947,9 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
 #undef FWD
   if (p.fwd > 1) {
     const unsigned blocks = (unsigned)(((int64_t)x->B * x->H * x->Lq + 3) / 4);
-    if (x->bf16) hipLaunchKernelGGL((xattn_join_kernel<uint16_t>), dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((xattn_join_kernel<float>), dim3(blocks), dim3(256), 0, st, a);
+#define JOIN(T, W) hipLaunchKernelGGL((xattn_join_kernel<T, W>), dim3(blocks), dim3(256), 0, st, a)
+    if (x->bf16) BY_WIDTH(uint16_t, JOIN); else BY_WIDTH(float, JOIN);
+#undef JOIN
   }
   return launch_status();
 }
