@@ -928,9 +928,16 @@ int styler_cross_attention_bwd(const styler_xattn_t* host_args, void* workspace,
  * the other way: the gradient dx of dy.  freqs: rot/2 doubles (angle per position); pos_kind 0: pos = l, 1: int64, 2: float, with
  * item stride posb (0: one row for all).  Strides (item, row, head) in elements, features contiguous; x == y with equal strides is
  * allowed (in place), any other overlap is not. */
-int styler_rotary(const void* x, int64_t xb, int64_t xl, int64_t xh, void* y, int64_t yb, int64_t yl, int64_t yh,
-                  const double* freqs, const void* pos, int64_t posb, int pos_kind, int B, int L, int H, int D, int rot,
-                  int interleaved, int inverse, float gain, int bf16, void* stream);
+typedef struct {
+  const void* x;
+  void* y;
+  const double* freqs;
+  const void* pos;
+  int64_t xb, xl, xh, yb, yl, yh, posb;
+  int32_t B, L, H, D, rot, pos_kind, interleaved, inverse, bf16;
+  float gain;
+} styler_rotary_t;
+int styler_rotary(const styler_rotary_t* host_args, void* stream);
 
 /* Group norm over channels-last [B, L, C] with an activation (STYLER_ACT_NONE / RELU / SILU / GELU), C % G == 0: statistics of
  * group g over the C / G channels of the rows t < len[b] (len may be NULL), biased variance; rows at or past len[b] give zeros.

@@ -4,6 +4,7 @@ The product path has NO CPU fallback: importing this module without the built li
 every op raises on a non-zero return code."""
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("STYLER_LIB") or os.path.join(_HERE, "libstyler_hip.so")     # STYLER_LIB: A/B builds
@@ -149,7 +150,7 @@ _SIGS = {
     "styler_cross_attention_workspace_bytes": [I, I, I, I, I, I, I, I],
     "styler_cross_attention": [P, P, I64, P],
     "styler_cross_attention_bwd": [P, P, I64, P],
-    "styler_rotary": [P, I64, I64, I64, P, I64, I64, I64, P, P, I64, I, I, I, I, I, I, I, I, F, I, P],
+    "styler_rotary": [P, P],
     "styler_groupnorm_act_workspace_bytes": [I, I, I, I, I, I],
     "styler_groupnorm_act": [P, P, I64, P],
     "styler_groupnorm_act_bwd": [P, P, I64, P],
@@ -197,16 +198,11 @@ class CopyDesc(ctypes.Structure):
                [(k, ctypes.c_int32) for k in ("d0", "d1", "d2", "flags")]
 
 
-class XattnArgs(ctypes.Structure):
-    _fields_ = [(k, P) for k in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "len", "q_len", "mask")] + \
-               [(k, I64) for k in ("qb", "ql", "qh", "kb", "kl", "kh", "vb", "vl", "vh", "ob", "ol", "oh", "gb", "gl", "gh", "maskb")] + \
-               [(k, ctypes.c_int32) for k in ("B", "Lq", "Lk", "H", "G", "D", "bf16")] + [("scale", F)]
-
-
-class GnArgs(ctypes.Structure):
-    _fields_ = [(k, P) for k in ("x", "dy", "out", "gamma", "beta", "stats", "dgamma", "dbeta", "len")] + \
-               [(k, I64) for k in ("xb", "xl", "db", "dl", "ob", "ol")] + \
-               [(k, ctypes.c_int32) for k in ("B", "L", "C", "G", "act", "bf16")] + [("eps", F)]
+# styler_xattn_t, styler_gn_t, styler_rotary_t of include/styler_hip.h as packed bytes (a ctypes.Structure takes twice the time to
+# fill, and these calls run once per token).  The entry points read them before they return.
+XATTN = struct.Struct("12Q16q7if")     # 12 pointers, 16 strides, sizes, scale
+GN = struct.Struct("9Q6q6if4x")
+ROTARY = struct.Struct("4Q7q9if")
 
 
 class LstmBwdDesc(ctypes.Structure):

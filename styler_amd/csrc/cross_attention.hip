@@ -295,6 +295,29 @@ __device__ __forceinline__ KeyWords<KT> key_words(const MaskBytes<KT>& m, bool h
   }
   return r;
 }
+// the word of a wave's 32 keys: block kb of a shared tile, or (FEW) the wave's own quarter
+template <bool FEW, int KT> __device__ __forceinline__ uint32_t few_word(const KeyWords<KT> k, int kb, int wave) {
+  uint32_t w = k.w[FEW ? 0 : kb];
+  if constexpr (FEW) {
+#pragma unroll
+    for (int i = 1; i < KT / 32; ++i) w = wave == i ? k.w[i] : w;
+  }
+  return w;
+}
+// Scores start at 0 for a seen key and at -inf for one that is not: its row was filled with zeros, so the product adds 0 and the
+// mask costs nothing after it.
+__device__ __forceinline__ void seen_start(f32x16& s, uint32_t w, int lh) {
+  zero16(s);
+  if (w != 0xffffffffu) {
+    const int un = (int)(~w >> (4 * lh));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int bit = (r & 3) + 8 * (r >> 2);
+      s[r] = __int_as_float(__builtin_amdgcn_sbfe(un, bit, 1) & 0xff800000);
+    }
+  }
+}
+
 // rows of keys per tile (shared-tile kernels) such that two tiles of K and V stay within 64 KB where two blocks per CU pay
 template <typename T, int DT> constexpr int key_tile() { return DT * sizeof(T) >= 512 ? 32 : 64; }
 
@@ -383,18 +406,8 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
         const int blk = FEW ? wave : kb;
-        zero16(s[kb]);
+        seen_start(s[kb], few_word<FEW>(cur, kb, wave), lh);
         mma_rows<T, DT>(s[kb], tk, blk, qf, li, lh);
-        uint32_t w = cur.w[FEW ? 0 : kb];
-        if (FEW) {
-#pragma unroll
-          for (int i = 1; i < KT / 32; ++i) w = wave == i ? cur.w[i] : w;
-        }
-        if (w != 0xffffffffu) {
-          const uint32_t wl = w >> (4 * lh);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = (wl >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[kb][r] : -INFINITY;
-        }
       }
       float mt = -INFINITY;
 #pragma unroll
@@ -629,24 +642,15 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       const int blk = FEW ? wave : kb;
-      uint32_t w = cur.w[FEW ? 0 : kb];
-      if (FEW) {
-#pragma unroll
-        for (int i = 1; i < KT / 32; ++i) w = wave == i ? cur.w[i] : w;
-      }
+      const uint32_t w = few_word<FEW>(cur, kb, wave);
       if (w == 0) continue;
       f32x16 s, dp;
-      zero16(s);
+      seen_start(s, w, lh);                              // (unseen: P = exp2(-inf) = 0)
       zero16(dp);
       mma_rows<T, DT>(s, tk, blk, qf, li, lh);
       mma_rows<T, DT>(dp, tv, blk, dof, li, lh);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * (dp[r] - dl);
-      if (w != 0xffffffffu) {
-        const uint32_t wl = w >> (4 * lh);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (wl >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[r] : 0.f;
-      }
       mma_cols<T, DT>(dq, tk, blk, s, lane);
     }
     if (NBUF == 1 && t + 1 < t1) {

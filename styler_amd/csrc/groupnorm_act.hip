@@ -22,11 +22,11 @@ struct GArgs {
   void* out;                                             // y or dx
   const float *gamma, *beta;
   float* stats;                                          // [B, G, 2] mean, rstd
-  float* ws;
+  float *ws, *pw;                                        // chunk sums [B, chunks, C, 2]; item sums [B, C, 2] (backward)
   float *dgamma, *dbeta;
   const int64_t* len;
   int64_t xb, xl, db, dl, ob, ol;                        // item and row strides of x, dy, out
-  int B, L, C, G, cg, chunks, rows, slab;                // rows: rows per chunk; slab: channels per block
+  int B, L, C, G, cg, chunks, rows, slab, slabs;         // rows: rows per chunk; slab: channels per block
   float eps;
 };
 
@@ -36,20 +36,41 @@ __device__ __forceinline__ int gn_len(const int64_t* len, int b, int L) {
   return n < 0 ? 0 : (n > L ? L : (int)n);
 }
 
+// The kernels would be bound by their instructions with the library's erff and divisions (67 M values in 90 us leave 52
+// instructions a value): one v_exp_f32 and one v_rcp_f32 a value instead.
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2, and e = exp(-z^2 / 2).  For z <= 0, Phi = e h(|z|) with h = erfcx / 2 as a polynomial in
+// t = 1 / (1 + p |z| / sqrt 2) (the form of Hastings' approximations; coefficients fitted here to erfcx over [0, inf) in the
+// norm max |exp(-x^2) err|: 2.6e-9), for z > 0, 1 - that.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.32f * 0.70710678118654752f, fabsf(z), 1.f));
+  e = __builtin_amdgcn_exp2f(-0.72134752044448170f * (z * z));
+  float h = 0.5f * -0.16305777512551112f;
+  h = fmaf(h, t, 0.5f * 0.6326713090095979f);
+  h = fmaf(h, t, 0.5f * -0.6115301283036071f);
+  h = fmaf(h, t, 0.5f * 0.6121517059588323f);
+  h = fmaf(h, t, 0.5f * -0.04181075739763211f);
+  h = fmaf(h, t, 0.5f * 0.21519066395074074f);
+  h = fmaf(h, t, 0.5f * 0.1756557856457516f);
+  h = fmaf(h, t, 0.5f * 0.18072919626182787f);
+  h *= t * e;
+  return z > 0.f ? 1.f - h : h;
+}
 template <int ACT> __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == STYLER_ACT_RELU) return fmaxf(z, 0.f);
-  if constexpr (ACT == STYLER_ACT_SILU) return z / (1.f + __expf(-z));
-  if constexpr (ACT == STYLER_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == STYLER_ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == STYLER_ACT_GELU) { float e; return z * normal_cdf(z, e); }
   return z;
 }
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == STYLER_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == STYLER_ACT_SILU) {
-    const float t = 1.f / (1.f + __expf(-z));
-    return t * (1.f + z * (1.f - t));
+    const float t = sigmoid(z);
+    return fmaf(z * t, 1.f - t, t);
   }
-  if constexpr (ACT == STYLER_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+  if constexpr (ACT == STYLER_ACT_GELU) { float e; const float c = normal_cdf(z, e); return fmaf(z * 0.3989422804014327f, e, c); }
   return 1.f;
 }
 
@@ -87,61 +108,93 @@ template <bool B16, int V> __device__ __forceinline__ void put(void* base, int64
   }
 }
 
-// Sums over the block's rl row lanes (thread = row lane * cv + column): column sums of a in sa, of b in sb [cv * V] on return.
-// red: T * V floats, used for a and then for b.  Two steps each: T / (cv * V) partial sums per channel, then those.
-template <int V, int T>
-__device__ __forceinline__ void col_sum(const float (&a)[V], float* red, float* sa, int cv, int rl, bool on) {
-  const int tid = threadIdx.x, W = cv * V;
-  if (on) {
-    float* r = red + tid / cv * W + tid % cv * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = a[i];
+// Sum over the lanes of a wave that hold the same column: lane & (cv - 1), cv a power of two up to 64.  The xor steps 32, 16 are
+// half and row swaps, 8, 4, 2, 1 rotations and permutations inside sixteen lanes (all lanes agree modulo the steps done).
+__device__ __forceinline__ float same_column_sum(float v, int cv) {
+  if (cv <= 32) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
   }
-  __syncthreads();
-  const int parts = max(1, min(rl, T / W)), per = (rl + parts - 1) / parts;
-  for (int j = tid; j < W * parts; j += T) {             // a (channel, part) pair is one thread's
-    const int c = j % W, p = j / W;
-    float x = 0.f;
-    for (int r = p * per; r < min(rl, (p + 1) * per); ++r) x += red[r * W + c];
-    if (p * per < rl) red[p * per * W + c] = x;          // the first of this thread's own rows
+  if (cv <= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  __syncthreads();
-  for (int c = tid; c < W; c += T) {
-    float x = 0.f;
-    for (int r = 0; r < rl; r += per) x += red[r * W + c];
-    sa[c] = x;
-  }
-  __syncthreads();
+  if (cv <= 8) v += dpp_f32<0x128>(v);
+  if (cv <= 4) v += dpp_f32<0x124>(v);
+  if (cv <= 2) v += dpp_f32<0x4E>(v);
+  if (cv <= 1) v += dpp_f32<0xB1>(v);
+  return v;
 }
+// Sums over the block's rl row lanes (thread = row lane * cv + column): column sums of a in sa, of b in sb [cv * V] on return.
+// red: T * V floats.
 template <int V, int T>
 __device__ __forceinline__ void col_sums(const float (&a)[V], const float (&b)[V], float* red, float* sa, float* sb, int cv, int rl, bool on) {
-  col_sum<V, T>(a, red, sa, cv, rl, on);
-  col_sum<V, T>(b, red, sb, cv, rl, on);
-}
-
-// join (n, mean, M2) of two sets
-__device__ __forceinline__ void join(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
-  const float t = n + n2;
-  if (n2 == 0.f) return;
-  const float d = mean2 - mean, f = n2 / t;
-  mean += d * f;
-  m2 += m22 + d * d * n * f;
-  n = t;
+  const int tid = threadIdx.x, W = cv * V;
+  if (cv <= 32 && (cv & (cv - 1)) == 0) {                // columns repeat inside a wave: one partial row per wave
+    const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = same_column_sum(a[i], cv), y = same_column_sum(b[i], cv);
+      if (lane < cv) {
+        red[wave * 2 * W + lane * V + i] = x;
+        red[wave * 2 * W + W + lane * V + i] = y;
+      }
+    }
+    __syncthreads();
+    for (int c = tid; c < 2 * W; c += T) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < T / 64; ++w) x += red[w * 2 * W + c];
+      (c < W ? sa : sb)[c < W ? c : c - W] = x;
+    }
+    __syncthreads();
+    return;
+  }
+  // one array after the other; two steps each: T / W partial sums per channel, then those
+  const int parts = max(1, min(rl, T / W)), per = (rl + parts - 1) / parts;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (on) {
+      float* r = red + tid / cv * W + tid % cv * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = q ? b[i] : a[i];
+    }
+    __syncthreads();
+    if (parts > 1) {
+      for (int j = tid; j < W * parts; j += T) {         // a (channel, part) pair is one thread's
+        const int c = j % W, p = j / W;
+        float x = 0.f;
+        for (int r = p * per; r < min(rl, (p + 1) * per); ++r) x += red[r * W + c];
+        if (p * per < rl) red[p * per * W + c] = x;      // the first of this thread's own rows
+      }
+      __syncthreads();
+    }
+    for (int c = tid; c < W; c += T) {
+      float x = 0.f;
+      for (int r = 0; r < rl; r += parts > 1 ? per : 1) x += red[r * W + c];
+      (q ? sb : sa)[c] = x;
+    }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------- fused
-// grid (slabs, B).  Thread = (row lane, column of V channels); it holds rows rl, rl + RL, ... (at most IT) in registers.
+// Thread = (row lane, column of V channels); it holds rows rl, rl + RL, ... (at most IT) in registers.  The slabs of an item run
+// on one XCD: their rows share memory lines where a slab is narrower than a line.
 template <bool B16, int V, int ACT, int IT, int T, bool BWD>
 __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
   extern __shared__ float sh[];
-  const int b = blockIdx.y, c0 = blockIdx.x * a.slab, tid = threadIdx.x;
+  const int nx = blockIdx.x >> 3, b = nx / a.slabs * 8 + (blockIdx.x & 7);
+  if (b >= a.B) return;
+  const int c0 = nx % a.slabs * a.slab, tid = threadIdx.x, lane = tid & 63;
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv;
   const bool on = rl < RL;
   const int n = gn_len(a.len, b, a.L), c = c0 + col * V;
-  float* red = sh;                                       // max(T V, 2 slab)
-  float* sa = sh + max(T * V, 2 * a.slab);               // slab
-  float* sb = sa + a.slab;                               // slab
-  float* gm = sb + a.slab;                               // 2 * groups of the slab
+  float* red = sh;                                       // max(T V, slab)
+  float* sa = sh + max(T * V, a.slab);                   // slab each
+  float* sb = sa + a.slab;
+  float* sk = sb + a.slab;
+  float* gm = sk + a.slab;                               // 2 * groups of the slab
   Raw<B16, V> xr[IT], gr[BWD ? IT : 1];
   const int64_t x0 = b * a.xb + c, g0 = b * a.db + c, o0 = b * a.ob + c;
 #pragma unroll
@@ -155,103 +208,103 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       if constexpr (BWD) gr[i].zero();
     }
   }
-  float s[V], q[V], K[V];
+  float s[V], q[V];
   const int ng = W / a.cg, gl0 = c0 / a.cg;
   if constexpr (!BWD) {
+    float K[V];
     Raw<B16, V> k0;
     if (on && n > 0) k0.load(a.x, x0); else k0.zero();
 #pragma unroll
     for (int j = 0; j < V; ++j) { K[j] = k0.get(j); s[j] = 0.f; q[j] = 0.f; }
+    if (tid < cv) {                                      // (row lane 0)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sk[tid * V + j] = K[j];
+    }
 #pragma unroll
     for (int i = 0; i < IT; ++i)
-      if (rl + i * RL < n) {
+      if (on && rl + i * RL < n) {
 #pragma unroll
         for (int j = 0; j < V; ++j) { const float d = xr[i].get(j) - K[j]; s[j] += d; q[j] = fmaf(d, d, q[j]); }
       }
     col_sums<V, T>(s, q, red, sa, sb, cv, RL, on);
-    // channel c: mean = K + s / n, M2 = q - s^2 / n; the group's channels joined in order
-    if (tid < cv) {                                      // (row lane 0 holds K of its channels)
-#pragma unroll
-      for (int j = 0; j < V; ++j) red[tid * V + j] = K[j];
-    }
-    __syncthreads();
-    for (int g = tid; g < ng; g += T) {
-      float N = 0.f, mean = 0.f, m2 = 0.f;
-      const float fn = (float)n;
-      if (n > 0)
-        for (int j = g * a.cg; j < (g + 1) * a.cg; ++j) {
-          const float sm = sa[j] / fn;
-          join(N, mean, m2, fn, red[j] + sm, fmaxf(0.f, sb[j] - sa[j] * sm));
+    // a wave per group: channel c has mean K + s / n and M2 = q - s^2 / n; all its channels have n values
+    const float fn = (float)n, inv = n > 0 ? 1.f / fn : 0.f, icg = 1.f / (float)a.cg;
+    for (int g = tid >> 6; g < ng; g += T / 64) {
+      float m = 0.f, m2 = 0.f;
+      for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) m += sk[j] + sa[j] * inv;
+      const float mean = wave_sum(m) * icg;
+      for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) {
+        const float sm = sa[j] * inv, d = (sk[j] + sm) - mean;
+        m2 += fmaxf(0.f, sb[j] - sa[j] * sm) + fn * d * d;
+      }
+      const float var = wave_sum(m2) * (inv * icg), rstd = n > 0 ? rsqrtf(var + a.eps) : 0.f;
+      if (lane == 0) {
+        gm[2 * g] = n > 0 ? mean : 0.f;
+        gm[2 * g + 1] = rstd;
+        if (a.stats) {
+          float* st = a.stats + ((int64_t)b * a.G + gl0 + g) * 2;
+          st[0] = n > 0 ? mean : 0.f;
+          st[1] = rstd;
         }
-      const float rstd = n > 0 ? rsqrtf(m2 / N + a.eps) : 0.f;
-      gm[2 * g] = mean;
-      gm[2 * g + 1] = rstd;
-      if (a.stats) {
-        float* st = a.stats + ((int64_t)b * a.G + gl0 + g) * 2;
-        st[0] = mean;
-        st[1] = rstd;
       }
     }
     __syncthreads();
-  } else {
-    for (int g = tid; g < ng; g += T) {
-      const float* st = a.stats + ((int64_t)b * a.G + gl0 + g) * 2;
-      gm[2 * g] = st[0];
-      gm[2 * g + 1] = st[1];
-    }
-    __syncthreads();
-  }
-  if (!BWD && !on) return;
-  float ga[V], be[V], mean[V], rstd[V];
+    if (!on) return;
+    float A[V], Z[V];                                    // z = A x + Z
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int g = on ? (col * V + j) / a.cg : 0;
-    ga[j] = on ? a.gamma[c + j] : 0.f;
-    be[j] = on ? a.beta[c + j] : 0.f;
-    mean[j] = gm[2 * g];
-    rstd[j] = gm[2 * g + 1];
-  }
-  if constexpr (!BWD) {
+    for (int j = 0; j < V; ++j) {
+      const int g = (col * V + j) / a.cg;
+      A[j] = gm[2 * g + 1] * a.gamma[c + j];
+      Z[j] = fmaf(-gm[2 * g], A[j], a.beta[c + j]);
+    }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int t = rl + i * RL;
       if (t >= a.L) break;
       float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = t < n ? act_of<ACT>((xr[i].get(j) - mean[j]) * rstd[j] * ga[j] + be[j]) : 0.f;
+      for (int j = 0; j < V; ++j) y[j] = t < n ? act_of<ACT>(fmaf(xr[i].get(j), A[j], Z[j])) : 0.f;
       put<B16, V>(a.out, o0 + t * a.ol, y);
     }
   } else {
+    float ga[V], be[V], R[V], S[V];                      // xh = R x + S
 #pragma unroll
-    for (int j = 0; j < V; ++j) { s[j] = 0.f; q[j] = 0.f; }
+    for (int j = 0; j < V; ++j) {
+      const float* st = a.stats + ((int64_t)b * a.G + (on ? (c + j) / a.cg : 0)) * 2;
+      ga[j] = on ? a.gamma[c + j] : 0.f;
+      be[j] = on ? a.beta[c + j] : 0.f;
+      R[j] = st[1];
+      S[j] = -st[0] * R[j];
+      s[j] = 0.f;
+      q[j] = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < IT; ++i)
-      if (rl + i * RL < n) {
+      if (on && rl + i * RL < n) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float xh = (xr[i].get(j) - mean[j]) * rstd[j];
-          const float dz = gr[i].get(j) * act_slope<ACT>(xh * ga[j] + be[j]);
+          const float xh = fmaf(xr[i].get(j), R[j], S[j]);
+          const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
           s[j] += dz;
           q[j] = fmaf(dz, xh, q[j]);
         }
       }
     col_sums<V, T>(s, q, red, sa, sb, cv, RL, on);
-    for (int j = tid; j < W; j += T) {                   // this item's share of the parameter gradients
-      a.ws[((int64_t)b * a.C + c0 + j) * 2] = sa[j];
-      a.ws[((int64_t)b * a.C + c0 + j) * 2 + 1] = sb[j];
-    }
-    for (int g = tid; g < ng; g += T) {
+    for (int j = tid; j < W; j += T)                     // this item's share of the parameter gradients
+      *reinterpret_cast<float2*>(a.pw + ((int64_t)b * a.C + c0 + j) * 2) = make_float2(sa[j], sb[j]);
+    const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
+    for (int g = tid >> 6; g < ng; g += T / 64) {
       float m1 = 0.f, m2 = 0.f;
-      for (int j = g * a.cg; j < (g + 1) * a.cg; ++j) { m1 = fmaf(sa[j], a.gamma[c0 + j], m1); m2 = fmaf(sb[j], a.gamma[c0 + j], m2); }
-      const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
-      red[2 * g] = m1 * inv;
-      red[2 * g + 1] = m2 * inv;
+      for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) { m1 = fmaf(sa[j], a.gamma[c0 + j], m1); m2 = fmaf(sb[j], a.gamma[c0 + j], m2); }
+      m1 = wave_sum(m1);
+      m2 = wave_sum(m2);
+      if (lane == 0) { gm[2 * g] = m1 * inv; gm[2 * g + 1] = m2 * inv; }
     }
     __syncthreads();
     if (!on) return;
     float m1[V], m2[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) { const int g = (col * V + j) / a.cg; m1[j] = red[2 * g]; m2[j] = red[2 * g + 1]; }
+    for (int j = 0; j < V; ++j) { const int g = (col * V + j) / a.cg; m1[j] = gm[2 * g]; m2[j] = gm[2 * g + 1]; }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int t = rl + i * RL;
@@ -259,9 +312,9 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = (xr[i].get(j) - mean[j]) * rstd[j];
-        const float dz = gr[i].get(j) * act_slope<ACT>(xh * ga[j] + be[j]);
-        y[j] = t < n ? rstd[j] * (dz * ga[j] - m1[j] - xh * m2[j]) : 0.f;
+        const float xh = fmaf(xr[i].get(j), R[j], S[j]);
+        const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
+        y[j] = t < n ? R[j] * (fmaf(dz, ga[j], -m1[j]) - xh * m2[j]) : 0.f;
       }
       put<B16, V>(a.out, o0 + t * a.ol, y);
     }
@@ -282,24 +335,21 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
   float* sa = sh + T * V;
   float* sb = sa + a.slab;
   float* ws = a.ws + (((int64_t)b * a.chunks + blockIdx.x) * a.C + c0) * 2;
-  if (t0 >= t1) {                                        // (the joining launch skips chunks without rows; the backward sums them)
-    if (BWD) for (int j = tid; j < 2 * W; j += T) ws[j] = 0.f;
-    return;
-  }
+  if (t0 >= t1) return;                                  // (the joining launch skips chunks without rows)
   float s[V], q[V], K[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) { s[j] = 0.f; q[j] = 0.f; K[j] = 0.f; }
   const int64_t x0 = b * a.xb + c, g0 = b * a.db + c;
   if (on) {
-    float ga[V], be[V], mean[V], rstd[V];
+    float ga[V], be[V], R[V], S[V];                      // xh = R x + S
     if constexpr (BWD) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float* st = a.stats + ((int64_t)b * a.G + (c + j) / a.cg) * 2;
         ga[j] = a.gamma[c + j];
         be[j] = a.beta[c + j];
-        mean[j] = st[0];
-        rstd[j] = st[1];
+        R[j] = st[1];
+        S[j] = -st[0] * R[j];
       }
     } else {
       Raw<B16, V> k0;
@@ -322,8 +372,8 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if constexpr (BWD) {
-            const float xh = (xr[u].get(j) - mean[j]) * rstd[j];
-            const float dz = gr[u].get(j) * act_slope<ACT>(xh * ga[j] + be[j]);
+            const float xh = fmaf(xr[u].get(j), R[j], S[j]);
+            const float dz = gr[u].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
             s[j] += dz;
             q[j] = fmaf(dz, xh, q[j]);
           } else {
@@ -355,58 +405,92 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
   }
 }
 
-// Join the chunks of group (b, g): grid (G, B), a block per group.  Forward: stats.  Backward: the group's two means -> gw [B, G, 2].
-template <bool BWD>
-__global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw) {
-  __shared__ float red[3][256];
-  const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int n = gn_len(a.len, b, a.L);
-  const int live = (n + a.rows - 1) / a.rows;
-  float N = 0.f, x = 0.f, y = 0.f;
-  for (int i = tid; i < live * a.cg; i += 256) {
-    const int ch = i / a.cg, c = g * a.cg + i % a.cg;
-    const float2 p = *reinterpret_cast<const float2*>(a.ws + (((int64_t)b * a.chunks + ch) * a.C + c) * 2);
-    if constexpr (BWD) { x = fmaf(p.x, a.gamma[c], x); y = fmaf(p.y, a.gamma[c], y); }
-    else join(N, x, y, (float)(min(n, (ch + 1) * a.rows) - ch * a.rows), p.x, p.y);
-  }
-  red[0][tid] = N; red[1][tid] = x; red[2][tid] = y;
+// Join the chunks of group (b, g): grid (G, B), a block per group, thread = (chunk lane, channel).  Forward, from (mean, M2) of
+// n_i rows each: mean = sum n_i mean_i / N, then M2 = sum M2_i + n_i (mean_i - mean)^2 -> stats.  Backward: the channels' sums
+// over the chunks -> pw [B, C, 2], and the group's two means -> gw [B, G, 2].
+__device__ __forceinline__ float block_sum256(float v, float* red) {
+  v = wave_sum(v);
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) {
-      if constexpr (BWD) { red[1][tid] += red[1][tid + o]; red[2][tid] += red[2][tid + o]; }
-      else join(red[0][tid], red[1][tid], red[2][tid], red[0][tid + o], red[1][tid + o], red[2][tid + o]);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+template <bool BWD>
+__global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw, float* pw) {
+  __shared__ float red[2][256];
+  const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int n = gn_len(a.len, b, a.L), live = (n + a.rows - 1) / a.rows;
+  const int cl = min(a.cg, 256), RL = 256 / cl, r0 = tid / cl, c = tid - r0 * cl;
+  const float* ws = a.ws + (int64_t)b * a.chunks * a.C * 2;
+  const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
+  float x = 0.f, y = 0.f;
+  for (int c0 = 0; c0 < a.cg; c0 += cl) {                // (one turn unless a group has more than 256 channels)
+    const int ch = g * a.cg + c0 + c;
+    const bool on = r0 < RL && c0 + c < a.cg;
+    float sx = 0.f, sy = 0.f;
+    if (on) {
+#pragma unroll 8
+      for (int i = r0; i < live; i += RL) {
+        const float2 p = *reinterpret_cast<const float2*>(ws + ((int64_t)i * a.C + ch) * 2);
+        if constexpr (BWD) { sx += p.x; sy += p.y; }
+        else sx = fmaf((float)(min(n, (i + 1) * a.rows) - i * a.rows), p.x, sx);
+      }
     }
-    __syncthreads();
+    if constexpr (BWD) {
+      __syncthreads();
+      red[0][tid] = sx;
+      red[1][tid] = sy;
+      __syncthreads();
+      if (tid < cl && on) {
+        for (int r = 1; r < RL; ++r) { sx += red[0][r * cl + c]; sy += red[1][r * cl + c]; }
+        *reinterpret_cast<float2*>(pw + ((int64_t)b * a.C + ch) * 2) = make_float2(sx, sy);
+        x = fmaf(sx, a.gamma[ch], x);
+        y = fmaf(sy, a.gamma[ch], y);
+      }
+    } else {
+      x += sx;
+    }
+  }
+  __syncthreads();
+  x = block_sum256(x, red[0]) * inv;
+  if constexpr (BWD) {
+    y = block_sum256(y, red[1]) * inv;
+  } else {
+    for (int c0 = 0; c0 < a.cg; c0 += cl) {
+      if (r0 >= RL || c0 + c >= a.cg) continue;
+#pragma unroll 8
+      for (int i = r0; i < live; i += RL) {
+        const float2 p = *reinterpret_cast<const float2*>(ws + ((int64_t)i * a.C + g * a.cg + c0 + c) * 2);
+        const float d = p.x - x;
+        y += fmaf((float)(min(n, (i + 1) * a.rows) - i * a.rows), d * d, p.y);
+      }
+    }
+    y = rsqrtf(block_sum256(y, red[1]) * inv + a.eps);
   }
   if (tid == 0) {
     float* st = (BWD ? gw : a.stats) + ((int64_t)b * a.G + g) * 2;
-    if constexpr (BWD) {
-      const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
-      st[0] = red[1][0] * inv;
-      st[1] = red[2][0] * inv;
-    } else {
-      st[0] = red[1][0];
-      st[1] = n > 0 ? rsqrtf(red[2][0] / red[0][0] + a.eps) : 0.f;
-    }
+    st[0] = n > 0 ? x : 0.f;
+    st[1] = n > 0 ? y : 0.f;
   }
 }
 
-// Elementwise part.  grid (chunks, slabs, B).
+// Elementwise part.  grid (chunks, slabs, B), walked from the end: the rows that the sums read last are those that the memory-side
+// cache still holds.
 template <bool B16, int V, int ACT, bool BWD>
 __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw) {
   constexpr int T = 256;
-  const int b = blockIdx.z, c0 = blockIdx.y * a.slab, tid = threadIdx.x;
+  const int b = a.B - 1 - blockIdx.z, c0 = blockIdx.y * a.slab, tid = threadIdx.x;
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv, c = c0 + col * V;
   if (rl >= RL) return;
-  const int n = gn_len(a.len, b, a.L), t0 = blockIdx.x * a.rows, t1 = min(a.L, t0 + a.rows);
-  float ga[V], be[V], mean[V], rstd[V], m1[V], m2[V];
+  const int n = gn_len(a.len, b, a.L), t0 = (a.chunks - 1 - (int)blockIdx.x) * a.rows, t1 = min(a.L, t0 + a.rows);
+  float ga[V], be[V], R[V], S[V], m1[V], m2[V];          // xh = R x + S; forward: z = R x + S, gamma and beta included
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int64_t g = ((int64_t)b * a.G + (c + j) / a.cg) * 2;
     ga[j] = a.gamma[c + j];
     be[j] = a.beta[c + j];
-    mean[j] = a.stats[g];
-    rstd[j] = a.stats[g + 1];
+    R[j] = BWD ? a.stats[g + 1] : a.stats[g + 1] * ga[j];
+    S[j] = BWD ? -a.stats[g] * R[j] : fmaf(-a.stats[g], R[j], be[j]);
     if constexpr (BWD) { m1[j] = gw[g]; m2[j] = gw[g + 1]; }
   }
   const int64_t x0 = b * a.xb + c, g0 = b * a.db + c, o0 = b * a.ob + c;
@@ -431,12 +515,12 @@ __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw)
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = (xr[u].get(j) - mean[j]) * rstd[j];
+        const float h = fmaf(xr[u].get(j), R[j], S[j]);
         if constexpr (BWD) {
-          const float dz = gr[u].get(j) * act_slope<ACT>(xh * ga[j] + be[j]);
-          y[j] = r < n ? rstd[j] * (dz * ga[j] - m1[j] - xh * m2[j]) : 0.f;
+          const float dz = gr[u].get(j) * act_slope<ACT>(fmaf(h, ga[j], be[j]));
+          y[j] = r < n ? R[j] * (fmaf(dz, ga[j], -m1[j]) - h * m2[j]) : 0.f;
         } else {
-          y[j] = r < n ? act_of<ACT>(xh * ga[j] + be[j]) : 0.f;
+          y[j] = r < n ? act_of<ACT>(h) : 0.f;
         }
       }
       put<B16, V>(a.out, o0 + (int64_t)r * a.ol, y);
@@ -444,27 +528,19 @@ __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw)
   }
 }
 
-// dgamma, dbeta: the sums of `parts` rows of ws [parts, C, 2], a block per 32 channels (8 row lanes), in a fixed order.
-__global__ __launch_bounds__(256) void gn_params_kernel(GArgs a, int64_t parts) {
-  __shared__ float red[2][8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+// dgamma, dbeta: the items' channel sums pw [B, C, 2] added in order.
+__global__ __launch_bounds__(256) void gn_params_kernel(GArgs a, const float* pw) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.C) return;
   float x = 0.f, y = 0.f;
-  if (c < a.C) {
 #pragma unroll 8
-    for (int64_t p = r; p < parts; p += 8) {
-      const float2 v = *reinterpret_cast<const float2*>(a.ws + (p * a.C + c) * 2);
-      x += v.x;
-      y += v.y;
-    }
+  for (int b = 0; b < a.B; ++b) {
+    const float2 v = *reinterpret_cast<const float2*>(pw + ((int64_t)b * a.C + c) * 2);
+    x += v.x;
+    y += v.y;
   }
-  red[0][r][threadIdx.x & 31] = x;
-  red[1][r][threadIdx.x & 31] = y;
-  __syncthreads();
-  if (r == 0 && c < a.C) {
-    for (int i = 1; i < 8; ++i) { x += red[0][i][threadIdx.x]; y += red[1][i][threadIdx.x]; }
-    a.dbeta[c] = x;
-    a.dgamma[c] = y;
-  }
+  a.dbeta[c] = x;
+  a.dgamma[c] = y;
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -477,36 +553,37 @@ struct GPlan { bool fused; int v, slab, slabs, chunks, rows, it, T; };
 
 int gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
-// bytes: of 16, what every row start and C divide; the plan depends on sizes alone besides it
 GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
   GPlan p = {};
   const int es = bf16 ? 2 : 4, cg = C / G;
   p.v = v;
-  // fused: the narrowest slab of whole groups and whole pieces whose rows are >= 128 bytes (a memory line)
+  // fused: a slab is whole groups and whole pieces, a memory line (128 bytes) wide where that gives a block per CU, else down to
+  // 32 bytes (the lines that slabs share are then shared in one XCD's cache)
   const int64_t unit = (int64_t)cg / gcd(cg, v) * v;
-  int64_t slab = unit * ((128 / es + unit - 1) / unit);
-  if (slab > C) slab = C;
-  const int64_t cv = slab / v;
-  const int it_max = bwd ? 8 : 16;
-  for (int T = 256; T <= 1024 && !p.fused; T *= 4) {
-    if (cv > T || slab > 1024) continue;
-    const int64_t it = (L + T / cv - 1) / (T / cv);
-    if (it <= (T == 256 ? 4 : it_max)) {
-      p.fused = true;
-      p.T = T;
-      p.it = it <= 4 ? 4 : it <= 8 ? 8 : 16;
+  const int it_max = bwd ? (bf16 && v == 8 ? 4 : 8) : 16;         // (rows a thread holds without spilling)
+  for (int line = 128; line >= 32 && !p.fused; line >>= 1) {
+    int64_t slab = unit * ((line / es + unit - 1) / unit);
+    if (slab > C) slab = C;
+    const int64_t cv = slab / v, slabs = (C + slab - 1) / slab;
+    if (line > 32 && B * slabs < 256 && slab > unit) continue;
+    for (int T = 256; T <= 1024 && !p.fused; T *= 4) {
+      if (cv > T || slab > 1024) continue;
+      const int64_t it = (L + T / cv - 1) / (T / cv);
+      if (it <= (T == 256 ? 4 : it_max)) {
+        p.fused = true;
+        p.T = T;
+        p.it = it <= 4 ? 4 : it <= 8 ? 8 : 16;
+        p.slab = (int)slab;
+        p.slabs = (int)slabs;
+      }
     }
   }
-  if (p.fused) {
-    p.slab = (int)slab;
-    p.slabs = (int)((C + slab - 1) / slab);
-    return p;
-  }
+  if (p.fused) return p;
   const int wide = 256 * v;
   p.slab = C < wide ? C : wide;
   p.slabs = (C + p.slab - 1) / p.slab;
-  // chunks: about 1024 blocks, at least 32 rows each
-  int64_t ch = (1024 + (int64_t)B * p.slabs - 1) / ((int64_t)B * p.slabs);
+  // chunks: about 2048 blocks, at least 32 rows each
+  int64_t ch = (2048 + (int64_t)B * p.slabs - 1) / ((int64_t)B * p.slabs);
   if (ch > (L + 31) / 32) ch = (L + 31) / 32;
   if (ch < 1) ch = 1;
   p.rows = (int)((L + ch - 1) / ch);
@@ -536,16 +613,16 @@ GArgs gn_args(const styler_gn_t* x, const GPlan& p) {
   a.x = x->x; a.dy = x->dy; a.out = x->out; a.gamma = x->gamma; a.beta = x->beta; a.stats = x->stats; a.dgamma = x->dgamma;
   a.dbeta = x->dbeta; a.len = x->len; a.xb = x->xb; a.xl = x->xl; a.db = x->db; a.dl = x->dl; a.ob = x->ob; a.ol = x->ol;
   a.B = x->B; a.L = x->L; a.C = x->C; a.G = x->G; a.cg = x->C / x->G; a.eps = x->eps;
-  a.chunks = p.chunks; a.rows = p.rows; a.slab = p.slab;
+  a.chunks = p.chunks; a.rows = p.rows; a.slab = p.slab; a.slabs = p.slabs;
   return a;
 }
 
 template <bool B16, int V, int ACT, bool BWD>
 void gn_launch(const GArgs& a, const GPlan& p, float* gw, hipStream_t st) {
   if (p.fused) {
-    const int red = p.T * V > 2 * p.slab ? p.T * V : 2 * p.slab;
-    const size_t lds = (size_t)(red + 4 * p.slab) * 4;     // 56 KB at most
-    const dim3 grid(p.slabs, a.B);
+    const int red = p.T * V > p.slab ? p.T * V : p.slab;
+    const size_t lds = (size_t)(red + 5 * p.slab) * 4;     // 52 KB at most
+    const dim3 grid((unsigned)((a.B + 7) / 8 * 8 * p.slabs));
 #define SLAB(IT, T) hipLaunchKernelGGL((gn_slab_kernel<B16, V, ACT, IT, T, BWD>), grid, dim3(T), lds, st, a)
     if (p.T == 256) SLAB(4, 256);
     else if (p.it == 4) SLAB(4, 1024);
@@ -557,7 +634,7 @@ void gn_launch(const GArgs& a, const GPlan& p, float* gw, hipStream_t st) {
   const dim3 grid(p.chunks, p.slabs, a.B);
   const size_t lds = (size_t)(256 * V + 2 * p.slab) * 4;
   hipLaunchKernelGGL((gn_sums_kernel<B16, V, ACT, BWD>), grid, dim3(256), lds, st, a);
-  hipLaunchKernelGGL((gn_join_kernel<BWD>), dim3(a.G, a.B), dim3(256), 0, st, a, gw);
+  hipLaunchKernelGGL((gn_join_kernel<BWD>), dim3(a.G, a.B), dim3(256), 0, st, a, gw, a.pw);
   hipLaunchKernelGGL((gn_write_kernel<B16, V, ACT, BWD>), grid, dim3(256), 0, st, a, (const float*)gw);
 }
 template <bool B16, int V, bool BWD>
@@ -584,27 +661,28 @@ void gn_dispatch(const GArgs& a, const GPlan& p, int bf16, int act, float* gw, h
 }  // namespace
 
 // The largest any vector width needs (the width depends on addresses, which the caller may not have yet): per-channel sums of
-// every chunk, the group means of the backward, and the forward's statistics where the caller keeps none.
+// every chunk, the group means and items' sums of the backward, and the forward's statistics where the caller keeps none.
 extern "C" int64_t styler_groupnorm_act_workspace_bytes(int B, int L, int C, int G, int bf16, int bwd) {
   if (B < 1 || L < 1 || C < 1 || G < 1 || C % G) return 0;
   int64_t most = 0;
   for (int v = bf16 ? 8 : 4; v >= 1; v >>= 1) {
     if (C % v) continue;
     const GPlan p = gn_plan(B, L, C, G, bf16, v, bwd != 0);
-    const int64_t n = p.fused ? (bwd ? (int64_t)B * C * 2 : 0) : (int64_t)B * p.chunks * C * 2;
+    const int64_t n = p.fused ? 0 : (int64_t)B * p.chunks * C * 2;
     if (n > most) most = n;
   }
-  return 4 * (most + 2 * (int64_t)B * G);
+  if (bwd) most += (int64_t)B * C * 2;
+  return most ? 4 * (most + 2 * (int64_t)B * G) : 0;
 }
 
 extern "C" int styler_groupnorm_act(const styler_gn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = gn_check(x, false)) return rc;
-  if (!workspace || workspace_bytes < styler_groupnorm_act_workspace_bytes(x->B, x->L, x->C, x->G, x->bf16, 0) || ((uintptr_t)workspace & 15))
-    return STYLER_EINVAL;
+  const int64_t need = styler_groupnorm_act_workspace_bytes(x->B, x->L, x->C, x->G, x->bf16, 0);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return STYLER_EINVAL;
   const GPlan p = gn_plan(x->B, x->L, x->C, x->G, x->bf16, gn_vec(x, false), false);
   GArgs a = gn_args(x, p);
   if (!a.stats && !p.fused) a.stats = (float*)workspace;
-  a.ws = (float*)workspace + 2 * (int64_t)x->B * x->G;
+  a.ws = workspace ? (float*)workspace + 2 * (int64_t)x->B * x->G : nullptr;
   gn_dispatch<false>(a, p, x->bf16, x->act, nullptr, (hipStream_t)stream);
   return launch_status();
 }
@@ -615,9 +693,9 @@ extern "C" int styler_groupnorm_act_bwd(const styler_gn_t* x, void* workspace, i
     return STYLER_EINVAL;
   const GPlan p = gn_plan(x->B, x->L, x->C, x->G, x->bf16, gn_vec(x, true), true);
   GArgs a = gn_args(x, p);
-  a.ws = (float*)workspace + 2 * (int64_t)x->B * x->G;
+  a.pw = (float*)workspace + 2 * (int64_t)x->B * x->G;
+  a.ws = a.pw + 2 * (int64_t)x->B * x->C;
   gn_dispatch<true>(a, p, x->bf16, x->act, (float*)workspace, (hipStream_t)stream);
-  hipLaunchKernelGGL(gn_params_kernel, dim3((x->C + 31) / 32), dim3(256), 0, (hipStream_t)stream, a,
-                     (int64_t)x->B * (p.fused ? 1 : p.chunks));
+  hipLaunchKernelGGL(gn_params_kernel, dim3((x->C + 255) / 256), dim3(256), 0, (hipStream_t)stream, a, (const float*)a.pw);
   return launch_status();
 }

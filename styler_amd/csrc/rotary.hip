@@ -6,7 +6,7 @@
 //
 // Angles.  pos * freq is formed in 64 bits, in turns, and reduced to (-1/2, 1/2] there: a position of 200 000 is 30 000 turns,
 // of which 32 bits keep three decimals.  The reduced angle goes to sincospi in 32 bits (no further reduction is needed).  A
-// thread computes the angles of its pairs once and applies them to several heads.
+// block forms the angles of its rows once, in LDS, one thread each; then all its threads stream the rows' heads.
 //
 // Bound by memory: every element is read and written once, in 16-byte pieces where layout and alignment allow.
 #include "common.h"
@@ -20,116 +20,132 @@ struct RArgs {
   const void* pos;
   int64_t xb, xl, xh, yb, yl, yh, posb;
   int64_t rows;
-  int L, H, D, rot, hpt, tpr, nrot, nslot, rpb;
+  int L, H, rot, nrot, nslot, rpb;
+  uint32_t mslot, mhead;                                 // magic numbers of nslot and H
   int pos_kind;                                          // 0: the row index, 1: int64, 2: fp32
   float gain, sign;
 };
 
-template <int N> struct Piece;                           // N 32-bit words
-template <> struct Piece<4> { typedef uint4 T; };
-template <> struct Piece<2> { typedef uint2 T; };
-template <> struct Piece<1> { typedef uint32_t T; };
+// i / d by a multiplication: m = floor(2^32 / d) + 1 is exact for i d < 2^32 (the host sees to it); d = 1 has m = 0
+__device__ __forceinline__ uint32_t div_magic(uint32_t i, uint32_t m) { return m ? __umulhi(i, m) : i; }
 
-// V consecutive elements of a bf16 or fp32 row
-template <bool B16, int V> struct Vec {
-  static constexpr int BYTES = V * (B16 ? 2 : 4);
-  float f[V];
+// V consecutive elements of a bf16 or fp32 row, kept as loaded
+template <bool B16, int V> struct Raw {
+  static constexpr int BYTES = V * (B16 ? 2 : 4), NW = (BYTES + 3) / 4;
+  uint32_t w[NW];
   __device__ __forceinline__ void load(const void* base, int64_t idx) {
-    if constexpr (B16 && V == 1) {
-      f[0] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(base)[idx] << 16);
-    } else {
-      typename Piece<BYTES / 4>::T raw = *reinterpret_cast<const typename Piece<BYTES / 4>::T*>(reinterpret_cast<const char*>(base) + idx * (B16 ? 2 : 4));
-      uint32_t w[BYTES / 4];
-      __builtin_memcpy(w, &raw, BYTES);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        f[i] = B16 ? __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) : __uint_as_float(w[i < BYTES / 4 ? i : 0]);
-    }
+    const char* p = reinterpret_cast<const char*>(base) + idx * (B16 ? 2 : 4);
+    if constexpr (BYTES == 16) { const uint4 u = *reinterpret_cast<const uint4*>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
+    else if constexpr (BYTES == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
+    else if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else w[0] = *reinterpret_cast<const uint16_t*>(p);
   }
   __device__ __forceinline__ void store(void* base, int64_t idx) const {
-    if constexpr (B16 && V == 1) {
-      reinterpret_cast<uint16_t*>(base)[idx] = (uint16_t)f32_to_bf16_bits(f[0]);
-    } else {
-      uint32_t w[BYTES / 4];
+    char* p = reinterpret_cast<char*>(base) + idx * (B16 ? 2 : 4);
+    if constexpr (BYTES == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (B16) return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __uint_as_float(w[i]);
+  }
+  __device__ __forceinline__ void set(const float (&f)[V]) {
 #pragma unroll
-      for (int i = 0; i < BYTES / 4; ++i) w[i] = B16 ? cvt_pk_bf16_rne(f[(2 * i) % V], f[(2 * i + 1) % V]) : __float_as_uint(f[i % V]);
-      typename Piece<BYTES / 4>::T raw;
-      __builtin_memcpy(&raw, w, BYTES);
-      *reinterpret_cast<typename Piece<BYTES / 4>::T*>(reinterpret_cast<char*>(base) + idx * (B16 ? 2 : 4)) = raw;
+    for (int i = 0; i < NW; ++i) {
+      if constexpr (!B16) w[i] = __float_as_uint(f[i]);
+      else if constexpr (V == 1) w[i] = f32_to_bf16_bits(f[0]);
+      else w[i] = cvt_pk_bf16_rne(f[2 * i], f[2 * i + 1]);
     }
   }
 };
 
-__device__ __forceinline__ void turn(double pos, double freq, float gain, float sign, float& c, float& s) {
-  const double t = pos * (freq * 0.15915494309189533577);      // turns (1 / 2 pi)
-  const float r = (float)(t - __builtin_rint(t));
-  float sn, cs;
-  sincospif(2.f * r, &sn, &cs);
-  c = cs * gain;
-  s = sn * gain * sign;
-}
-
-constexpr int UNROLL = 4;                                // heads whose loads are in flight together
-// A block covers rpb rows (item, position), tpr threads a row; a thread has one slot of the row -- V pairs (half layout) or V / 2
-// pairs (interleaved), or V features that pass through -- in hpt heads.  V: elements per access (interleaved and V = 1: the two
-// elements of a pair are read one by one, as the half layout's are).
+constexpr int UNROLL = 4;                                // items whose loads are in flight together
+// A block covers rpb rows (item, position).  An item is one slot of one head: V pairs (half layout; interleaved: the V / 2 pairs
+// of V consecutive features), or V features that pass through.  V: elements per access (interleaved and V = 1: the two elements
+// of a pair are read one by one, as the half layout's are).
 template <bool B16, bool INTER, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(RArgs a) {
   constexpr int NP = INTER ? (V + 1) / 2 : V;
   constexpr bool WHOLE = INTER && V > 1;                 // an access holds whole pairs
-  const int rib = threadIdx.x / a.tpr;
-  const int64_t row = (int64_t)blockIdx.x * a.rpb + rib;
-  if (rib >= a.rpb || row >= a.rows) return;
-  const int b = (int)(row / a.L), l = (int)(row - (int64_t)b * a.L);
-  const int h0 = blockIdx.y * a.hpt, h1 = min(a.H, h0 + a.hpt);
-  const int64_t x0 = b * a.xb + l * a.xl, y0 = b * a.yb + l * a.yl;
-  double pos = (double)l;
-  if (a.pos_kind == 1) pos = (double)reinterpret_cast<const int64_t*>(a.pos)[b * a.posb + l];
-  else if (a.pos_kind == 2) pos = (double)reinterpret_cast<const float*>(a.pos)[b * a.posb + l];
-  for (int slot = threadIdx.x - rib * a.tpr; slot < a.nslot; slot += a.tpr) {
-    if (slot >= a.nrot) {                                // features past rot
-      const int d = a.rot + (slot - a.nrot) * V;
-      for (int h = h0; h < h1; ++h) {
-        Vec<B16, V> u;
-        u.load(a.x, x0 + h * a.xh + d);
-        u.store(a.y, y0 + h * a.yh + d);
-      }
-      continue;
+  extern __shared__ __attribute__((aligned(16))) char sh[];
+  int64_t* from = reinterpret_cast<int64_t*>(sh);                        // [rpb] where the rows start in x and in y
+  int64_t* to = from + a.rpb;
+  float2* turns = reinterpret_cast<float2*>(to + a.rpb);                 // [rpb][rot / 2] (cos, sin), gain and sign applied
+  const int64_t r0 = (int64_t)blockIdx.x * a.rpb;
+  const int nrow = (int)min((int64_t)a.rpb, a.rows - r0), half = a.rot >> 1;
+  for (int r = threadIdx.x; r < nrow; r += 256) {
+    const uint32_t row = (uint32_t)(r0 + r), b = row / (uint32_t)a.L, l = row - b * a.L;
+    from[r] = b * a.xb + l * a.xl;
+    to[r] = b * a.yb + l * a.yl;
+  }
+  __syncthreads();
+  const uint32_t total = (uint32_t)nrow * a.H * a.nslot;
+  Raw<B16, V> u[UNROLL], w[WHOLE ? 1 : UNROLL];
+  int64_t at[UNROLL];                                    // where the item's first element goes in y
+  int tr[UNROLL];                                        // index of the item's first pair in turns, -1: passes through
+  auto fetch = [&](uint32_t i0) {
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const uint32_t i = min(i0 + k * 256, total - 1);
+      const uint32_t rh = div_magic(i, a.mslot), slot = i - rh * a.nslot, r = div_magic(rh, a.mhead), h = rh - r * a.H;
+      const bool turned = (int)slot < a.nrot;
+      const int d = turned ? slot * (INTER && V == 1 ? 2 : V) : a.rot + (slot - a.nrot) * V;
+      const int64_t x0 = from[r] + h * a.xh + d;
+      at[k] = to[r] + h * a.yh + d;
+      tr[k] = turned ? r * half + (INTER ? d / 2 : d) : -1;
+      u[k].load(a.x, x0);
+      if constexpr (!WHOLE) w[k].load(a.x, x0 + (turned ? (INTER ? 1 : half) : 0));
     }
-    const int d = slot * (INTER && V == 1 ? 2 : V), e = INTER ? d + 1 : d + a.rot / 2;     // e: where the second elements start
-    float c[NP], s[NP];
+  };
+  if (threadIdx.x < total) fetch(threadIdx.x);           // in flight while the angles are formed
+  for (int i = threadIdx.x; i < nrow * half; i += 256) {
+    const int r = i / half, p = i - r * half;
+    const uint32_t row = (uint32_t)(r0 + r), b = row / (uint32_t)a.L, l = row - b * a.L;
+    double pos = (double)l;
+    if (a.pos_kind == 1) pos = (double)reinterpret_cast<const int64_t*>(a.pos)[b * a.posb + l];
+    else if (a.pos_kind == 2) pos = (double)reinterpret_cast<const float*>(a.pos)[b * a.posb + l];
+    const double t = pos * (a.freq[p] * 0.15915494309189533577);         // turns (1 / 2 pi)
+    float sn, cs;
+    sincospif(2.f * (float)(t - __builtin_rint(t)), &sn, &cs);
+    turns[i] = make_float2(cs * a.gain, sn * a.gain * a.sign);
+  }
+  __syncthreads();
+  for (uint32_t i0 = threadIdx.x; i0 < total; i0 += 256 * UNROLL) {
+    if (i0 >= 256 * UNROLL) fetch(i0);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) turn(pos, a.freq[(INTER ? d / 2 : d) + i], a.gain, a.sign, c[i], s[i]);
-    for (int h = h0; h < h1; h += UNROLL) {
-      Vec<B16, V> u[UNROLL], w[WHOLE ? 1 : UNROLL];
-#pragma unroll
-      for (int k = 0; k < UNROLL; ++k) {
-        const int64_t p = x0 + (h + k < h1 ? h + k : h1 - 1) * a.xh;
-        u[k].load(a.x, p + d);
-        if constexpr (!WHOLE) w[k].load(a.x, p + e);
+    for (int k = 0; k < UNROLL; ++k) {
+      if (i0 + k * 256 >= total) break;
+      if (tr[k] < 0) {
+        u[k].store(a.y, at[k]);
+        continue;
       }
+      float2 t[NP];
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) {
-        if (h + k >= h1) break;
-        const int64_t p = y0 + (h + k) * a.yh;
-        if constexpr (WHOLE) {
-          Vec<B16, V> r;
+      for (int j = 0; j < NP; ++j) t[j] = turns[tr[k] + j];
+      float y[V];
+      if constexpr (WHOLE) {
 #pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            r.f[2 * i] = u[k].f[2 * i] * c[i] - u[k].f[2 * i + 1] * s[i];
-            r.f[2 * i + 1] = u[k].f[2 * i + 1] * c[i] + u[k].f[2 * i] * s[i];
-          }
-          r.store(a.y, p + d);
-        } else {
-          Vec<B16, V> r, q;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            r.f[i] = u[k].f[i] * c[i] - w[k].f[i] * s[i];
-            q.f[i] = w[k].f[i] * c[i] + u[k].f[i] * s[i];
-          }
-          r.store(a.y, p + d);
-          q.store(a.y, p + e);
+        for (int j = 0; j < NP; ++j) {
+          const float p = u[k].get(2 * j), q = u[k].get(2 * j + 1);
+          y[2 * j] = p * t[j].x - q * t[j].y;
+          y[2 * j + 1] = q * t[j].x + p * t[j].y;
         }
+        u[k].set(y);
+        u[k].store(a.y, at[k]);
+      } else {
+        float z[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float p = u[k].get(j), q = w[k].get(j);
+          y[j] = p * t[j].x - q * t[j].y;
+          z[j] = q * t[j].x + p * t[j].y;
+        }
+        u[k].set(y);
+        w[k].set(z);
+        u[k].store(a.y, at[k]);
+        w[k].store(a.y, at[k] + (INTER ? 1 : half));
       }
     }
   }
@@ -137,46 +153,49 @@ __global__ __launch_bounds__(256) void rotary_kernel(RArgs a) {
 
 }  // namespace
 
-extern "C" int styler_rotary(const void* x, int64_t xb, int64_t xl, int64_t xh, void* y, int64_t yb, int64_t yl, int64_t yh,
-                             const double* freqs, const void* pos, int64_t posb, int pos_kind, int B, int L, int H, int D, int rot,
-                             int interleaved, int inverse, float gain, int bf16, void* stream) {
-  if (!x || !y || !freqs || B < 1 || L < 1 || H < 1 || D < 2 || rot < 2 || rot > D || (rot & 1)) return STYLER_EINVAL;
-  if (pos_kind < 0 || pos_kind > 2 || (pos_kind != 0 && !pos)) return STYLER_EINVAL;
-  if ((int64_t)B * L > 0x7fffffff) return STYLER_EINVAL;
-  const int es = bf16 ? 2 : 4;
-  if (((uintptr_t)x | (uintptr_t)y) % es) return STYLER_EALIGN;
+extern "C" int styler_rotary(const styler_rotary_t* p, void* stream) {
+  if (!p || !p->x || !p->y || !p->freqs || p->B < 1 || p->L < 1 || p->H < 1 || p->D < 2) return STYLER_EINVAL;
+  const int rot = p->rot, H = p->H, D = p->D, es = p->bf16 ? 2 : 4;
+  if (rot < 2 || rot > D || (rot & 1) || D > 8192) return STYLER_EINVAL;         // (a row's angles: 32 KB of LDS at most)
+  if ((int64_t)p->B * p->L > 0x7fffffff) return STYLER_EINVAL;
+  if (p->pos_kind < 0 || p->pos_kind > 2 || (p->pos_kind != 0 && !p->pos)) return STYLER_EINVAL;
+  if (((uintptr_t)p->x | (uintptr_t)p->y) % es) return STYLER_EALIGN;
+  const int64_t st[] = {p->xb, p->xl, p->xh, p->yb, p->yl, p->yh};
+  const bool copy = rot < D && !(p->x == p->y && p->xb == p->yb && p->xl == p->yl && p->xh == p->yh);
   // elements per access: the widest of 16, 8, 4, 2 bytes that divides every offset a thread forms
   int v = 16 / es;
-  const bool copy = !(x == y && xb == yb && xl == yl && xh == yh) && rot < D;
   auto ok = [&](int n) {
-    const int64_t bytes = (int64_t)n * es;
-    if (((uintptr_t)x | (uintptr_t)y) % bytes) return false;
-    const int64_t st[] = {xb, xl, xh, yb, yl, yh};
+    if (((uintptr_t)p->x | (uintptr_t)p->y) % (n * es)) return false;
     for (int64_t s : st) if (s % n) return false;
-    if (interleaved ? rot % n : (rot / 2) % n) return false;
+    if (p->interleaved ? rot % n : (rot / 2) % n) return false;
     return !(copy && D % n);
   };
   while (v > 1 && !ok(v)) v >>= 1;
   RArgs a = {};
-  a.x = x; a.y = y; a.freq = freqs; a.pos = pos; a.xb = xb; a.xl = xl; a.xh = xh; a.yb = yb; a.yl = yl; a.yh = yh; a.posb = posb;
-  a.rows = (int64_t)B * L; a.L = L; a.H = H; a.D = D; a.rot = rot; a.pos_kind = pos_kind; a.gain = gain; a.sign = inverse ? -1.f : 1.f;
-  a.nrot = interleaved && v > 1 ? rot / v : rot / 2 / v;
+  a.x = p->x; a.y = p->y; a.freq = p->freqs; a.pos = p->pos; a.xb = p->xb; a.xl = p->xl; a.xh = p->xh; a.yb = p->yb; a.yl = p->yl;
+  a.yh = p->yh; a.posb = p->posb; a.rows = (int64_t)p->B * p->L; a.L = p->L; a.H = H; a.rot = rot; a.pos_kind = p->pos_kind;
+  a.gain = p->gain; a.sign = p->inverse ? -1.f : 1.f;
+  a.nrot = p->interleaved && v > 1 ? rot / v : rot / 2 / v;
   a.nslot = a.nrot + (copy ? (D - rot) / v : 0);
-  a.tpr = a.nslot < 256 ? a.nslot : 256;
-  a.rpb = 256 / a.tpr;
-  const int64_t blocks = (a.rows + a.rpb - 1) / a.rpb;
-  // heads per thread: all eight share one set of angles once the rows alone fill the chip; a few rows are spread over the
-  // heads instead
-  a.hpt = H < 8 ? H : 8;
-  while (a.hpt > 1 && blocks * ((H + a.hpt - 1) / a.hpt) < 512) a.hpt = (a.hpt + 1) / 2;
-  const dim3 grid((unsigned)blocks, (unsigned)((H + a.hpt - 1) / a.hpt));
-  hipStream_t st = (hipStream_t)stream;
-#define GO(B16, I, V) hipLaunchKernelGGL((rotary_kernel<B16, I, V>), grid, dim3(256), 0, st, a)
-  if (bf16) {
-    if (interleaved) { if (v == 8) GO(true, true, 8); else if (v == 4) GO(true, true, 4); else if (v == 2) GO(true, true, 2); else GO(true, true, 1); }
+  const int64_t per_row = (int64_t)H * a.nslot;
+  if (per_row * (H > a.nslot ? H : a.nslot) >= (int64_t)1 << 31) return STYLER_EINVAL;
+  a.mslot = a.nslot == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / a.nslot) + 1;
+  a.mhead = H == 1 ? 0 : (uint32_t)(((uint64_t)1 << 32) / H) + 1;
+  // rows per block: four items a thread, angles within 32 KB, and not fewer blocks than fill the chip several times over
+  int64_t rpb = 1024 / per_row;
+  if (rpb * (rot / 2) > 4096) rpb = 4096 / (rot / 2);
+  while (rpb > 1 && a.rows / rpb < 768) rpb >>= 1;
+  if (rpb < 1) rpb = 1;
+  a.rpb = (int)rpb;
+  const int64_t blocks = (a.rows + rpb - 1) / rpb;
+  const size_t lds = (size_t)rpb * (rot / 2 * 8 + 16);
+  hipStream_t s = (hipStream_t)stream;
+#define GO(B16, I, V) hipLaunchKernelGGL((rotary_kernel<B16, I, V>), dim3((unsigned)blocks), dim3(256), lds, s, a)
+  if (p->bf16) {
+    if (p->interleaved) { if (v == 8) GO(true, true, 8); else if (v == 4) GO(true, true, 4); else if (v == 2) GO(true, true, 2); else GO(true, true, 1); }
     else { if (v == 8) GO(true, false, 8); else if (v == 4) GO(true, false, 4); else if (v == 2) GO(true, false, 2); else GO(true, false, 1); }
   } else {
-    if (interleaved) { if (v == 4) GO(false, true, 4); else if (v == 2) GO(false, true, 2); else GO(false, true, 1); }
+    if (p->interleaved) { if (v == 4) GO(false, true, 4); else if (v == 2) GO(false, true, 2); else GO(false, true, 1); }
     else { if (v == 4) GO(false, false, 4); else if (v == 2) GO(false, false, 2); else GO(false, false, 1); }
   }
 #undef GO

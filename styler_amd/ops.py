@@ -5,13 +5,13 @@ function here hands raw device pointers + sizes to libstyler_hip.so.  Activation
 channels-last [B, L, C]; a channel slice `x[..., a:b]` of a wider buffer is a legal argument (the row
 stride travels as `ld`), which is how torch.cat / torch.split copies of the reference disappear."""
 import contextlib
-import ctypes
+import functools
 import math
 import os
 
 import torch
 
-from ._lib import GnArgs, XattnArgs, lib
+from ._lib import GN, ROTARY, XATTN, lib
 
 ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
 ACT_LEAKY = 4                      # leaky_relu(0.1), the vocoder's LRELU_SLOPE
@@ -1868,17 +1868,20 @@ def adam_step(p, g, m, v, sumsq_buf, max_norm, lr, beta1, beta2, eps, step, grad
 
 # ---- operators of a decoder block that reads an encoder's states: group norm + activation, rotary positions, cross attention --------
 # fp32 or bf16 tensors with their own strides; what a kernel cannot read in place (features not contiguous, rows not on 16 bytes) is
-# copied first.  They run on the current stream of the tensors' device, whichever device is current.
+# copied first.  They run on the current stream of the tensors' device, whichever device is current.  A token's call is bound by this
+# file: shapes, strides and types are looked at once each, and the arguments go over as one packed structure.
 _ON_CURRENT = contextlib.nullcontext()
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _refuse(name, what):
     raise StylerHipError(f"{name}: {what}")
 
 
-def _on(t):
-    """Makes t's device the current one for the launches and allocations inside."""
-    return _ON_CURRENT if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on(device):
+    """Makes `device` the current one for the launches inside."""
+    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _like(name, t, what, shape, dtype, device):
@@ -1889,70 +1892,86 @@ def _like(name, t, what, shape, dtype, device):
 
 
 def _vector(name, t, what, n, dtype, device):
-    return None if t is None else _like(name, t, what, (n,), dtype, device).contiguous()
+    """`t` [n], contiguous; None stays None."""
+    if t is None:
+        return None
+    _like(name, t, what, (n,), dtype, device)
+    return t if n < 2 or t.stride(0) == 1 else t.contiguous()
 
 
-def _main_type(name, t):
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        _refuse(name, f"float32 or bfloat16 expected, got {t.dtype}")
-    return 1 if t.dtype == torch.bfloat16 else 0
+def _addr(t):
+    return 0 if t is None else t.data_ptr()
 
 
-def _on_gpu(name, t):
-    if not t.is_cuda:
-        _refuse(name, "there is no CPU form")
+def _new(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _stride(t, i):
-    return t.stride(i) if t.shape[i] > 1 else 0
+def _rows_ok(shape, st):
+    """Inner dimension contiguous, no two rows in the same place (an output)."""
+    return (st[-1] == 1 or shape[-1] == 1) and not any(n > 1 and s == 0 for n, s in zip(shape, st))
 
 
-def _heads(t):
-    """[B, L, H, D] as the attention kernels read it: features contiguous, rows on 16 bytes, a tile's rows within 2^31 bytes."""
-    es = t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and _stride(t, 1) * es < 1 << 23 and \
-            all(_stride(t, i) * es % 16 == 0 for i in range(3)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _heads(t, es):
+    """(t, strides) of [B, L, H, D] as the attention kernels read it: features contiguous, rows on 16 bytes, a tile's rows (128)
+    within 2^31 bytes of each other; what is not gets copied."""
+    b, l, h, d = t.stride()
+    m = 16 // es - 1
+    if d == 1 and not (b & m or l & m or h & m) and l * es < 1 << 23 and not t.data_ptr() & 15:
+        return t, (b, l, h)
+    B, L, H, D = t.shape
+    b, l, h = b if B > 1 else 0, l if L > 1 else 0, h if H > 1 else 0        # (a stride that no step uses)
+    if d != 1 or b & m or l & m or h & m or l * es >= 1 << 23 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        b, l, h, _ = t.stride()
+    return t, (b, l, h)
 
 
-def _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale):
-    bf16 = _main_type(name, q)
-    if q.dim() != 4 or k.dim() != 4:
+@functools.lru_cache(maxsize=4096)
+def _xattn_ws(*sizes):
+    return lib.styler_cross_attention_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _gn_ws(*sizes):
+    return lib.styler_groupnorm_act_workspace_bytes(*sizes)
+
+
+def _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, writes):
+    bf16, qs, ks, device = _TYPES.get(q.dtype), q.shape, k.shape, q.device
+    if bf16 is None:
+        _refuse(name, f"float32 or bfloat16 expected, got {q.dtype}")
+    if len(qs) != 4 or len(ks) != 4:
         _refuse(name, "q [B, Lq, H, D] and k, v [B, Lk, G, D] expected")
-    B, Lq, H, D = q.shape
-    Lk, G = k.shape[1], k.shape[2]
-    _like(name, k, "k", (B, Lk, G, D), q.dtype, q.device)
-    _like(name, v, "v", (B, Lk, G, D), q.dtype, q.device)
+    B, Lq, H, D = qs
+    Lk, G = ks[1], ks[2]
+    _like(name, k, "k", (B, Lk, G, D), q.dtype, device)
+    _like(name, v, "v", ks, q.dtype, device)
     if G < 1 or H < 1 or H % G:
         _refuse(name, f"the query heads ({H}) must be a multiple of the key heads ({G})")
     if D % 8 or not 8 <= D <= 128:
         _refuse(name, f"head width {D}: a multiple of 8 up to 128 expected")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-30 < scale < 1e30:
         _refuse(name, f"scale {scale}: a positive finite number expected")
-    lens = _vector(name, lens, "lens", B, torch.int64, q.device)
-    q_lens = _vector(name, q_lens, "q_lens", B, torch.int64, q.device)
+    lens = _vector(name, lens, "lens", B, torch.int64, device)
+    q_lens = _vector(name, q_lens, "q_lens", B, torch.int64, device)
+    maskb = 0
     if mask is not None:
-        if mask.dtype != torch.bool or mask.device != q.device or mask.dim() != 2 or mask.shape[0] not in (1, B) or mask.shape[1] != Lk:
-            _refuse(name, f"mask must be bool [{B} or 1, {Lk}] on {q.device} (True: a key that is not seen)")
+        if mask.dtype != torch.bool or mask.device != device or mask.dim() != 2 or mask.shape[0] not in (1, B) or mask.shape[1] != Lk:
+            _refuse(name, f"mask must be bool [{B} or 1, {Lk}] on {device} (True: a key that is not seen)")
         if Lk > 1 and mask.stride(1) != 1:
             mask = mask.contiguous()
-    _like(name, out, "out", (B, Lq, H, D), q.dtype, q.device)
-    if lse is not None and not _like(name, lse, "lse", (B, H, Lq), torch.float32, q.device).is_contiguous():
+        maskb = mask.stride(0) if mask.shape[0] > 1 else 0
+    if lse is not None and not _like(name, lse, "lse", (B, H, Lq), torch.float32, device).is_contiguous():
         _refuse(name, "lse must be contiguous")
-    _on_gpu(name, q)
-    q, k, v = _heads(q), _heads(k), _heads(v)
-    a = XattnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, _ptr(lse), _ptr(lens),
-                  _ptr(q_lens), _ptr(mask),
-                  _stride(q, 0), _stride(q, 1), _stride(q, 2), _stride(k, 0), _stride(k, 1), _stride(k, 2),
-                  _stride(v, 0), _stride(v, 1), _stride(v, 2), _stride(out, 0), _stride(out, 1), _stride(out, 2), 0, 0, 0,
-                  0 if mask is None or mask.shape[0] == 1 else mask.stride(0), B, Lq, Lk, H, G, D, bf16, scale)
-    return a, (q, k, v, lens, q_lens, mask)              # (the second: what must outlive the launch's enqueueing)
-
-
-def _workspace(n, device):
-    return torch.empty(n, device=device, dtype=torch.uint8) if n else None
+    if out is not None:
+        _like(name, out, "out", qs, q.dtype, device)
+        if writes and not (_rows_ok(qs, out.stride()) and _heads(out, 2 if bf16 else 4)[0] is out):
+            _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
+    if not q.is_cuda:
+        _refuse(name, "there is no CPU form")
+    return (B, Lq, Lk, H, G, D, bf16), scale, lens, q_lens, mask, maskb
 
 
 def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, out=None, lse=None):
@@ -1961,23 +1980,24 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
 
     lens int64 [B]: keys at or past it are not seen; mask bool [B or 1, Lk]: True = not seen.  What stands in rows that are not
     seen is never used.  q_lens int64 [B]: queries at or past it, like queries that see no key, give zeros and lse = -inf.
-    lse (optional, fp32 [B, H, Lq]) receives the logarithm of the softmax's denominator, which cross_attention_bwd needs."""
+    lse (optional, fp32 [B, H, Lq]) receives the logarithm of the softmax's denominator, which cross_attention_bwd needs.
+    out (optional): the result's tensor, which shares no memory with the inputs."""
     name = "cross_attention"
-    if q.dim() != 4:
-        _refuse(name, "q [B, Lq, H, D] expected")
+    sizes, scale, lens, q_lens, mask, maskb = _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, True)
+    es = 2 if sizes[6] else 4
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    elif out.dim() != 4 or out.stride(3) != 1 or _heads(out) is not out or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(4)):
-        _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
-    a, keep = _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale)
-    if out.numel() == 0 or a.Lk == 0:
+        out = _new(q)
+    if out.numel() == 0 or sizes[2] == 0:
         if lse is not None:
             lse.fill_(-math.inf)
         return out.zero_()
-    with _on(q):
-        n = lib.styler_cross_attention_workspace_bytes(a.B, a.Lq, a.Lk, a.H, a.G, a.D, a.bf16, 0)
-        ws = _workspace(n, q.device)
-        _chk(lib.styler_cross_attention(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_cross_attention")
+    (q, qt), (k, kt), (v, vt) = _heads(q, es), _heads(k, es), _heads(v, es)
+    n = _xattn_ws(*sizes, 0)
+    with _on(q.device):
+        ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+        args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _addr(lse), _addr(lens),
+                          _addr(q_lens), _addr(mask), *qt, *kt, *vt, *_heads(out, es)[1], 0, 0, 0, maskb, *sizes, scale)
+        _chk(lib.styler_cross_attention(args, _addr(ws), n, _raw_stream(q.device.index)), "styler_cross_attention")
     return out
 
 
@@ -1988,21 +2008,20 @@ def cross_attention_bwd(q, k, v, out, dout, lse, lens=None, *, q_lens=None, mask
     name = "cross_attention_bwd"
     if lse is None:
         _refuse(name, "the forward's lse is needed")
-    if out.dim() != 4 or q.dim() != 4:
-        _refuse(name, "q and out [B, Lq, H, D] expected")
     _like(name, dout, "dout", q.shape, q.dtype, q.device)
-    out, dout, lse = _heads(out), _heads(dout), lse.contiguous()
-    a, keep = _xattn_args(name, q, k, v, out, lse, lens, q_lens, mask, scale)
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    dk, dv = torch.empty(k.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=q.device, dtype=q.dtype)
-    if q.numel() == 0 or k.numel() == 0:
+    sizes, scale, lens, q_lens, mask, maskb = _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, False)
+    es = 2 if sizes[6] else 4
+    dq, dk, dv = _new(q), _new(k), _new(k)
+    if dq.numel() == 0 or dk.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.gb, a.gl, a.gh = _stride(dout, 0), _stride(dout, 1), _stride(dout, 2)
-    with _on(q):
-        n = lib.styler_cross_attention_workspace_bytes(a.B, a.Lq, a.Lk, a.H, a.G, a.D, a.bf16, 1)
-        ws = _workspace(n, q.device)
-        _chk(lib.styler_cross_attention_bwd(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_cross_attention_bwd")
+    (q, qt), (k, kt), (v, vt), (out, ot), (dout, gt) = (_heads(t, es) for t in (q, k, v, out, dout))
+    n = _xattn_ws(*sizes, 1)
+    with _on(q.device):
+        ws = torch.empty(n, device=q.device, dtype=torch.uint8)
+        args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                          dv.data_ptr(), lse.data_ptr(), _addr(lens), _addr(q_lens), _addr(mask), *qt, *kt, *vt, *ot, *gt, maskb,
+                          *sizes, scale)
+        _chk(lib.styler_cross_attention_bwd(args, ws.data_ptr(), n, _raw_stream(q.device.index)), "styler_cross_attention_bwd")
     return dq, dk, dv
 
 
@@ -2038,65 +2057,86 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
     [B or 1, L]; None: 0 .. L - 1.  Angles are formed in 64 bits.  inverse: the opposite turn, i.e. dx from dy.
     out (optional): the result's tensor; out=x works in place, any other overlap with x does not."""
     name = "rotary"
-    bf16 = _main_type(name, x)
-    if x.dim() != 4:
+    bf16, shape, device, n = _TYPES.get(x.dtype), x.shape, x.device, freqs.numel()
+    if bf16 is None:
+        _refuse(name, f"float32 or bfloat16 expected, got {x.dtype}")
+    if len(shape) != 4:
         _refuse(name, "x [B, L, H, D] expected")
-    B, L, H, D = x.shape
-    if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != x.device or not 2 <= 2 * freqs.numel() <= D:
-        _refuse(name, f"freqs must be float64 [up to {D // 2}] on {x.device}")
-    freqs = freqs.contiguous()
+    B, L, H, D = shape
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != device or not 2 <= 2 * n <= D:
+        _refuse(name, f"freqs must be float64 [up to {D // 2}] on {device}")
     kind, posb = 0, 0
     if pos is not None:
-        if pos.dtype not in (torch.int64, torch.float32) or pos.device != x.device or pos.dim() not in (1, 2) or \
-                pos.shape[-1] != L or (pos.dim() == 2 and pos.shape[0] not in (1, B)):
-            _refuse(name, f"pos must be int64 or float32 [{L}] or [{B} or 1, {L}] on {x.device}")
+        ps, pt = pos.shape, pos.dtype
+        kind = 1 if pt == torch.int64 else 2
+        if (kind == 2 and pt != torch.float32) or pos.device != device or len(ps) not in (1, 2) or ps[-1] != L or \
+                (len(ps) == 2 and ps[0] not in (1, B)):
+            _refuse(name, f"pos must be int64 or float32 [{L}] or [{B} or 1, {L}] on {device}")
         if L > 1 and pos.stride(-1) != 1:
             pos = pos.contiguous()
-        kind = 1 if pos.dtype == torch.int64 else 2
-        posb = pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else 0
+        if len(ps) == 2 and ps[0] > 1:
+            posb = pos.stride(0)
     if not math.isfinite(gain):
         _refuse(name, f"gain {gain}: a finite number expected")
-    if out is not None:
-        _like(name, out, "out", x.shape, x.dtype, x.device)
-        if out.stride(3) != 1 or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(3)):
-            _refuse(name, "out must have contiguous features and distinct rows")
-    _on_gpu(name, x)
+    if out is not None and not _rows_ok(_like(name, out, "out", shape, x.dtype, device).shape, out.stride()):
+        _refuse(name, "out must have contiguous features and distinct rows")
+    if not x.is_cuda:
+        _refuse(name, "there is no CPU form")
     if x.stride(3) != 1:
         x = x.contiguous()
+    if freqs.stride(0) != 1:
+        freqs = freqs.contiguous()
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = _new(x)
     if x.numel() == 0:
         return out
-    with _on(x):
-        _chk(lib.styler_rotary(x.data_ptr(), _stride(x, 0), _stride(x, 1), _stride(x, 2), out.data_ptr(), _stride(out, 0),
-                               _stride(out, 1), _stride(out, 2), freqs.data_ptr(), _ptr(pos), posb, kind, B, L, H, D,
-                               2 * freqs.numel(), 1 if interleaved else 0, 1 if inverse else 0, float(gain), bf16, _stream()),
-             "styler_rotary")
+    xb, xl, xh, _ = x.stride()
+    yb, yl, yh, _ = out.stride()
+    if B == 1:
+        xb = yb = 0
+    if L == 1:
+        xl = yl = 0
+    if H == 1:
+        xh = yh = 0
+    with _on(device):
+        args = ROTARY.pack(x.data_ptr(), out.data_ptr(), freqs.data_ptr(), _addr(pos), xb, xl, xh, yb, yl, yh, posb, B, L, H, D, 2 * n,
+                           kind, 1 if interleaved else 0, 1 if inverse else 0, bf16, gain)
+        _chk(lib.styler_rotary(args, _raw_stream(device.index)), "styler_rotary")
     return out
 
 
-def _gn_args(name, x, gamma, beta, groups, act, eps, lens, stats):
-    bf16 = _main_type(name, x)
-    if x.dim() != 3:
+def _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, other, what):
+    bf16, shape, device = _TYPES.get(x.dtype), x.shape, x.device
+    if bf16 is None:
+        _refuse(name, f"float32 or bfloat16 expected, got {x.dtype}")
+    if len(shape) != 3:
         _refuse(name, "x [B, L, C] expected")
-    B, L, C = x.shape
+    B, L, C = shape
     if groups < 1 or C < 1 or C % groups:
         _refuse(name, f"{C} channels do not divide into {groups} groups")
     if act not in (ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU):
         _refuse(name, f"activation {act}: ACT_NONE, ACT_RELU, ACT_SILU or ACT_GELU expected")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+    if not 0.0 <= eps < math.inf:
         _refuse(name, f"eps {eps}: a number >= 0 expected")
-    gamma = _vector(name, gamma, "gamma", C, torch.float32, x.device)
-    beta = _vector(name, beta, "beta", C, torch.float32, x.device)
-    lens = _vector(name, lens, "lens", B, torch.int64, x.device)
-    if stats is not None and not _like(name, stats, "stats", (B, groups, 2), torch.float32, x.device).is_contiguous():
+    gamma = _vector(name, gamma, "gamma", C, torch.float32, device)
+    beta = _vector(name, beta, "beta", C, torch.float32, device)
+    lens = _vector(name, lens, "lens", B, torch.int64, device)
+    if stats is not None and not _like(name, stats, "stats", (B, groups, 2), torch.float32, device).is_contiguous():
         _refuse(name, "stats must be contiguous")
-    _on_gpu(name, x)
-    if x.stride(2) != 1 and C > 1:
-        x = x.contiguous()
-    a = GnArgs(x.data_ptr(), None, None, gamma.data_ptr(), beta.data_ptr(), _ptr(stats), None, None, _ptr(lens),
-               _stride(x, 0), _stride(x, 1), 0, 0, 0, 0, B, L, C, groups, act, bf16, eps)
-    return a, (x, gamma, beta, lens)
+    if other is not None:
+        _like(name, other, what, shape, x.dtype, device)
+    if not x.is_cuda:
+        _refuse(name, "there is no CPU form")
+    return (B, L, C, groups), bf16, gamma, beta, lens
+
+
+def _gn_rows(t, B, L, C):
+    """(t, item stride, row stride) with contiguous channels."""
+    b, l, c = t.stride()
+    if c != 1 and C > 1:
+        t = t.contiguous()
+        b, l, c = t.stride()
+    return t, b if B > 1 else 0, l if L > 1 else 0
 
 
 def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, out=None, stats=None):
@@ -2105,20 +2145,21 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
     groupnorm_act_bwd.  out (optional) may be x."""
     name = "groupnorm_act"
-    a, keep = _gn_args(name, x, gamma, beta, groups, act, eps, lens, stats)
+    sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, out, "out")
+    B, L, C, _ = sizes
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    else:
-        _like(name, out, "out", x.shape, x.dtype, x.device)
-        if (a.C > 1 and out.stride(2) != 1) or any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(2)):
-            _refuse(name, "out must have contiguous channels and distinct rows")
+        out = _new(x)
+    elif not _rows_ok(out.shape, out.stride()):
+        _refuse(name, "out must have contiguous channels and distinct rows")
     if out.numel() == 0:
         return out
-    a.out, a.ob, a.ol = out.data_ptr(), _stride(out, 0), _stride(out, 1)
-    with _on(x):
-        n = lib.styler_groupnorm_act_workspace_bytes(a.B, a.L, a.C, a.G, a.bf16, 0)
-        ws = _workspace(n, x.device)
-        _chk(lib.styler_groupnorm_act(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_groupnorm_act")
+    (x, xb, xl), (_, ob, ol) = _gn_rows(x, B, L, C), _gn_rows(out, B, L, C)
+    n = _gn_ws(*sizes, bf16, 0)
+    with _on(x.device):
+        ws = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
+        args = GN.pack(x.data_ptr(), 0, out.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _addr(stats), 0, 0, _addr(lens),
+                       xb, xl, 0, 0, ob, ol, *sizes, act, bf16, eps)
+        _chk(lib.styler_groupnorm_act(args, _addr(ws), n, _raw_stream(x.device.index)), "styler_groupnorm_act")
     return out
 
 
@@ -2128,18 +2169,16 @@ def groupnorm_act_bwd(x, dy, gamma, beta, stats, groups, act=ACT_SILU, *, lens=N
     name = "groupnorm_act_bwd"
     if stats is None:
         _refuse(name, "the forward's stats are needed")
-    a, keep = _gn_args(name, x, gamma, beta, groups, act, 0.0, lens, stats)
-    dy = _like(name, dy, "dy", x.shape, x.dtype, x.device)
-    if dy.stride(2) != 1 and a.C > 1:
-        dy = dy.contiguous()
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    dgamma, dbeta = torch.empty(a.C, device=x.device), torch.empty(a.C, device=x.device)
+    sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, 0.0, lens, stats, dy, "dy")
+    B, L, C, _ = sizes
+    dx, dgamma, dbeta = _new(x), _new(gamma), _new(gamma)
     if dx.numel() == 0:
         return dx, dgamma.zero_(), dbeta.zero_()
-    a.dy, a.out, a.dgamma, a.dbeta = dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr()
-    a.db, a.dl, a.ob, a.ol = _stride(dy, 0), _stride(dy, 1), _stride(dx, 0), _stride(dx, 1)
-    with _on(x):
-        n = lib.styler_groupnorm_act_workspace_bytes(a.B, a.L, a.C, a.G, a.bf16, 1)
-        ws = _workspace(n, x.device)
-        _chk(lib.styler_groupnorm_act_bwd(ctypes.byref(a), _ptr(ws), n, _stream()), "styler_groupnorm_act_bwd")
+    (x, xb, xl), (dy, db, dl), (_, ob, ol) = _gn_rows(x, B, L, C), _gn_rows(dy, B, L, C), _gn_rows(dx, B, L, C)
+    n = _gn_ws(*sizes, bf16, 1)
+    with _on(x.device):
+        ws = torch.empty(n, device=x.device, dtype=torch.uint8)
+        args = GN.pack(x.data_ptr(), dy.data_ptr(), dx.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
+                       dgamma.data_ptr(), dbeta.data_ptr(), _addr(lens), xb, xl, db, dl, ob, ol, *sizes, act, bf16, 0.0)
+        _chk(lib.styler_groupnorm_act_bwd(args, ws.data_ptr(), n, _raw_stream(x.device.index)), "styler_groupnorm_act_bwd")
     return dx, dgamma, dbeta
