@@ -259,6 +259,34 @@ __device__ __forceinline__ void store_zero(T* row, int D, int lh) {
   }
 }
 
+// A wave's 32 rows of acc times the lanes' c -> memory, whole rows at a time: the accumulator holds 4 features of a row per lane, so
+// stored directly a wave would touch 32 rows with 8 or 16 bytes each, 4 DT / 32 times over.  `lds`: 32 * DT * sizeof(To) bytes of the
+// wave's own (a tile buffer that every wave has finished with).  at(row): where row 0..31 goes, nullptr = not stored.  Lanes with
+// keep = false store zeros (whatever their accumulators hold).
+template <typename To, int DT, typename At>
+__device__ __forceinline__ void store_tile(char* lds, const f32x16 (&acc)[DT / 32], int D, int lane, float c, bool keep, At at) {
+  constexpr int RB = DT * sizeof(To), LPR = RB / 16, RPI = 64 / LPR;         // lanes per row, rows per instruction
+  const int li = lane & 31, lh = lane >> 5;
+#pragma unroll
+  for (int dt = 0; dt < DT / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float x = keep ? acc[dt][g * 4] * c : 0.f, y = keep ? acc[dt][g * 4 + 1] * c : 0.f;
+      const float z = keep ? acc[dt][g * 4 + 2] * c : 0.f, w = keep ? acc[dt][g * 4 + 3] * c : 0.f;
+      const int byte = (dt * 32 + g * 8 + lh * 4) * sizeof(To);
+      char* p = lds + li * RB + (((byte / 16) ^ Swz<RB>::of(li)) * 16 + byte % 16);
+      if constexpr (sizeof(To) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(cvt_pk_bf16_rne(x, y), cvt_pk_bf16_rne(z, w));
+      else *reinterpret_cast<float4*>(p) = make_float4(x, y, z, w);
+    }
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int row = i * RPI + lane / LPR, d = (lane % LPR) * (16 / (int)sizeof(To));
+    const uint4 u = *reinterpret_cast<const uint4*>(lds + row * RB + (((lane % LPR) ^ Swz<RB>::of(row)) * 16));
+    To* p = at(row);
+    if (p && d < D) *reinterpret_cast<uint4*>(p + d) = u;
+  }
+}
+
 // The seen keys of a tile as bit words, 32 keys each (uniform over the wave).  Without a mask they follow from the length; with
 // one, lane i holds the mask bytes of keys i and (tiles of 128) 64 + i, fetched one tile before they are needed.
 template <int KT> struct KeyWords {
@@ -304,18 +332,42 @@ template <bool FEW, int KT> __device__ __forceinline__ uint32_t few_word(const K
   }
   return w;
 }
-// Scores start at 0 for a seen key and at -inf for one that is not: its row was filled with zeros, so the product adds 0 and the
-// mask costs nothing after it.
-__device__ __forceinline__ void seen_start(f32x16& s, uint32_t w, int lh) {
-  zero16(s);
-  if (w != 0xffffffffu) {
-    const int un = (int)(~w >> (4 * lh));
+// Scores start at 0 for a seen key and at -inf for one that is not (its row was filled with zeros, so the product adds 0): the mask
+// is the accumulator's first value, read from LDS, and costs nothing after it.  Only tiles that have unseen keys write and read it.
+template <int KT>
+__device__ __forceinline__ void start_put(float* start, const KeyWords<KT> k, int tid) {
+  uint32_t all = k.w[0], w = k.w[0];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int bit = (r & 3) + 8 * (r >> 2);
-      s[r] = __int_as_float(__builtin_amdgcn_sbfe(un, bit, 1) & 0xff800000);
-    }
+  for (int i = 1; i < KT / 32; ++i) {
+    all &= k.w[i];
+    w = (tid >> 5) == i ? k.w[i] : w;
   }
+  if (all != 0xffffffffu && tid < KT) start[tid] = (w >> (tid & 31)) & 1u ? 0.f : -INFINITY;
+}
+// s = tile rows (blk * 32 ..) . f + that start (two copies of the product: a full tile's starts at the constant 0, without a register)
+template <typename T, int DT>
+__device__ __forceinline__ void mma_rows_seen(f32x16& s, const char* tile, int blk, const Frag<T, DT>& f, const float* start, uint32_t w, int li,
+                                              int lh) {
+  if (w == 0xffffffffu) {
+    zero16(s);
+    mma_rows<T, DT>(s, tile, blk, f, li, lh);
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 x = *reinterpret_cast<const float4*>(start + g * 8 + lh * 4);
+      s[g * 4] = x.x; s[g * 4 + 1] = x.y; s[g * 4 + 2] = x.z; s[g * 4 + 3] = x.w;
+    }
+    mma_rows<T, DT>(s, tile, blk, f, li, lh);
+  }
+}
+// the other half wave's value joined in: lane and lane ^ 32 hold the same row
+__device__ __forceinline__ float both_max(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
 // rows of keys per tile (shared-tile kernels) such that two tiles of K and V stay within 64 KB where two blocks per CU pay
@@ -332,12 +384,13 @@ __device__ __forceinline__ void tile_range(int n, int s, int S, int& t0, int& t1
 // FEW = true (M <= 32): all waves hold the same 32 rows and a wave takes 32 of the tile's 128 keys -- every wave works where
 // a block of rows would leave three idle; the four partial softmaxes are joined through LDS.
 template <typename T, int DT, bool FEW>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fwd_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <= 128 && !FEW ? 4 : 2)) void xattn_fwd_kernel(XArgs a) {
   constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
   constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM + (FEW ? 1152 : 0)];
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (FEW ? 1152 : 0)];
+  float* start = reinterpret_cast<float*>(smem + SMEM);          // [buffer][KT], see start_put
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
@@ -378,6 +431,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
     dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
     dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
+    start_put(start + buf * KT, kw, tid);
   };
   fill(t0, 0, cur);
   Frag<T, DT> qf;
@@ -403,18 +457,19 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
       const char* tk = smem + buf * 2 * TILE;
       const char* tv = tk + TILE;
       f32x16 s[NB];
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
         const int blk = FEW ? wave : kb;
-        seen_start(s[kb], few_word<FEW>(cur, kb, wave), lh);
-        mma_rows<T, DT>(s[kb], tk, blk, qf, li, lh);
+        mma_rows_seen<T, DT>(s[kb], tk, blk, qf, start + buf * KT + blk * 32, few_word<FEW>(cur, kb, wave), li, lh);
       }
+      __builtin_amdgcn_s_setprio(0);
       float mt = -INFINITY;
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      mt = both_max(mt);
       // The maximum moves only when a tile exceeds it by more than 8 in the log2 domain (p <= 256 is harmless; o and l
       // carry the same maximum): the rescaling of o leaves the common path.
       const bool move = mt * SC > mx * SC + 8.f;
@@ -437,9 +492,11 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
           s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], SC, off));
           ls += s[kb][r];
         }
-      l += ls + __shfl_xor(ls, 32, 64);
+      l += ls;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT>(o, tv, FEW ? wave : kb, s[kb], lane);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {
       wait_tiles();                                      // every wave has read the tile: it may be overwritten
@@ -449,6 +506,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
     wait_tiles();
     cur = nxt;
   }
+  l = both_sum(l);                                       // (a lane summed its half of the keys)
   if (!live) {                                           // a row past the queries: as one that sees no key
     mx = -INFINITY;
     l = 0.f;
@@ -457,17 +515,21 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : 2)) void xattn_fw
   }
   const float m2 = mx == -INFINITY ? -INFINITY : mx * SC;      // log2 domain
   if constexpr (!FEW) {
-    if (m >= M) return;
+    const int mw = m0 + wave * 32;
     if (a.splits > 1) {
-      store_row<float, DT>(a.part + (sp * prows + prow) * a.D, o, a.D, lh, 1.f);
-      if (lh == 0) { pml[0] = m2; pml[1] = l; }
+      store_tile<float, DT>(smem + wave * 32 * DT * 4, o, a.D, lane, 1.f, true, [&](int r) {
+        return mw + r < M ? a.part + (sp * prows + (int64_t)bg * M + mw + r) * a.D : nullptr;
+      });
+      if (lh == 0 && m < M) { pml[0] = m2; pml[1] = l; }
     } else {
-      store_row<T, DT>(orow, o, a.D, lh, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
-      if (a.lse && lh == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
+      store_tile<T, DT>(smem + wave * 32 * RB, o, a.D, lane, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), true, [&](int r) {
+        return mw + r < M ? reinterpret_cast<T*>(a.out) + b * a.ob + (mw + r) / a.R * a.ol + (g * a.R + (mw + r) % a.R) * a.oh : nullptr;
+      });
+      if (a.lse && lh == 0 && m < M) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
     }
   } else {
     // join the four waves: ml[wave][32] = (max, sum), then o scaled to the common maximum, summed in wave order
-    float* ml = reinterpret_cast<float*>(smem + SMEM);
+    float* ml = reinterpret_cast<float*>(smem + SMEM + 2 * KT * 4);
     float* inv = ml + 256;
     if (lh == 0) { ml[(wave * 32 + li) * 2] = m2; ml[(wave * 32 + li) * 2 + 1] = l; }
     wait_tiles();
@@ -567,12 +629,13 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // ------------------------------------------------------------------------------------------------------------- dQ (and delta)
 // Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
 template <typename T, int DT, bool FEW>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >= 256 || FEW ? 2 : 3)) void xattn_dq_kernel(XArgs a) {
   constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
   constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM];
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4];
+  float* start = reinterpret_cast<float*>(smem + SMEM);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
@@ -590,7 +653,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   load_frag<T, DT>(dof, reinterpret_cast<const T*>(a.dout) + b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
   load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.o) + b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
   dl = frag_dot<DT>(qf, dof);
-  dl += __shfl_xor(dl, 32, 64);
+  dl = both_sum(dl);
   if (live) {
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
@@ -619,6 +682,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
     dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
     dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
+    start_put(start + buf * KT, kw, tid);
   };
   fill(t0, 0, cur);
   load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
@@ -626,6 +690,9 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
   f32x16 dq[DT / 32];
 #pragma unroll
   for (int i = 0; i < DT / 32; ++i) zero16(dq[i]);
+  f32x16 minus_dl;                                       // where do . v starts: dP - delta comes out of the product
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus_dl[r] = -dl;
   const float SC = a.scale * LOG2E;
   wait_tiles();
   for (int t = t0; t < t1; ++t) {
@@ -645,13 +712,16 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
       const uint32_t w = few_word<FEW>(cur, kb, wave);
       if (w == 0) continue;
       f32x16 s, dp;
-      seen_start(s, w, lh);                              // (unseen: P = exp2(-inf) = 0)
-      zero16(dp);
-      mma_rows<T, DT>(s, tk, blk, qf, li, lh);
+      dp = minus_dl;
+      __builtin_amdgcn_s_setprio(1);
+      mma_rows_seen<T, DT>(s, tk, blk, qf, start + buf * KT + blk * 32, w, li, lh);      // (unseen: P = exp2(-inf) = 0)
       mma_rows<T, DT>(dp, tv, blk, dof, li, lh);
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * (dp[r] - dl);
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * dp[r];
+      __builtin_amdgcn_s_setprio(1);
       mma_cols<T, DT>(dq, tk, blk, s, lane);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {
       wait_tiles();
@@ -662,9 +732,15 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
     cur = nxt;
   }
   if constexpr (!FEW) {
-    if (m >= M) return;
-    if (a.splits > 1) store_row<float, DT>(a.part + (sp * prows + prow) * a.D, dq, a.D, lh, a.scale);
-    else store_row<T, DT>(dqrow, dq, a.D, lh, a.scale);
+    const int mw = m0 + wave * 32;
+    if (a.splits > 1)
+      store_tile<float, DT>(smem + wave * 32 * DT * 4, dq, a.D, lane, a.scale, true, [&](int r) {
+        return mw + r < M ? a.part + (sp * prows + (int64_t)bg * M + mw + r) * a.D : nullptr;
+      });
+    else
+      store_tile<T, DT>(smem + wave * 32 * RB, dq, a.D, lane, a.scale, true, [&](int r) {
+        return mw + r < M ? reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + (mw + r) / a.R) * a.H + g * a.R + (mw + r) % a.R) * a.D : nullptr;
+      });
   } else {
     float* so = reinterpret_cast<float*>(smem);
     constexpr int LDO = DT + 4;
@@ -702,7 +778,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dq
 // key computes stays in its own lane; zeros are stored for it.
 template <typename T, int DT> constexpr int row_tile() { return DT * sizeof(T) >= 256 ? 32 : 64; }
 template <typename T, int DT>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dkv_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
   constexpr int RB = DT * sizeof(T), RT = row_tile<T, DT>(), TILE = RT * RB;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
@@ -712,6 +788,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dk
   const int klen = clamp_len(a.len, b, a.Lk), qv = clamp_len(a.qlen, b, a.Lq);
   const int key = kt * 128 + wave * 32 + li;
   const bool seen = key < klen && !(a.mask && a.mask[b * a.maskb + key]);
+  const bool some = __builtin_amdgcn_ballot_w64(seen) != 0;
   const int64_t krow = ((int64_t)b * a.Lk + key) * a.G + g, krows = (int64_t)a.B * a.Lk * a.G;
   const int nt = (qv + RT - 1) / RT, total = nt * a.R;
   int t0, t1;
@@ -769,13 +846,16 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dk
     const char* tq = smem + buf * 2 * TILE;
     const char* tg = tq + TILE;
     const float* st = stat + buf * 2 * RT;
+    if (some)                                            // (a wave whose keys are all unseen only helps to load)
 #pragma unroll
     for (int blk = 0; blk < RT / 32; ++blk) {
       f32x16 s, dp;
       zero16(s);
       zero16(dp);
+      __builtin_amdgcn_s_setprio(1);
       mma_rows<T, DT>(s, tq, blk, kf, li, lh);
       mma_rows<T, DT>(dp, tg, blk, vf, li, lh);
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
         const float4 L = *reinterpret_cast<const float4*>(st + blk * 32 + gq * 8 + lh * 4);
@@ -788,23 +868,34 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 256 ? 1 : 2)) void xattn_dk
           dp[r] = s[r] * (dp[r] - de[e]);
         }
       }
+      __builtin_amdgcn_s_setprio(1);
       mma_cols<T, DT>(dv, tg, blk, s, lane);
       mma_cols<T, DT>(dk, tq, blk, dp, lane);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (t + 1 < t1) put_stat(buf ^ 1);
     wait_tiles();
   }
-  if (key >= a.Lk) return;
+  // whole rows where the wave's share of the tile buffers holds them (a partial result of the widest heads does not fit)
+  const int kw = kt * 128 + wave * 32;
   if (a.splits > 1) {
-    float* pk = a.part + (sp * 2 * krows + krow) * a.D;
-    float* pv = a.part + ((sp * 2 + 1) * krows + krow) * a.D;
-    if (seen) { store_row<float, DT>(pk, dk, a.D, lh, a.scale); store_row<float, DT>(pv, dv, a.D, lh, 1.f); }
-    else { store_zero<float, DT>(pk, a.D, lh); store_zero<float, DT>(pv, a.D, lh); }
+    float* pk = a.part + sp * 2 * krows * a.D;
+    float* pv = pk + krows * a.D;
+    if constexpr (32 * DT * 4 <= TILE) {
+      auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; }; };
+      store_tile<float, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(pk));
+      store_tile<float, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(pv));
+    } else if (key < a.Lk) {
+      if (seen) { store_row<float, DT>(pk + krow * a.D, dk, a.D, lh, a.scale); store_row<float, DT>(pv + krow * a.D, dv, a.D, lh, 1.f); }
+      else { store_zero<float, DT>(pk + krow * a.D, a.D, lh); store_zero<float, DT>(pv + krow * a.D, a.D, lh); }
+    }
   } else {
-    T* pk = reinterpret_cast<T*>(a.dk) + krow * a.D;
-    T* pv = reinterpret_cast<T*>(a.dv) + krow * a.D;
-    if (seen) { store_row<T, DT>(pk, dk, a.D, lh, a.scale); store_row<T, DT>(pv, dv, a.D, lh, 1.f); }
-    else { store_zero<T, DT>(pk, a.D, lh); store_zero<T, DT>(pv, a.D, lh); }
+    static_assert(32 * RB <= TILE, "");
+    auto at = [&](void* base) {
+      return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<T*>(base) + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; };
+    };
+    store_tile<T, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(a.dk));
+    store_tile<T, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(a.dv));
   }
 }
 
@@ -846,17 +937,22 @@ int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
 struct Plan { bool few; int nrt, fwd, dq, nkt, dkv; };
 Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   Plan p;
+#ifdef XA_TUNE
+  static const int W0 = getenv("XW0") ? atoi(getenv("XW0")) : 512, W1 = getenv("XW1") ? atoi(getenv("XW1")) : 512, W2 = getenv("XW2") ? atoi(getenv("XW2")) : 512, L0 = getenv("XL0") ? atoi(getenv("XL0")) : 2, L1 = getenv("XL1") ? atoi(getenv("XL1")) : 4, L2 = getenv("XL2") ? atoi(getenv("XL2")) : 8;
+#else
+  const int W0 = 512, W1 = 512, W2 = 512, L0 = 2, L1 = 4, L2 = 8;
+#endif
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
   const int rb = (D <= 32 ? 32 : D <= 64 ? 64 : 128) * (bf16 ? 2 : 4);
   p.few = M <= 32;
   p.nrt = (int)(p.few ? 1 : (M + 127) / 128);
   const int KT = p.few ? 128 : (rb >= 512 ? 32 : 64);
   const int64_t kt = (Lk + KT - 1) / KT;
-  p.fwd = split_count(BG * p.nrt, kt, 512, 2);
-  p.dq = split_count(BG * p.nrt, kt, 512, 4);
+  p.fwd = split_count(BG * p.nrt, kt, W0, L0);
+  p.dq = split_count(BG * p.nrt, kt, W1, L1);
   p.nkt = (Lk + 127) / 128;
   const int RT = rb >= 256 ? 32 : 64;
-  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), 512, 8);
+  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), W2, L2);
   return p;
 }
 
