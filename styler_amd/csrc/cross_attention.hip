@@ -38,7 +38,7 @@ struct XArgs {
   const uint8_t* mask;
   int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh;   // strides (elements): item, row, head; g: dout
   int64_t maskb;
-  int B, Lq, Lk, H, G, R, D, nrt, splits, chunk;
+  int B, Lq, Lk, H, G, R, D, nrt, splits, chunk, sort;
   float scale;
 };
 
@@ -55,6 +55,22 @@ __device__ __forceinline__ int xcd_block(int total, int chunk) {
   const int n = blockIdx.x, i = n >> 3;
   const int v = ((i / chunk) * 8 + (n & 7)) * chunk + i % chunk;
   return v < total ? v : -1;
+}
+
+// Ragged batches are walked from the item with the most work (keys times queries) to the least, so that the last blocks are the
+// shortest: item number `r` in that order.  Every wave finds it by itself -- lane i counts the items that come before item i,
+// 3 B instructions.  Only for up to 16 items whose blocks' walks are
+// long against that (8 x 1203 x 1001 fp32: 620 -> 570 us; 48 x 1000 x 133, sorted all the same: 74 -> 82).
+__device__ __forceinline__ int item_at(const XArgs& a, int r, int lane) {
+  if (!a.sort) return r;
+  const int i = lane < a.B ? lane : 0;
+  const float w = (float)clamp_len(a.len, i, a.Lk) * (float)clamp_len(a.qlen, i, a.Lq);
+  int before = 0;
+  for (int j = 0; j < a.B; ++j) {
+    const float x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+    before += (x > w || (x == w && j < lane)) ? 1 : 0;
+  }
+  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.B && before == r));
 }
 
 // ---- LDS tiles: rows of DT elements, RB bytes ---------------------------------------------------------------------------------
@@ -323,13 +339,11 @@ __device__ __forceinline__ KeyWords<KT> key_words(const MaskBytes<KT>& m, bool h
   }
   return r;
 }
-// the word of a wave's 32 keys: block kb of a shared tile, or (FEW) the wave's own quarter
-template <bool FEW, int KT> __device__ __forceinline__ uint32_t few_word(const KeyWords<KT> k, int kb, int wave) {
-  uint32_t w = k.w[FEW ? 0 : kb];
-  if constexpr (FEW) {
+// word `blk` of a tile (blk is uniform, not a constant: a chain of selects keeps the words in registers)
+template <int KT> __device__ __forceinline__ uint32_t word_at(const KeyWords<KT> k, int blk) {
+  uint32_t w = k.w[0];
 #pragma unroll
-    for (int i = 1; i < KT / 32; ++i) w = wave == i ? k.w[i] : w;
-  }
+  for (int i = 1; i < KT / 32; ++i) w = blk == i ? k.w[i] : w;
   return w;
 }
 // Scores start at 0 for a seen key and at -inf for one that is not (its row was filled with zeros, so the product adds 0): the mask
@@ -370,8 +384,16 @@ __device__ __forceinline__ float both_sum(float v) {
   return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-// rows of keys per tile (shared-tile kernels) such that two tiles of K and V stay within 64 KB where two blocks per CU pay
-template <typename T, int DT> constexpr int key_tile() { return DT * sizeof(T) >= 512 ? 32 : 64; }
+// A block's four waves are RG = 4 / KG groups of 32 rows by KG groups of keys: KG = 1 where rows fill the chip, 4 where there are
+// at most 32 of them, 2 between (and where blocks of 128 rows would be too few, or too uneven, to fill it).  A tile holds NB blocks
+// of 32 keys for each key group: two where two tiles of K and V fit in 64 KB (two blocks a CU), so that the softmax's bookkeeping is
+// shared by 64 keys.
+template <typename T, int DT, int KG> constexpr int key_blocks() { return KG == 1 && DT * sizeof(T) < 512 ? 2 : 1; }
+
+// Waves per SIMD to ask registers for: `most` where rows are shared out alone; two with key groups, one where LDS holds one block.
+template <typename T, int DT, int KG> constexpr int waves_wanted(int most) {
+  return DT * sizeof(T) >= 512 || (KG == 4 && DT * sizeof(T) >= 256) ? 1 : (KG == 1 ? most : 2);
+}
 
 // a block's share of the key tiles: split s of S takes tiles [s n / S, (s + 1) n / S) of the n that the item has
 __device__ __forceinline__ void tile_range(int n, int s, int S, int& t0, int& t1) {
@@ -379,25 +401,37 @@ __device__ __forceinline__ void tile_range(int n, int s, int S, int& t0, int& t1
   t1 = (int)((int64_t)n * (s + 1) / S);
 }
 
+// 4 features of block row r, summed over the key groups in order ([wave][32 rows of LDO] floats)
+template <int KG, int LDO> __device__ __forceinline__ float4 group_sum(const float* so, int r, int d) {
+  const float* p = so + ((r / 32) * KG * 32 + r % 32) * LDO + d;
+  float4 x = *reinterpret_cast<const float4*>(p);
+#pragma unroll
+  for (int w = 1; w < KG; ++w) {
+    const float4 y = *reinterpret_cast<const float4*>(p + w * 32 * LDO);
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
+  return x;
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
-// FEW = false: a block owns 128 rows (32 per wave) and walks key tiles that its waves share.
-// FEW = true (M <= 32): all waves hold the same 32 rows and a wave takes 32 of the tile's 128 keys -- every wave works where
-// a block of rows would leave three idle; the four partial softmaxes are joined through LDS.
-template <typename T, int DT, bool FEW>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <= 128 && !FEW ? 4 : 2)) void xattn_fwd_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
-  constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
+template <typename T, int DT, int KG>
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
+  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG>(), KT = 32 * KG * NB;
+  constexpr int TILE = KT * RB;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
-  constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (FEW ? 1152 : 0)];
+  constexpr int LDO = DT + 4;                            // rows of the join start 4 banks apart
+  constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  static_assert(KG > 1 || 4 * 32 * DT * 4 <= SMEM, "");
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (KG > 1 ? 1280 : 0)];
   float* start = reinterpret_cast<float*>(smem + SMEM);          // [buffer][KT], see start_put
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int rg = wave / KG, kg = wave % KG;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
-  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, nth = v / (a.nrt * a.splits), g = nth % a.G, b = item_at(a, nth / a.G, lane), bg = b * a.G + g;
   const int M = a.Lq * a.R;
   const int klen = clamp_len(a.len, b, a.Lk), Mv = clamp_len(a.qlen, b, a.Lq) * a.R;
-  const int m0 = rt * (FEW ? 32 : 128), m = m0 + (FEW ? 0 : wave * 32) + li;
+  const int m0 = rt * 32 * RG, m = m0 + rg * 32 + li;
   const int qi = m / a.R, head = g * a.R + m % a.R;
   const bool live = m < Mv;
   T* orow = reinterpret_cast<T*>(a.out) + b * a.ob + qi * a.ol + head * a.oh;
@@ -406,7 +440,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <=
   int t0, t1;
   tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
   if (m0 >= Mv || t0 >= t1) {                            // no live row, or no key in this share
-    if (FEW ? wave == 0 : true)
+    if (kg == 0)
       if (m < M) {
         if (a.splits > 1) { if (lh == 0) { pml[0] = -INFINITY; pml[1] = 0.f; } }
         else {
@@ -460,8 +494,8 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <=
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
-        const int blk = FEW ? wave : kb;
-        mma_rows_seen<T, DT>(s[kb], tk, blk, qf, start + buf * KT + blk * 32, few_word<FEW>(cur, kb, wave), li, lh);
+        const int blk = kg * NB + kb;
+        mma_rows_seen<T, DT>(s[kb], tk, blk, qf, start + buf * KT + blk * 32, word_at(cur, blk), li, lh);
       }
       __builtin_amdgcn_s_setprio(0);
       float mt = -INFINITY;
@@ -495,7 +529,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <=
       l += ls;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT>(o, tv, FEW ? wave : kb, s[kb], lane);
+      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT>(o, tv, kg * NB + kb, s[kb], lane);
       __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {
@@ -514,7 +548,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <=
     for (int i = 0; i < DT / 32; ++i) zero16(o[i]);
   }
   const float m2 = mx == -INFINITY ? -INFINITY : mx * SC;      // log2 domain
-  if constexpr (!FEW) {
+  if constexpr (KG == 1) {
     const int mw = m0 + wave * 32;
     if (a.splits > 1) {
       store_tile<float, DT>(smem + wave * 32 * DT * 4, o, a.D, lane, 1.f, true, [&](int r) {
@@ -528,43 +562,40 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) <=
       if (a.lse && lh == 0 && m < M) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
     }
   } else {
-    // join the four waves: ml[wave][32] = (max, sum), then o scaled to the common maximum, summed in wave order
+    // join the key groups of a row group: ml[wave][32] = (max, sum), then o scaled to the common maximum, summed in group order
     float* ml = reinterpret_cast<float*>(smem + SMEM + 2 * KT * 4);
-    float* inv = ml + 256;
+    float* inv = ml + 256;                               // [RG * 32]
     if (lh == 0) { ml[(wave * 32 + li) * 2] = m2; ml[(wave * 32 + li) * 2 + 1] = l; }
     wait_tiles();
     float mm = -INFINITY, lt = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + li) * 2]);
+    for (int w = 0; w < KG; ++w) mm = fmaxf(mm, ml[((rg * KG + w) * 32 + li) * 2]);
     const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) lt += ml[(w * 32 + li) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + li) * 2] - base);
+    for (int w = 0; w < KG; ++w) {
+      const float* p = ml + ((rg * KG + w) * 32 + li) * 2;
+      lt += p[1] * __builtin_amdgcn_exp2f(p[0] - base);
+    }
     const float c = __builtin_amdgcn_exp2f(m2 - base);
-    // [wave][32 rows of DT + 4 floats]: the rows of a half wave start 4 banks apart
-    float* so = reinterpret_cast<float*>(smem);
-    constexpr int LDO = DT + 4;
-    static_assert(4 * 32 * LDO * 4 <= SMEM, "");
+    float* so = reinterpret_cast<float*>(smem);          // [wave][32 rows of LDO]
 #pragma unroll
     for (int dt = 0; dt < DT / 32; ++dt)
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq)
         *reinterpret_cast<float4*>(so + (wave * 32 + li) * LDO + dt * 32 + gq * 8 + lh * 4) =
             make_float4(o[dt][gq * 4] * c, o[dt][gq * 4 + 1] * c, o[dt][gq * 4 + 2] * c, o[dt][gq * 4 + 3] * c);
-    if (wave == 0 && lh == 0 && m < M) {
-      if (a.splits > 1) { pml[0] = mm; pml[1] = lt; }
-      else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = lt == 0.f ? -INFINITY : (mm + log2f(lt)) * LN2;
+    if (kg == 0 && lh == 0) {
+      inv[rg * 32 + li] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+      if (m < M) {
+        if (a.splits > 1) { pml[0] = mm; pml[1] = lt; }
+        else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = lt == 0.f ? -INFINITY : (mm + log2f(lt)) * LN2;
+      }
     }
-    if (wave == 0 && lh == 0) inv[li] = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
     wait_tiles();
-    for (int i = tid; i < 32 * (DT / 4); i += 256) {
+    for (int i = tid; i < RG * 32 * (DT / 4); i += 256) {
       const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
       if (mr >= M || d >= a.D) continue;
-      float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(so + (w * 32 + r) * LDO + d);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
+      const float4 x = group_sum<KG, LDO>(so, r, d);
       if (a.splits > 1) {
         *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
       } else {
@@ -628,21 +659,24 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------- dQ (and delta)
 // Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
-template <typename T, int DT, bool FEW>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >= 256 || FEW ? 2 : 3)) void xattn_dq_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), KT = FEW ? 128 : key_tile<T, DT>();
-  constexpr int TILE = KT * RB, NB = FEW ? 1 : KT / 32;
+template <typename T, int DT, int KG>
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
+  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG>(), KT = 32 * KG * NB;
+  constexpr int TILE = KT * RB;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
-  constexpr int JOIN = FEW ? 4 * 32 * (DT + 4) * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  constexpr int LDO = DT + 4;
+  constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  static_assert(KG > 1 || 4 * 32 * DT * 4 <= SMEM, "");
   __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4];
   float* start = reinterpret_cast<float*>(smem + SMEM);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int rg = wave / KG, kg = wave % KG;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
-  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int rt = v % a.nrt, sp = (v / a.nrt) % a.splits, nth = v / (a.nrt * a.splits), g = nth % a.G, b = item_at(a, nth / a.G, lane), bg = b * a.G + g;
   const int M = a.Lq * a.R;
   const int klen = clamp_len(a.len, b, a.Lk), Mv = clamp_len(a.qlen, b, a.Lq) * a.R;
-  const int m0 = rt * (FEW ? 32 : 128), m = m0 + (FEW ? 0 : wave * 32) + li;
+  const int m0 = rt * 32 * RG, m = m0 + rg * 32 + li;
   const int qi = m / a.R, head = g * a.R + m % a.R;
   const bool live = m < Mv;
   T* dqrow = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + qi) * a.H + head) * a.D;
@@ -658,11 +692,11 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
   }
-  if (sp == 0 && m < M && lh == 0 && (!FEW || wave == 0)) a.delta[srow] = dl;
+  if (sp == 0 && m < M && lh == 0 && kg == 0) a.delta[srow] = dl;
   int t0, t1;
   tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
   if (m0 >= Mv || t0 >= t1) {
-    if (m < M && (!FEW || wave == 0)) {
+    if (m < M && kg == 0) {
       if (a.splits > 1) store_zero<float, DT>(a.part + (sp * prows + prow) * a.D, a.D, lh);
       else store_zero<T, DT>(dqrow, a.D, lh);
     }
@@ -708,8 +742,8 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     const char* tv = tk + TILE;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
-      const int blk = FEW ? wave : kb;
-      const uint32_t w = few_word<FEW>(cur, kb, wave);
+      const int blk = kg * NB + kb;
+      const uint32_t w = word_at(cur, blk);
       if (w == 0) continue;
       f32x16 s, dp;
       dp = minus_dl;
@@ -731,7 +765,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     wait_tiles();
     cur = nxt;
   }
-  if constexpr (!FEW) {
+  if constexpr (KG == 1) {
     const int mw = m0 + wave * 32;
     if (a.splits > 1)
       store_tile<float, DT>(smem + wave * 32 * DT * 4, dq, a.D, lane, a.scale, true, [&](int r) {
@@ -742,9 +776,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
         return mw + r < M ? reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + (mw + r) / a.R) * a.H + g * a.R + (mw + r) % a.R) * a.D : nullptr;
       });
   } else {
-    float* so = reinterpret_cast<float*>(smem);
-    constexpr int LDO = DT + 4;
-    static_assert(4 * 32 * LDO * 4 <= SMEM, "");
+    float* so = reinterpret_cast<float*>(smem);          // sums over the key groups
 #pragma unroll
     for (int dt = 0; dt < DT / 32; ++dt)
 #pragma unroll
@@ -752,15 +784,10 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
         *reinterpret_cast<float4*>(so + (wave * 32 + li) * LDO + dt * 32 + gq * 8 + lh * 4) =
             make_float4(dq[dt][gq * 4], dq[dt][gq * 4 + 1], dq[dt][gq * 4 + 2], dq[dt][gq * 4 + 3]);
     wait_tiles();
-    for (int i = tid; i < 32 * (DT / 4); i += 256) {
+    for (int i = tid; i < RG * 32 * (DT / 4); i += 256) {
       const int r = i / (DT / 4), d = (i % (DT / 4)) * 4, mr = m0 + r;
       if (mr >= M || d >= a.D) continue;
-      float4 x = *reinterpret_cast<const float4*>(so + r * LDO + d);
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {                      // in wave order
-        const float4 y = *reinterpret_cast<const float4*>(so + (w * 32 + r) * LDO + d);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
+      float4 x = group_sum<KG, LDO>(so, r, d);
       x.x *= a.scale; x.y *= a.scale; x.z *= a.scale; x.w *= a.scale;
       if (a.splits > 1) *reinterpret_cast<float4*>(a.part + (sp * prows + (int64_t)bg * M + mr) * a.D + d) = x;
       else {
@@ -773,28 +800,52 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
 }
 
 // ------------------------------------------------------------------------------------------------------------- dK, dV
-// A block owns 128 keys (32 per wave, a lane one key: its K and V rows stay in registers) and walks tiles of query rows, head
-// after head of the group.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen
-// key computes stays in its own lane; zeros are stored for it.
-template <typename T, int DT> constexpr int row_tile() { return DT * sizeof(T) >= 256 ? 32 : 64; }
-template <typename T, int DT>
+// acc of the giving waves -> acc of their partners through LDS (all waves of the block call it)
+template <int N> __device__ __forceinline__ void add_from(f32x16 (&acc)[N], char* lds, int lane, bool gives) {
+  float4* p = reinterpret_cast<float4*>(lds) + lane;
+  if (gives) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) p[(i * 4 + g) * 64] = make_float4(acc[i][g * 4], acc[i][g * 4 + 1], acc[i][g * 4 + 2], acc[i][g * 4 + 3]);
+  }
+  wait_tiles();
+  if (!gives) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 x = p[(i * 4 + g) * 64];
+        acc[i][g * 4] += x.x; acc[i][g * 4 + 1] += x.y; acc[i][g * 4 + 2] += x.z; acc[i][g * 4 + 3] += x.w;
+      }
+  }
+  wait_tiles();
+}
+
+// A block owns 32 KW keys (KW = 4, or 2 where that would be too few blocks), a lane one key: its K and V rows stay in registers.
+// The block walks tiles of 64 query rows, head after head of the group; with KW = 2 two waves share the keys and each takes half of
+// a tile's rows.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen key computes
+// stays in its own lane; zeros are stored for it.
+template <typename T, int DT> constexpr int DKV_UNROLL = DT * sizeof(T) >= 256 ? 1 : 2;        // (twice the registers spill)
+template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), RT = row_tile<T, DT>(), TILE = RT * RB;
+  constexpr int RB = DT * sizeof(T), RT = 64, TILE = RT * RB, RW = 4 / KW;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+  const int kwv = wave / RW, rwv = wave % RW;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
   if (v < 0) return;
-  const int kt = v % a.nrt, sp = (v / a.nrt) % a.splits, bg = v / (a.nrt * a.splits), g = bg % a.G, b = bg / a.G;
+  const int kt = v % a.nrt, sp = (v / a.nrt) % a.splits, nth = v / (a.nrt * a.splits), g = nth % a.G, b = item_at(a, nth / a.G, lane);
   const int klen = clamp_len(a.len, b, a.Lk), qv = clamp_len(a.qlen, b, a.Lq);
-  const int key = kt * 128 + wave * 32 + li;
+  const int key = kt * 32 * KW + kwv * 32 + li;
   const bool seen = key < klen && !(a.mask && a.mask[b * a.maskb + key]);
   const bool some = __builtin_amdgcn_ballot_w64(seen) != 0;
   const int64_t krow = ((int64_t)b * a.Lk + key) * a.G + g, krows = (int64_t)a.B * a.Lk * a.G;
   const int nt = (qv + RT - 1) / RT, total = nt * a.R;
   int t0, t1;
   tile_range(total, sp, a.splits, t0, t1);
-  if (kt * 128 >= klen || t0 >= t1) {
-    if (key < a.Lk) {
+  if (kt * 32 * KW >= klen || t0 >= t1) {
+    if (key < a.Lk && rwv == 0) {
       if (a.splits > 1) {
         store_zero<float, DT>(a.part + (sp * 2 * krows + krow) * a.D, a.D, lh);
         store_zero<float, DT>(a.part + ((sp * 2 + 1) * krows + krow) * a.D, a.D, lh);
@@ -847,8 +898,9 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     const char* tg = tq + TILE;
     const float* st = stat + buf * 2 * RT;
     if (some)                                            // (a wave whose keys are all unseen only helps to load)
-#pragma unroll
-    for (int blk = 0; blk < RT / 32; ++blk) {
+#pragma unroll DKV_UNROLL<T, DT>
+    for (int hb = 0; hb < 2 / RW; ++hb) {
+      const int blk = rwv * (2 / RW) + hb;
       f32x16 s, dp;
       zero16(s);
       zero16(dp);
@@ -876,21 +928,20 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     if (t + 1 < t1) put_stat(buf ^ 1);
     wait_tiles();
   }
-  // whole rows where the wave's share of the tile buffers holds them (a partial result of the widest heads does not fit)
-  const int kw = kt * 128 + wave * 32;
+  if constexpr (RW == 2) {                               // the second half of the rows joins the first
+    add_from(dk, smem + kwv * 32 * DT * 4, lane, rwv == 1);
+    add_from(dv, smem + kwv * 32 * DT * 4, lane, rwv == 1);
+    if (rwv == 1) return;
+  }
+  const int kw = kt * 32 * KW + kwv * 32;
   if (a.splits > 1) {
     float* pk = a.part + sp * 2 * krows * a.D;
     float* pv = pk + krows * a.D;
-    if constexpr (32 * DT * 4 <= TILE) {
-      auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; }; };
-      store_tile<float, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(pk));
-      store_tile<float, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(pv));
-    } else if (key < a.Lk) {
-      if (seen) { store_row<float, DT>(pk + krow * a.D, dk, a.D, lh, a.scale); store_row<float, DT>(pv + krow * a.D, dv, a.D, lh, 1.f); }
-      else { store_zero<float, DT>(pk + krow * a.D, a.D, lh); store_zero<float, DT>(pv + krow * a.D, a.D, lh); }
-    }
+    static_assert(32 * DT * 4 <= TILE, "");
+    auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; }; };
+    store_tile<float, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(pk));
+    store_tile<float, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(pv));
   } else {
-    static_assert(32 * RB <= TILE, "");
     auto at = [&](void* base) {
       return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<T*>(base) + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; };
     };
@@ -934,25 +985,24 @@ int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : (int)s;
 }
-struct Plan { bool few; int nrt, fwd, dq, nkt, dkv; };
+struct Plan { int kg, nrt, fwd, dq, kw, nkt, dkv; };
+// Sizes alone decide.  512 blocks are two per CU.  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
+// 81 us (every share writes its part once more); two key groups from 512 blocks of 128 rows down: 8 x 500 x 700 49 us, from 1024: the
+// fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).
 Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   Plan p;
-#ifdef XA_TUNE
-  static const int W0 = getenv("XW0") ? atoi(getenv("XW0")) : 512, W1 = getenv("XW1") ? atoi(getenv("XW1")) : 512, W2 = getenv("XW2") ? atoi(getenv("XW2")) : 512, L0 = getenv("XL0") ? atoi(getenv("XL0")) : 2, L1 = getenv("XL1") ? atoi(getenv("XL1")) : 4, L2 = getenv("XL2") ? atoi(getenv("XL2")) : 8;
-#else
-  const int W0 = 512, W1 = 512, W2 = 512, L0 = 2, L1 = 4, L2 = 8;
-#endif
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
   const int rb = (D <= 32 ? 32 : D <= 64 ? 64 : 128) * (bf16 ? 2 : 4);
-  p.few = M <= 32;
-  p.nrt = (int)(p.few ? 1 : (M + 127) / 128);
-  const int KT = p.few ? 128 : (rb >= 512 ? 32 : 64);
+  p.kg = M <= 32 ? 4 : M <= 64 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
+  const int rows = 128 / p.kg;
+  p.nrt = (int)((M + rows - 1) / rows);
+  const int KT = 32 * p.kg * (p.kg == 1 && rb < 512 ? 2 : 1);
   const int64_t kt = (Lk + KT - 1) / KT;
-  p.fwd = split_count(BG * p.nrt, kt, W0, L0);
-  p.dq = split_count(BG * p.nrt, kt, W1, L1);
-  p.nkt = (Lk + 127) / 128;
-  const int RT = rb >= 256 ? 32 : 64;
-  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), W2, L2);
+  p.fwd = split_count(BG * p.nrt, kt, 512, 2);
+  p.dq = split_count(BG * p.nrt, kt, 512, 4);
+  p.kw = BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
+  p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
+  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + 63) / 64) * (H / G), 512, 8);
   return p;
 }
 
@@ -968,21 +1018,24 @@ dim3 grid_for(XArgs& a) {
 }
 
 template <typename T, int DT>
-void launch_fwd(XArgs& a, bool few, hipStream_t st) {
+void launch_fwd(XArgs& a, int kg, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (few) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, true>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, false>), g, dim3(256), 0, st, a);
+  if (kg == 4) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
+  else if (kg == 2) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
-void launch_dq(XArgs& a, bool few, hipStream_t st) {
+void launch_dq(XArgs& a, int kg, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (few) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, true>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, false>), g, dim3(256), 0, st, a);
+  if (kg == 4) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
+  else if (kg == 2) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
-void launch_dkv(XArgs& a, hipStream_t st) {
+void launch_dkv(XArgs& a, int kw, hipStream_t st) {
   const dim3 g = grid_for(a);
-  hipLaunchKernelGGL((xattn_dkv_kernel<T, DT>), g, dim3(256), 0, st, a);
+  if (kw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
 }
 #define BY_WIDTH(T, CALL)              \
   do {                                 \
@@ -1017,6 +1070,7 @@ XArgs args(const styler_xattn_t* x) {
   a.lse = x->lse; a.len = x->len; a.qlen = x->q_len; a.mask = x->mask; a.maskb = x->maskb;
   a.qb = x->qb; a.ql = x->ql; a.qh = x->qh; a.kb = x->kb; a.kl = x->kl; a.kh = x->kh; a.vb = x->vb; a.vl = x->vl; a.vh = x->vh;
   a.ob = x->ob; a.ol = x->ol; a.oh = x->oh; a.gb = x->gb; a.gl = x->gl; a.gh = x->gh;
+  a.sort = (x->len || x->q_len) && x->B > 1 && x->B <= 16 && (int64_t)x->Lq * x->Lk >= 1 << 18;
   a.B = x->B; a.Lq = x->Lq; a.Lk = x->Lk; a.H = x->H; a.G = x->G; a.R = x->H / x->G; a.D = x->D; a.scale = x->scale;
   return a;
 }
@@ -1042,7 +1096,7 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   a.nrt = p.nrt; a.splits = p.fwd; a.part = p.fwd > 1 ? (float*)workspace : nullptr;
-#define FWD(T, W) launch_fwd<T, W>(a, p.few, st)
+#define FWD(T, W) launch_fwd<T, W>(a, p.kg, st)
   if (x->bf16) BY_WIDTH(uint16_t, FWD); else BY_WIDTH(float, FWD);
 #undef FWD
   if (p.fwd > 1) {
@@ -1065,7 +1119,7 @@ extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspa
   a.delta = (float*)workspace;
   a.part = (float*)workspace + (qrows + 3) / 4 * 4;
   a.nrt = p.nrt; a.splits = p.dq;
-#define DQ(T, W) launch_dq<T, W>(a, p.few, st)
+#define DQ(T, W) launch_dq<T, W>(a, p.kg, st)
   if (x->bf16) BY_WIDTH(uint16_t, DQ); else BY_WIDTH(float, DQ);
 #undef DQ
   if (p.dq > 1) {
@@ -1074,7 +1128,7 @@ extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspa
     else hipLaunchKernelGGL((xattn_sum_kernel<float, true>), dim3(blocks), dim3(256), 0, st, a);
   }
   a.nrt = p.nkt; a.splits = p.dkv;
-#define DKV(T, W) launch_dkv<T, W>(a, st)
+#define DKV(T, W) launch_dkv<T, W>(a, p.kw, st)
   if (x->bf16) BY_WIDTH(uint16_t, DKV); else BY_WIDTH(float, DKV);
 #undef DKV
   if (p.dkv > 1) {
