@@ -134,6 +134,16 @@ __device__ __forceinline__ void wait_tiles() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// the other half wave's value joined in: lane and lane ^ 32 hold the same row
+__device__ __forceinline__ float both_max(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
 // ---- matrix products ----------------------------------------------------------------------------------------------------------
 // Frag: a lane's own row (32 rows of a wave), the half of its features that its half wave (lh) feeds to the product over d.
 template <typename T, int DT> struct Frag;
@@ -151,28 +161,6 @@ __device__ __forceinline__ void load_frag(Frag<T, DT>& f, const T* row, int D, i
     f.v[i] = *reinterpret_cast<const typename std::remove_reference<decltype(f.v[0])>::type*>(&u);
   }
 }
-template <int DT> __device__ __forceinline__ float frag_dot(const Frag<uint16_t, DT>& a, const Frag<uint16_t, DT>& b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < DT / 16; ++i) {
-    const uint4 x = *reinterpret_cast<const uint4*>(&a.v[i]), y = *reinterpret_cast<const uint4*>(&b.v[i]);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), s);
-      s = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), s);
-    }
-  }
-  return s;
-}
-template <int DT> __device__ __forceinline__ float frag_dot(const Frag<float, DT>& a, const Frag<float, DT>& b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < DT / 8; ++i)
-    s = fmaf(a.v[i].x, b.v[i].x, fmaf(a.v[i].y, b.v[i].y, fmaf(a.v[i].z, b.v[i].z, fmaf(a.v[i].w, b.v[i].w, s))));
-  return s;
-}
-
 __device__ __forceinline__ void zero16(f32x16& a) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) a[r] = 0.f;
@@ -200,6 +188,30 @@ __device__ __forceinline__ void mma_rows(f32x16& s, const char* tile, int blk, c
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, f.v[i].w, s, 0, 0, 0);
     }
   }
+}
+
+// x_row . y_row of the lane's own row: the diagonal of the rows' product, by the same instructions in the same order as mma_rows
+// forms a tile row's -- equal rows give equal bits, so dP - delta is 0, not a rounding, where a query sees one key alone.
+template <typename T, int DT>
+__device__ __forceinline__ float frag_dot(const Frag<T, DT>& x, const Frag<T, DT>& y, int li, int lh) {
+  f32x16 s;
+  zero16(s);
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[i], y.v[i], s, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < DT / 8; ++i) {
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[i].x, y.v[i].x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[i].y, y.v[i].y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[i].z, y.v[i].z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[i].w, y.v[i].w, s, 0, 0, 0);
+    }
+  }
+  float d = 0.f;                                         // row li stands in register (li & 3) + 4 (li >> 3) of half wave (li >> 2) & 1
+#pragma unroll
+  for (int r = 0; r < 16; ++r) d = r == (li & 3) + 4 * (li >> 3) ? s[r] : d;
+  return both_sum(lh == ((li >> 2) & 1) ? d : 0.f);
 }
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16& a, int s2) {
@@ -374,16 +386,6 @@ __device__ __forceinline__ void mma_rows_seen(f32x16& s, const char* tile, int b
     mma_rows<T, DT>(s, tile, blk, f, li, lh);
   }
 }
-// the other half wave's value joined in: lane and lane ^ 32 hold the same row
-__device__ __forceinline__ float both_max(float v) {
-  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
-}
-__device__ __forceinline__ float both_sum(float v) {
-  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
-}
-
 // A block's four waves are RG = 4 / KG groups of 32 rows by KG groups of keys: KG = 1 where rows fill the chip, 4 where there are
 // at most 32 of them, 2 between (and where blocks of 128 rows would be too few, or too uneven, to fill it).  A tile holds NB blocks
 // of 32 keys for each key group: two where two tiles of K and V fit in 64 KB (two blocks a CU), so that the softmax's bookkeeping is
@@ -517,13 +519,14 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= al;
       }
-      const float off = mx == -INFINITY ? 0.f : -mx * SC;
+      const float sub = mx == -INFINITY ? 0.f : mx, off = -sub * SC;
       float ls = 0.f;
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], SC, off));
+          // (fp32: (s - max) SC, so that the largest P is 1 to the last bit; bf16 rounds P anyway and takes one instruction)
+          s[kb][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[kb][r], SC, off) : (s[kb][r] - sub) * SC);
           ls += s[kb][r];
         }
       l += ls;
@@ -686,8 +689,7 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   float dl = 0.f, lse2 = INFINITY;
   load_frag<T, DT>(dof, reinterpret_cast<const T*>(a.dout) + b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
   load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.o) + b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
-  dl = frag_dot<DT>(qf, dof);
-  dl = both_sum(dl);
+  dl = frag_dot<T, DT>(qf, dof, li, lh);
   if (live) {
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
@@ -724,9 +726,6 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   f32x16 dq[DT / 32];
 #pragma unroll
   for (int i = 0; i < DT / 32; ++i) zero16(dq[i]);
-  f32x16 minus_dl;                                       // where do . v starts: dP - delta comes out of the product
-#pragma unroll
-  for (int r = 0; r < 16; ++r) minus_dl[r] = -dl;
   const float SC = a.scale * LOG2E;
   wait_tiles();
   for (int t = t0; t < t1; ++t) {
@@ -746,13 +745,13 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
       const uint32_t w = word_at(cur, blk);
       if (w == 0) continue;
       f32x16 s, dp;
-      dp = minus_dl;
+      zero16(dp);
       __builtin_amdgcn_s_setprio(1);
       mma_rows_seen<T, DT>(s, tk, blk, qf, start + buf * KT + blk * 32, w, li, lh);      // (unseen: P = exp2(-inf) = 0)
       mma_rows<T, DT>(dp, tv, blk, dof, li, lh);
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * dp[r];
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * (dp[r] - dl);
       __builtin_amdgcn_s_setprio(1);
       mma_cols<T, DT>(dq, tk, blk, s, lane);
       __builtin_amdgcn_s_setprio(0);

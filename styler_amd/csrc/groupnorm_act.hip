@@ -12,7 +12,8 @@
 //     group, a third writes the output.  x is read twice.
 // Statistics: a thread sums (x - K) and (x - K)^2 of its channel, K = the chunk's first row -- a channel's offset, which may be
 // large against its spread, is gone before the squares are formed; (count, mean, M2) triples are then joined pairwise exactly.
-// Everything is summed in a fixed order in 32 bits; there are no atomics.
+// Values enter as (x - mean), not folded into a multiply-add with -mean rstd: where a group hardly varies rstd is large, and the
+// folded form keeps the rounding of mean rstd.  Everything is summed in a fixed order in 32 bits; there are no atomics.
 #include "common.h"
 
 namespace {
@@ -250,12 +251,13 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
     }
     __syncthreads();
     if (!on) return;
-    float A[V], Z[V];                                    // z = A x + Z
+    float A[V], Z[V], mean[V];                           // z = A (x - mean) + Z
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int g = (col * V + j) / a.cg;
+      mean[j] = gm[2 * g];
       A[j] = gm[2 * g + 1] * a.gamma[c + j];
-      Z[j] = fmaf(-gm[2 * g], A[j], a.beta[c + j]);
+      Z[j] = a.beta[c + j];
     }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -263,18 +265,18 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       if (t >= a.L) break;
       float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = t < n ? act_of<ACT>(fmaf(xr[i].get(j), A[j], Z[j])) : 0.f;
+      for (int j = 0; j < V; ++j) y[j] = t < n ? act_of<ACT>(fmaf(xr[i].get(j) - mean[j], A[j], Z[j])) : 0.f;
       put<B16, V>(a.out, o0 + t * a.ol, y);
     }
   } else {
-    float ga[V], be[V], R[V], S[V];                      // xh = R x + S
+    float ga[V], be[V], R[V], S[V];                      // xh = R (x - S)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float* st = a.stats + ((int64_t)b * a.G + (on ? (c + j) / a.cg : 0)) * 2;
       ga[j] = on ? a.gamma[c + j] : 0.f;
       be[j] = on ? a.beta[c + j] : 0.f;
       R[j] = st[1];
-      S[j] = -st[0] * R[j];
+      S[j] = st[0];
       s[j] = 0.f;
       q[j] = 0.f;
     }
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       if (on && rl + i * RL < n) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float xh = fmaf(xr[i].get(j), R[j], S[j]);
+          const float xh = (xr[i].get(j) - S[j]) * R[j];
           const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
           s[j] += dz;
           q[j] = fmaf(dz, xh, q[j]);
@@ -312,9 +314,9 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = fmaf(xr[i].get(j), R[j], S[j]);
+        const float xh = (xr[i].get(j) - S[j]) * R[j];
         const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
-        y[j] = t < n ? R[j] * (fmaf(dz, ga[j], -m1[j]) - xh * m2[j]) : 0.f;
+        y[j] = t < n ? R[j] * (mul_rounded(dz, ga[j]) - m1[j] - xh * m2[j]) : 0.f;
       }
       put<B16, V>(a.out, o0 + t * a.ol, y);
     }
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
   for (int j = 0; j < V; ++j) { s[j] = 0.f; q[j] = 0.f; K[j] = 0.f; }
   const int64_t x0 = b * a.xb + c, g0 = b * a.db + c;
   if (on) {
-    float ga[V], be[V], R[V], S[V];                      // xh = R x + S
+    float ga[V], be[V], R[V], S[V];                      // xh = R (x - S)
     if constexpr (BWD) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
         ga[j] = a.gamma[c + j];
         be[j] = a.beta[c + j];
         R[j] = st[1];
-        S[j] = -st[0] * R[j];
+        S[j] = st[0];
       }
     } else {
       Raw<B16, V> k0;
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if constexpr (BWD) {
-            const float xh = fmaf(xr[u].get(j), R[j], S[j]);
+            const float xh = (xr[u].get(j) - S[j]) * R[j];
             const float dz = gr[u].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
             s[j] += dz;
             q[j] = fmaf(dz, xh, q[j]);
@@ -483,14 +485,14 @@ __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw)
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv, c = c0 + col * V;
   if (rl >= RL) return;
   const int n = gn_len(a.len, b, a.L), t0 = (a.chunks - 1 - (int)blockIdx.x) * a.rows, t1 = min(a.L, t0 + a.rows);
-  float ga[V], be[V], R[V], S[V], m1[V], m2[V];          // xh = R x + S; forward: z = R x + S, gamma and beta included
+  float ga[V], be[V], R[V], S[V], m1[V], m2[V];          // h = R (x - S); forward: R includes gamma
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int64_t g = ((int64_t)b * a.G + (c + j) / a.cg) * 2;
     ga[j] = a.gamma[c + j];
     be[j] = a.beta[c + j];
     R[j] = BWD ? a.stats[g + 1] : a.stats[g + 1] * ga[j];
-    S[j] = BWD ? -a.stats[g] * R[j] : fmaf(-a.stats[g], R[j], be[j]);
+    S[j] = a.stats[g];
     if constexpr (BWD) { m1[j] = gw[g]; m2[j] = gw[g + 1]; }
   }
   const int64_t x0 = b * a.xb + c, g0 = b * a.db + c, o0 = b * a.ob + c;
@@ -515,12 +517,13 @@ __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw)
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float h = fmaf(xr[u].get(j), R[j], S[j]);
+        const float x = xr[u].get(j) - S[j];
         if constexpr (BWD) {
+          const float h = x * R[j];
           const float dz = gr[u].get(j) * act_slope<ACT>(fmaf(h, ga[j], be[j]));
-          y[j] = r < n ? R[j] * (fmaf(dz, ga[j], -m1[j]) - h * m2[j]) : 0.f;
+          y[j] = r < n ? R[j] * (mul_rounded(dz, ga[j]) - m1[j] - h * m2[j]) : 0.f;
         } else {
-          y[j] = r < n ? act_of<ACT>(h) : 0.f;
+          y[j] = r < n ? act_of<ACT>(fmaf(x, R[j], be[j])) : 0.f;
         }
       }
       put<B16, V>(a.out, o0 + (int64_t)r * a.ol, y);
@@ -553,6 +556,9 @@ struct GPlan { bool fused; int v, slab, slabs, chunks, rows, it, T; };
 
 int gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
+// rows a thread of 1024 holds without spilling (the backward keeps x and dy)
+constexpr int it_max(bool b16, int v, bool bwd) { return bwd ? (b16 && v == 8 ? 4 : 8) : 16; }
+
 GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
   GPlan p = {};
   const int es = bf16 ? 2 : 4, cg = C / G;
@@ -561,7 +567,6 @@ GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
   // bytes (the lines that slabs share are then shared in one XCD's cache).  16 x 1000 x 320 bf16, forward / backward: 80 blocks
   // 13.7 / 16.6 us, 160 blocks 11.0 / 16.6, 320 blocks 13.3 / 23.5
   const int64_t unit = (int64_t)cg / gcd(cg, v) * v;
-  const int it_max = bwd ? (bf16 && v == 8 ? 4 : 8) : 16;         // (rows a thread holds without spilling)
   for (int line = 128; line >= 32 && !p.fused; line >>= 1) {
     int64_t slab = unit * ((line / es + unit - 1) / unit);
     if (slab > C) slab = C;
@@ -570,7 +575,7 @@ GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
     for (int T = 256; T <= 1024 && !p.fused; T *= 4) {
       if (cv > T || slab > 1024) continue;
       const int64_t it = (L + T / cv - 1) / (T / cv);
-      if (it <= (T == 256 ? 4 : it_max)) {
+      if (it <= (T == 256 ? 4 : it_max(bf16 != 0, v, bwd))) {
         p.fused = true;
         p.T = T;
         p.it = it <= 4 ? 4 : it <= 8 ? 8 : 16;
@@ -627,8 +632,8 @@ void gn_launch(const GArgs& a, const GPlan& p, float* gw, hipStream_t st) {
 #define SLAB(IT, T) hipLaunchKernelGGL((gn_slab_kernel<B16, V, ACT, IT, T, BWD>), grid, dim3(T), lds, st, a)
     if (p.T == 256) SLAB(4, 256);
     else if (p.it == 4) SLAB(4, 1024);
-    else if (p.it == 8) SLAB(8, 1024);
-    else if constexpr (!BWD) SLAB(16, 1024);
+    else if (p.it == 8) { if constexpr (it_max(B16, V, BWD) >= 8) SLAB(8, 1024); }
+    else if constexpr (it_max(B16, V, BWD) >= 16) SLAB(16, 1024);
 #undef SLAB
     return;
   }

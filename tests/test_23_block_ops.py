@@ -585,3 +585,36 @@ def test_groupnorm_act_refusals():
     ]:
         with pytest.raises(ops.StylerHipError, match=text):
             bad()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("Lq", [1, 50, 200])
+def test_one_seen_key_has_no_score_gradient(dev, dtype, Lq):
+    """A query that sees one key gives that key's value, and its scores have no gradient: exactly, not up to a rounding."""
+    from styler_amd import ops
+    B, H, G, D = 3, 4, 2, 64
+    q, k, v, do = attention_case(dev, B, Lq, 90, H, G, D, dtype, seed=21, spread=4.0)
+    mask = torch.ones(B, 90, dtype=torch.bool, device=dev)
+    for b, j in enumerate((0, 37, 89)):
+        mask[b, j] = False
+    for kk, vv, m in ((k[:, :1], v[:, :1], None), (k, v, mask)):
+        lse = torch.empty(B, H, Lq, device=dev)
+        out = ops.cross_attention(q, kk, vv, mask=m, lse=lse)
+        ref = vv[:, :1] if m is None else torch.stack([v[b, j] for b, j in enumerate((0, 37, 89))])[:, None]
+        assert torch.equal(out, ref.repeat_interleave(H // G, 2).expand(B, Lq, H, D))
+        dq, dk, dv = ops.cross_attention_bwd(q, kk, vv, out, do, lse, mask=m)
+        assert not dq.any() and not dk.any() and bool(dv.any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+def test_groupnorm_act_of_single_values(dev, dtype):
+    """A group of one value is its own mean: y = act(beta) and dx = 0 to the last bit."""
+    from styler_amd import ops
+    x, dy, gamma, beta = gn_case(dev, 8, 1, 128, dtype, seed=13)
+    stats = torch.empty(8, 128, 2, device=dev)
+    y = ops.groupnorm_act(x, gamma, beta, 128, ops.ACT_NONE, stats=stats)
+    assert torch.equal(y, beta.to(dtype).expand(8, 1, 128))
+    dx, dgamma, dbeta = ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, 128, ops.ACT_NONE)
+    assert not dx.any() and not dgamma.any()
