@@ -37,6 +37,8 @@ struct XArgs {
   const int64_t *len, *qlen;
   const uint8_t* mask;
   int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh;   // strides (elements): item, row, head; g: dout
+  const void *t0, *t1;                                 // what tiles are made of: k and v, or (dk, dv) q and dout
+  int64_t t0b, t0l, t0h, t0p, t1b, t1l, t1h, t1p;      // item, row, head, plane
   int64_t maskb;
   int B, Lq, Lk, H, G, R, D, nrt, splits, chunk, sort;
   float scale;
@@ -107,8 +109,9 @@ template <int RB> struct DmaLane {
 template <int RB, int ROWS, int NW>
 __device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* base, int64_t ldbytes, const DmaLane<RB>& dl, int wave,
                                          const uint32_t (&w)[NW]) {
-  constexpr int RPI = DmaLane<RB>::RPI, N = ROWS / (4 * RPI);        // instructions per wave
-  static_assert(N >= 1 && NW == ROWS / 32, "");
+  constexpr int RPI = DmaLane<RB>::RPI, N = ROWS >= 4 * RPI ? ROWS / (4 * RPI) : 1;        // instructions per wave
+  static_assert(NW == ROWS / 32, "");
+  if (ROWS < 4 * RPI && wave * RPI >= ROWS) return;                  // (narrow rows: two waves fill the tile)
   const uint64_t at = reinterpret_cast<uint64_t>(base);
   const i32x4 rs = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), 0x7fffffff, 0x00020000};      // raw buffer, 2^31 - 1 bytes
   const uint32_t l0 = (uint32_t)(uintptr_t)(lds_void*)smem + lds + wave * 1024;
@@ -117,7 +120,7 @@ __device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* b
     const int r0 = i * 4 * RPI;                                      // (the word of row r0 + dl.row: 4 RPI divides 32 or is 32 k)
     uint32_t word = w[r0 / 32];
     int bit = r0 % 32 + dl.row;
-    if constexpr (4 * RPI > 32) { if (dl.row >= 32) word = w[r0 / 32 + 1]; bit &= 31; }
+    if constexpr (4 * RPI > 32 && ROWS > 32) { if (dl.row >= 32) word = w[r0 / 32 + 1]; bit &= 31; }
     const uint32_t off = (word >> bit) & 1u ? dl.off[i % DmaLane<RB>::VAR] : OOB;
     // asm: the compiler lets no transposing LDS read start before the DMA it knows of has landed (it cannot tell the buffers
     // apart), i.e. it would wait for the NEXT tile in the middle of this one.  wait_tiles orders the DMA; the asm has no outputs.
@@ -145,58 +148,127 @@ __device__ __forceinline__ float both_sum(float v) {
 }
 
 // ---- matrix products ----------------------------------------------------------------------------------------------------------
+// Operands are bf16 as they stand (NP = 1), fp32 (NP = 1, v_mfma_f32_32x32x2_f32), or fp32 as three bf16 planes (NP = 3): x = hi + mid + lo
+// with hi = bf16(x), mid = bf16(x - hi), lo = bf16(x - hi - mid), 2^-27 of x short at most.  A product of two such numbers is six
+// bf16 products (mid lo, lo mid and lo lo are below 2^-26 of it): 6 x 32 cycles of the matrix pipe for 32 x 32 x 16 where the fp32
+// instruction takes 512, and the sums are fp32 either way.
 // Frag: a lane's own row (32 rows of a wave), the half of its features that its half wave (lh) feeds to the product over d.
 template <typename T, int DT> struct Frag;
 template <int DT> struct Frag<uint16_t, DT> { bf16x8 v[DT / 16]; };
 template <int DT> struct Frag<float, DT> { float4 v[DT / 8]; };
+template <typename T, int DT, int NP> struct Rows { Frag<T, DT> p[NP]; };
 
-template <typename T, int DT>
-__device__ __forceinline__ void load_frag(Frag<T, DT>& f, const T* row, int D, int lh, bool ok) {
-  constexpr int E = 16 / sizeof(T);                          // elements per 16-byte piece; lane lh takes the pieces 2 i + lh
+// 8 values -> their planes
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[3]) {
+  float r[8];
 #pragma unroll
-  for (int i = 0; i < DT / E / 2; ++i) {
-    const int d = (2 * i + lh) * E;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (ok && d < D) u = *reinterpret_cast<const uint4*>(row + d);
-    f.v[i] = *reinterpret_cast<const typename std::remove_reference<decltype(f.v[0])>::type*>(&u);
+  for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = cvt_pk_bf16_rne(r[2 * e], r[2 * e + 1]);
+      r[2 * e] -= __uint_as_float(w[e] << 16);
+      r[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+    }
+    const uint4 u = make_uint4(w[0], w[1], w[2], w[3]);
+    p[k] = *reinterpret_cast<const bf16x8*>(&u);
   }
+}
+
+// the lane's row of a tensor in memory (planes are made here); E: its element type there
+template <typename T, int DT, int NP>
+__device__ __forceinline__ void load_rows(Rows<T, DT, NP>& f, const void* base, int64_t at, int D, int lh, bool ok) {
+  if constexpr (NP == 1) {
+    const T* row = reinterpret_cast<const T*>(base) + at;
+    constexpr int E = 16 / sizeof(T);                        // elements per 16-byte piece; lane lh takes the pieces 2 i + lh
+#pragma unroll
+    for (int i = 0; i < DT / E / 2; ++i) {
+      const int d = (2 * i + lh) * E;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (ok && d < D) u = *reinterpret_cast<const uint4*>(row + d);
+      f.p[0].v[i] = *reinterpret_cast<const typename std::remove_reference<decltype(f.p[0].v[0])>::type*>(&u);
+    }
+  } else {
+    const float* row = reinterpret_cast<const float*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i) {
+      const int d = (2 * i + lh) * 8;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+      if (ok && d < D) {
+        a = *reinterpret_cast<const float4*>(row + d);
+        b = *reinterpret_cast<const float4*>(row + d + 4);
+      }
+      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      bf16x8 q[3];
+      split8(x, q);
+      f.p[0].v[i] = q[0]; f.p[1].v[i] = q[1]; f.p[2].v[i] = q[2];
+    }
+  }
+}
+// s += a . b over 16 features, planes from the smallest products to the largest.  SWAP: the operands' roles are exchanged against
+// another kernel's, which forms the same product: the same order there and here gives the same bits.
+template <bool SWAP> __device__ __forceinline__ void mma_planes(f32x16& s, const bf16x8 (&a)[3], const bf16x8 (&b)[3]) {
+  constexpr int I[6] = {2, 0, 1, 1, 0, 0}, J[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int k = 0; k < 6; ++k)
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[SWAP ? J[k] : I[k]], b[SWAP ? I[k] : J[k]], s, 0, 0, 0);
 }
 __device__ __forceinline__ void zero16(f32x16& a) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
 
-// s[32 tile rows][32 lane rows] += tile(rows blk * 32 ..) . frag
-template <typename T, int DT>
-__device__ __forceinline__ void mma_rows(f32x16& s, const char* tile, int blk, const Frag<T, DT>& f, int li, int lh) {
+// s[32 tile rows][32 lane rows] += tile(rows blk * 32 ..) . lane rows      (TS: bytes from plane to plane of the tile)
+template <typename T, int DT, int NP, int TS, bool SWAP = false>
+__device__ __forceinline__ void mma_rows(f32x16& s, const char* tile, int blk, const Rows<T, DT, NP>& f, int li, int lh) {
   constexpr int RB = DT * sizeof(T);
   const char* row = tile + (blk * 32 + li) * RB;
   const uint32_t x = (lh ^ Swz<RB>::of(li)) * 16;
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (NP == 3) {
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i) {
+      bf16x8 a[3], b[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        a[k] = *reinterpret_cast<const bf16x8*>(row + k * TS + (x ^ (i * 32)));
+        b[k] = f.p[k].v[i];
+      }
+      mma_planes<SWAP>(s, a, b);
+    }
+  } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < DT / 16; ++i) {
       const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + (x ^ (i * 32)));
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, f.v[i], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, f.p[0].v[i], s, 0, 0, 0);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < DT / 8; ++i) {
-      const float4 a = *reinterpret_cast<const float4*>(row + (x ^ (i * 32)));
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, f.v[i].x, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, f.v[i].y, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, f.v[i].z, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, f.v[i].w, s, 0, 0, 0);
+      const float4 a = *reinterpret_cast<const float4*>(row + (x ^ (i * 32))), b = f.p[0].v[i];
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, s, 0, 0, 0);
     }
   }
 }
 
 // x_row . y_row of the lane's own row: the diagonal of the rows' product, by the same instructions in the same order as mma_rows
 // forms a tile row's -- equal rows give equal bits, so dP - delta is 0, not a rounding, where a query sees one key alone.
-template <typename T, int DT>
-__device__ __forceinline__ float frag_dot(const Frag<T, DT>& x, const Frag<T, DT>& y, int li, int lh) {
+template <typename T, int DT, int NP>
+__device__ __forceinline__ float rows_dot(const Rows<T, DT, NP>& xs, const Rows<T, DT, NP>& ys, int li, int lh) {
+  const Frag<T, DT>&x = xs.p[0], &y = ys.p[0];
   f32x16 s;
   zero16(s);
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (NP == 3) {
+#pragma unroll
+    for (int i = 0; i < DT / 16; ++i) {
+      const bf16x8 a[3] = {x.v[i], xs.p[1].v[i], xs.p[2].v[i]}, b[3] = {y.v[i], ys.p[1].v[i], ys.p[2].v[i]};
+      mma_planes<false>(s, a, b);
+    }
+  } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < DT / 16; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v[i], y.v[i], s, 0, 0, 0);
   } else {
@@ -220,9 +292,9 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& a, int s2) {
   return *reinterpret_cast<bf16x8*>(&v);
 }
 
-// acc[dt][32 features][32 lane rows] += tile(rows blk * 32 ..)^T . p      (p: accumulator registers of a 32 x 32 product; bf16:
-// rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain)
-template <typename T, int DT>
+// acc[dt][32 features][32 lane rows] += tile(rows blk * 32 ..)^T . p      (p: accumulator registers of a 32 x 32 product.  bf16:
+// rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain; planes: split like the operands)
+template <typename T, int DT, int NP, int TS>
 __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* tile, int blk, const f32x16& p, int lane) {
   constexpr int RB = DT * sizeof(T);
   const int li = lane & 31, lh = lane >> 5;
@@ -232,18 +304,30 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* til
     const char* base = tile + (blk * 32 + r0) * RB;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      const bf16x8 pb = pack8(p, s2);
+      bf16x8 pb[3];
+      if constexpr (NP == 3) {
+        const float v[8] = {p[s2 * 8], p[s2 * 8 + 1], p[s2 * 8 + 2], p[s2 * 8 + 3], p[s2 * 8 + 4], p[s2 * 8 + 5], p[s2 * 8 + 6], p[s2 * 8 + 7]};
+        split8(v, pb);
+      } else {
+        pb[0] = pack8(p, s2);
+      }
 #pragma unroll
       for (int dt = 0; dt < DT / 32; ++dt) {
-        // rows r0 + 16 s2 and r0 + 16 s2 + 8: the swizzle of r0 + 16 s2 is that of r0 where a tile row has 8 or 16 pieces (a
-        // period of 16 rows); with 4 pieces the period is 16 too
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(base + s2 * 16 * RB + (x ^ (dt * 64)))));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(base + (s2 * 16 + 8) * RB + (x ^ (dt * 64) ^ (Swz<RB>::of(8) * 16)))));
-        const uint2 ua = *reinterpret_cast<const uint2*>(&a), ub = *reinterpret_cast<const uint2*>(&b);
-        uint4 u = make_uint4(ua.x, ua.y, ub.x, ub.y);
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<bf16x8*>(&u), pb, acc[dt], 0, 0, 0);
+        bf16x8 a[3];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          // rows r0 + 16 s2 and r0 + 16 s2 + 8: the swizzle has a period of 16 rows
+          const char* q = base + k * TS + s2 * 16 * RB;
+          const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(q + (x ^ (dt * 64)))));
+          const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(const_cast<char*>(q + 8 * RB + (x ^ (dt * 64) ^ (Swz<RB>::of(8) * 16)))));
+          const uint2 ua = *reinterpret_cast<const uint2*>(&t), ub = *reinterpret_cast<const uint2*>(&b);
+          const uint4 u = make_uint4(ua.x, ua.y, ub.x, ub.y);
+          a[k] = *reinterpret_cast<const bf16x8*>(&u);
+        }
+        if constexpr (NP == 3) mma_planes<false>(acc[dt], a, pb);
+        else acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], pb[0], acc[dt], 0, 0, 0);
       }
     }
   } else {
@@ -371,31 +455,34 @@ __device__ __forceinline__ void start_put(float* start, const KeyWords<KT> k, in
   if (all != 0xffffffffu && tid < KT) start[tid] = (w >> (tid & 31)) & 1u ? 0.f : -INFINITY;
 }
 // s = tile rows (blk * 32 ..) . f + that start (two copies of the product: a full tile's starts at the constant 0, without a register)
-template <typename T, int DT>
-__device__ __forceinline__ void mma_rows_seen(f32x16& s, const char* tile, int blk, const Frag<T, DT>& f, const float* start, uint32_t w, int li,
-                                              int lh) {
+template <typename T, int DT, int NP, int TS>
+__device__ __forceinline__ void mma_rows_seen(f32x16& s, const char* tile, int blk, const Rows<T, DT, NP>& f, const float* start, uint32_t w,
+                                              int li, int lh) {
   if (w == 0xffffffffu) {
     zero16(s);
-    mma_rows<T, DT>(s, tile, blk, f, li, lh);
+    mma_rows<T, DT, NP, TS>(s, tile, blk, f, li, lh);
   } else {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float4 x = *reinterpret_cast<const float4*>(start + g * 8 + lh * 4);
       s[g * 4] = x.x; s[g * 4 + 1] = x.y; s[g * 4 + 2] = x.z; s[g * 4 + 3] = x.w;
     }
-    mma_rows<T, DT>(s, tile, blk, f, li, lh);
+    mma_rows<T, DT, NP, TS>(s, tile, blk, f, li, lh);
   }
 }
+
 // A block's four waves are RG = 4 / KG groups of 32 rows by KG groups of keys: KG = 1 where rows fill the chip, 4 where there are
 // at most 32 of them, 2 between (and where blocks of 128 rows would be too few, or too uneven, to fill it).  A tile holds NB blocks
 // of 32 keys for each key group: two where two tiles of K and V fit in 64 KB (two blocks a CU), so that the softmax's bookkeeping is
 // shared by 64 keys.
-template <typename T, int DT, int KG> constexpr int key_blocks() { return KG == 1 && DT * sizeof(T) < 512 ? 2 : 1; }
+template <typename T, int DT, int KG, int NP> constexpr int key_blocks() { return KG == 1 && DT * sizeof(T) * NP <= 256 ? 2 : 1; }
 
-// Waves per SIMD to ask registers for: `most` where rows are shared out alone; two with key groups, one where LDS holds one block.
-template <typename T, int DT, int KG> constexpr int waves_wanted(int most) {
-  return DT * sizeof(T) >= 512 || (KG == 4 && DT * sizeof(T) >= 256) ? 1 : (KG == 1 ? most : 2);
+// Waves per SIMD to ask registers for: `most` where rows are shared out alone, as far as LDS lets them in; two with key groups.
+template <typename T, int DT, int KG, int NP> constexpr int waves_wanted(int most) {
+  return DT * sizeof(T) * NP >= 512 || (KG == 4 && DT * sizeof(T) >= 256) ? 1 : (KG == 1 ? most : 2);
 }
+template <typename T, int NP> struct OutOf { typedef T type; };
+template <typename T> struct OutOf<T, 3> { typedef float type; };
 
 // a block's share of the key tiles: split s of S takes tiles [s n / S, (s + 1) n / S) of the n that the item has
 __device__ __forceinline__ void tile_range(int n, int s, int S, int& t0, int& t1) {
@@ -416,10 +503,11 @@ template <int KG, int LDO> __device__ __forceinline__ float4 group_sum(const flo
 }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DT, int KG>
-__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG>(), KT = 32 * KG * NB;
-  constexpr int TILE = KT * RB;
+template <typename T, int DT, int KG, int NP>
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : DT * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
+  typedef typename OutOf<T, NP>::type O;
+  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
+  constexpr int TS = KT * RB, TILE = NP * TS;            // a plane of a tile, a tile
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int LDO = DT + 4;                            // rows of the join start 4 banks apart
   constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
@@ -436,7 +524,7 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   const int m0 = rt * 32 * RG, m = m0 + rg * 32 + li;
   const int qi = m / a.R, head = g * a.R + m % a.R;
   const bool live = m < Mv;
-  T* orow = reinterpret_cast<T*>(a.out) + b * a.ob + qi * a.ol + head * a.oh;
+  O* orow = reinterpret_cast<O*>(a.out) + b * a.ob + qi * a.ol + head * a.oh;
   const int64_t prow = (int64_t)bg * M + m, prows = (int64_t)a.B * a.G * M;
   float* pml = a.part ? a.part + prows * a.splits * a.D + (sp * prows + prow) * 2 : nullptr;
   int t0, t1;
@@ -446,17 +534,17 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
       if (m < M) {
         if (a.splits > 1) { if (lh == 0) { pml[0] = -INFINITY; pml[1] = 0.f; } }
         else {
-          store_zero<T, DT>(orow, a.D, lh);
+          store_zero<O, DT>(orow, a.D, lh);
           if (a.lse && lh == 0) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = -INFINITY;
         }
       }
     return;
   }
-  const T* kbase = reinterpret_cast<const T*>(a.k) + b * a.kb + g * a.kh;
-  const T* vbase = reinterpret_cast<const T*>(a.v) + b * a.vb + g * a.vh;
+  const T* kbase = reinterpret_cast<const T*>(a.t0) + b * a.t0b + g * a.t0h;
+  const T* vbase = reinterpret_cast<const T*>(a.t1) + b * a.t1b + g * a.t1h;
   const uint8_t* mask = a.mask ? a.mask + b * a.maskb : nullptr;
-  const int dbytes = a.D * (int)sizeof(T);
-  const int64_t klb = a.kl * (int64_t)sizeof(T), vlb = a.vl * (int64_t)sizeof(T);
+  const int dbytes = (NP == 3 ? DT : a.D) * (int)sizeof(T);
+  const int64_t klb = a.t0l * (int64_t)sizeof(T), vlb = a.t1l * (int64_t)sizeof(T);
 
   MaskBytes<KT> mb;
   mask_fetch(mb, mask, t0 * KT, klen, lane);
@@ -465,13 +553,16 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   kdl.init(klb, dbytes, wave, lane);
   vdl.init(vlb, dbytes, wave, lane);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
-    dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
-    dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      dma_tile<RB, KT>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + (int64_t)t * KT * a.t0l, klb, kdl, wave, kw.w);
+      dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + (int64_t)t * KT * a.t1l, vlb, vdl, wave, kw.w);
+    }
     start_put(start + buf * KT, kw, tid);
   };
   fill(t0, 0, cur);
-  Frag<T, DT> qf;
-  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
+  Rows<T, DT, NP> qf;
+  load_rows(qf, a.q, b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
   mask_fetch(mb, mask, (t0 + 1) * KT, klen, lane);
 
   f32x16 o[DT / 32];
@@ -497,7 +588,7 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
         const int blk = kg * NB + kb;
-        mma_rows_seen<T, DT>(s[kb], tk, blk, qf, start + buf * KT + blk * 32, word_at(cur, blk), li, lh);
+        mma_rows_seen<T, DT, NP, TS>(s[kb], tk, blk, qf, start + buf * KT + blk * 32, word_at(cur, blk), li, lh);
       }
       __builtin_amdgcn_s_setprio(0);
       float mt = -INFINITY;
@@ -526,13 +617,13 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           // (fp32: (s - max) SC, so that the largest P is 1 to the last bit; bf16 rounds P anyway and takes one instruction)
-          s[kb][r] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(s[kb][r], SC, off) : (s[kb][r] - sub) * SC);
+          s[kb][r] = __builtin_amdgcn_exp2f(sizeof(O) == 2 ? fmaf(s[kb][r], SC, off) : (s[kb][r] - sub) * SC);
           ls += s[kb][r];
         }
       l += ls;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT>(o, tv, kg * NB + kb, s[kb], lane);
+      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT, NP, TS>(o, tv, kg * NB + kb, s[kb], lane);
       __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {
@@ -559,8 +650,8 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
       });
       if (lh == 0 && m < M) { pml[0] = m2; pml[1] = l; }
     } else {
-      store_tile<T, DT>(smem + wave * 32 * RB, o, a.D, lane, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), true, [&](int r) {
-        return mw + r < M ? reinterpret_cast<T*>(a.out) + b * a.ob + (mw + r) / a.R * a.ol + (g * a.R + (mw + r) % a.R) * a.oh : nullptr;
+      store_tile<O, DT>(smem + wave * 32 * DT * sizeof(O), o, a.D, lane, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), true, [&](int r) {
+        return mw + r < M ? reinterpret_cast<O*>(a.out) + b * a.ob + (mw + r) / a.R * a.ol + (g * a.R + (mw + r) % a.R) * a.oh : nullptr;
       });
       if (a.lse && lh == 0 && m < M) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
     }
@@ -662,10 +753,11 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------- dQ (and delta)
 // Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
-template <typename T, int DT, int KG>
-__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG>(), KT = 32 * KG * NB;
-  constexpr int TILE = KT * RB;
+template <typename T, int DT, int KG, int NP>
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
+  typedef typename OutOf<T, NP>::type O;
+  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
+  constexpr int TS = KT * RB, TILE = NP * TS;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int LDO = DT + 4;
   constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
@@ -682,14 +774,14 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   const int m0 = rt * 32 * RG, m = m0 + rg * 32 + li;
   const int qi = m / a.R, head = g * a.R + m % a.R;
   const bool live = m < Mv;
-  T* dqrow = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + qi) * a.H + head) * a.D;
+  O* dqrow = reinterpret_cast<O*>(a.dq) + (((int64_t)b * a.Lq + qi) * a.H + head) * a.D;
   const int64_t prow = (int64_t)bg * M + m, prows = (int64_t)a.B * a.G * M;
   const int64_t srow = ((int64_t)b * a.H + head) * a.Lq + qi;
-  Frag<T, DT> qf, dof;
-  float dl = 0.f, lse2 = INFINITY;
-  load_frag<T, DT>(dof, reinterpret_cast<const T*>(a.dout) + b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
-  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.o) + b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
-  dl = frag_dot<T, DT>(qf, dof, li, lh);
+  Rows<T, DT, NP> qf, dof;
+  float lse2 = INFINITY;
+  load_rows(dof, a.dout, b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
+  load_rows(qf, a.o, b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
+  const float dl = rows_dot(qf, dof, li, lh);
   if (live) {
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
@@ -700,15 +792,15 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   if (m0 >= Mv || t0 >= t1) {
     if (m < M && kg == 0) {
       if (a.splits > 1) store_zero<float, DT>(a.part + (sp * prows + prow) * a.D, a.D, lh);
-      else store_zero<T, DT>(dqrow, a.D, lh);
+      else store_zero<O, DT>(dqrow, a.D, lh);
     }
     return;
   }
-  const T* kbase = reinterpret_cast<const T*>(a.k) + b * a.kb + g * a.kh;
-  const T* vbase = reinterpret_cast<const T*>(a.v) + b * a.vb + g * a.vh;
+  const T* kbase = reinterpret_cast<const T*>(a.t0) + b * a.t0b + g * a.t0h;
+  const T* vbase = reinterpret_cast<const T*>(a.t1) + b * a.t1b + g * a.t1h;
   const uint8_t* mask = a.mask ? a.mask + b * a.maskb : nullptr;
-  const int dbytes = a.D * (int)sizeof(T);
-  const int64_t klb = a.kl * (int64_t)sizeof(T), vlb = a.vl * (int64_t)sizeof(T);
+  const int dbytes = (NP == 3 ? DT : a.D) * (int)sizeof(T);
+  const int64_t klb = a.t0l * (int64_t)sizeof(T), vlb = a.t1l * (int64_t)sizeof(T);
   MaskBytes<KT> mb;
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
@@ -716,12 +808,15 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
   kdl.init(klb, dbytes, wave, lane);
   vdl.init(vlb, dbytes, wave, lane);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
-    dma_tile<RB, KT>(smem, buf * 2 * TILE, kbase + (int64_t)t * KT * a.kl, klb, kdl, wave, kw.w);
-    dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE, vbase + (int64_t)t * KT * a.vl, vlb, vdl, wave, kw.w);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      dma_tile<RB, KT>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + (int64_t)t * KT * a.t0l, klb, kdl, wave, kw.w);
+      dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + (int64_t)t * KT * a.t1l, vlb, vdl, wave, kw.w);
+    }
     start_put(start + buf * KT, kw, tid);
   };
   fill(t0, 0, cur);
-  load_frag<T, DT>(qf, reinterpret_cast<const T*>(a.q) + b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
+  load_rows(qf, a.q, b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
   mask_fetch(mb, mask, (t0 + 1) * KT, klen, lane);
   f32x16 dq[DT / 32];
 #pragma unroll
@@ -747,13 +842,13 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
       f32x16 s, dp;
       zero16(dp);
       __builtin_amdgcn_s_setprio(1);
-      mma_rows_seen<T, DT>(s, tk, blk, qf, start + buf * KT + blk * 32, w, li, lh);      // (unseen: P = exp2(-inf) = 0)
-      mma_rows<T, DT>(dp, tv, blk, dof, li, lh);
+      mma_rows_seen<T, DT, NP, TS>(s, tk, blk, qf, start + buf * KT + blk * 32, w, li, lh);      // (unseen: P = exp2(-inf) = 0)
+      mma_rows<T, DT, NP, TS>(dp, tv, blk, dof, li, lh);
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)) * (dp[r] - dl);
       __builtin_amdgcn_s_setprio(1);
-      mma_cols<T, DT>(dq, tk, blk, s, lane);
+      mma_cols<T, DT, NP, TS>(dq, tk, blk, s, lane);
       __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {
@@ -771,8 +866,8 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG>(DT * sizeof(T) <= 128
         return mw + r < M ? a.part + (sp * prows + (int64_t)bg * M + mw + r) * a.D : nullptr;
       });
     else
-      store_tile<T, DT>(smem + wave * 32 * RB, dq, a.D, lane, a.scale, true, [&](int r) {
-        return mw + r < M ? reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.Lq + (mw + r) / a.R) * a.H + g * a.R + (mw + r) % a.R) * a.D : nullptr;
+      store_tile<O, DT>(smem + wave * 32 * DT * sizeof(O), dq, a.D, lane, a.scale, true, [&](int r) {
+        return mw + r < M ? reinterpret_cast<O*>(a.dq) + (((int64_t)b * a.Lq + (mw + r) / a.R) * a.H + g * a.R + (mw + r) % a.R) * a.D : nullptr;
       });
   } else {
     float* so = reinterpret_cast<float*>(smem);          // sums over the key groups
@@ -822,13 +917,16 @@ template <int N> __device__ __forceinline__ void add_from(f32x16 (&acc)[N], char
 }
 
 // A block owns 32 KW keys (KW = 4, or 2 where that would be too few blocks), a lane one key: its K and V rows stay in registers.
-// The block walks tiles of 64 query rows, head after head of the group; with KW = 2 two waves share the keys and each takes half of
+// The block walks tiles of 64 query rows (32 of planes), head after head of the group; with KW = 2 two waves share the keys and each takes half of
 // a tile's rows.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen key computes
 // stays in its own lane; zeros are stored for it.
-template <typename T, int DT> constexpr int DKV_UNROLL = DT * sizeof(T) >= 256 ? 1 : 2;        // (twice the registers spill)
-template <typename T, int DT, int KW>
-__global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
-  constexpr int RB = DT * sizeof(T), RT = 64, TILE = RT * RB, RW = 4 / KW;
+template <typename T, int DT, int NP> constexpr int DKV_UNROLL = DT * sizeof(T) * NP >= 256 ? 1 : 2;        // (twice the registers spill)
+template <typename T, int DT, int KW, int NP>
+__global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(T) * NP >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
+  typedef typename OutOf<T, NP>::type O;
+  constexpr int RB = DT * sizeof(T), RT = NP == 3 ? 32 : 64, TS = RT * RB, TILE = NP * TS, RW = 4 / KW, NBLK = RT / 32 / RW;
+  constexpr int SHARE = 32 * DT * 4;                     // LDS of a wave for its results, once the tiles are done with
+  static_assert(NBLK >= 1 && 4 * SHARE <= 4 * TILE, "");
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
   const int kwv = wave / RW, rwv = wave % RW;
@@ -849,14 +947,14 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
         store_zero<float, DT>(a.part + (sp * 2 * krows + krow) * a.D, a.D, lh);
         store_zero<float, DT>(a.part + ((sp * 2 + 1) * krows + krow) * a.D, a.D, lh);
       } else {
-        store_zero<T, DT>(reinterpret_cast<T*>(a.dk) + krow * a.D, a.D, lh);
-        store_zero<T, DT>(reinterpret_cast<T*>(a.dv) + krow * a.D, a.D, lh);
+        store_zero<O, DT>(reinterpret_cast<O*>(a.dk) + krow * a.D, a.D, lh);
+        store_zero<O, DT>(reinterpret_cast<O*>(a.dv) + krow * a.D, a.D, lh);
       }
     }
     return;
   }
-  const int dbytes = a.D * (int)sizeof(T);
-  const int64_t qlb = a.ql * (int64_t)sizeof(T), glb = a.gl * (int64_t)sizeof(T);
+  const int dbytes = (NP == 3 ? DT : a.D) * (int)sizeof(T);
+  const int64_t qlb = a.t0l * (int64_t)sizeof(T), glb = a.t1l * (int64_t)sizeof(T);
   float* stat = reinterpret_cast<float*>(smem + 4 * TILE);         // [buf][lse2 | delta][RT]
   float sreg = 0.f;
   DmaLane<RB> qdl, gdl;
@@ -867,8 +965,13 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     uint32_t w[RT / 32];
 #pragma unroll
     for (int i = 0; i < RT / 32; ++i) w[i] = left >= 32 * (i + 1) ? 0xffffffffu : (left <= 32 * i ? 0u : (1u << (left - 32 * i)) - 1u);
-    dma_tile<RB, RT>(smem, buf * 2 * TILE, reinterpret_cast<const T*>(a.q) + b * a.qb + (int64_t)q0 * a.ql + head * a.qh, qlb, qdl, wave, w);
-    dma_tile<RB, RT>(smem, buf * 2 * TILE + TILE, reinterpret_cast<const T*>(a.dout) + b * a.gb + (int64_t)q0 * a.gl + head * a.gh, glb, gdl, wave, w);
+    const T* qp = reinterpret_cast<const T*>(a.t0) + b * a.t0b + (int64_t)q0 * a.t0l + head * a.t0h;
+    const T* gp = reinterpret_cast<const T*>(a.t1) + b * a.t1b + (int64_t)q0 * a.t1l + head * a.t1h;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      dma_tile<RB, RT>(smem, buf * 2 * TILE + k * TS, qp + k * a.t0p, qlb, qdl, wave, w);
+      dma_tile<RB, RT>(smem, buf * 2 * TILE + TILE + k * TS, gp + k * a.t1p, glb, gdl, wave, w);
+    }
     if (tid < 2 * RT) {
       const int q = q0 + tid % RT;
       const int64_t s = ((int64_t)b * a.H + head) * a.Lq + q;
@@ -881,9 +984,9 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
   };
   auto put_stat = [&](int buf) { if (tid < 2 * RT) stat[buf * 2 * RT + tid] = sreg; };
   fill(t0, 0);
-  Frag<T, DT> kf, vf;
-  load_frag<T, DT>(kf, reinterpret_cast<const T*>(a.k) + b * a.kb + (int64_t)key * a.kl + g * a.kh, a.D, lh, seen);
-  load_frag<T, DT>(vf, reinterpret_cast<const T*>(a.v) + b * a.vb + (int64_t)key * a.vl + g * a.vh, a.D, lh, seen);
+  Rows<T, DT, NP> kf, vf;
+  load_rows(kf, a.k, b * a.kb + (int64_t)key * a.kl + g * a.kh, a.D, lh, seen);
+  load_rows(vf, a.v, b * a.vb + (int64_t)key * a.vl + g * a.vh, a.D, lh, seen);
   f32x16 dk[DT / 32], dv[DT / 32];
 #pragma unroll
   for (int i = 0; i < DT / 32; ++i) { zero16(dk[i]); zero16(dv[i]); }
@@ -897,15 +1000,15 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
     const char* tg = tq + TILE;
     const float* st = stat + buf * 2 * RT;
     if (some)                                            // (a wave whose keys are all unseen only helps to load)
-#pragma unroll DKV_UNROLL<T, DT>
-    for (int hb = 0; hb < 2 / RW; ++hb) {
-      const int blk = rwv * (2 / RW) + hb;
+#pragma unroll DKV_UNROLL<T, DT, NP>
+    for (int hb = 0; hb < NBLK; ++hb) {
+      const int blk = rwv * NBLK + hb;
       f32x16 s, dp;
       zero16(s);
       zero16(dp);
       __builtin_amdgcn_s_setprio(1);
-      mma_rows<T, DT>(s, tq, blk, kf, li, lh);
-      mma_rows<T, DT>(dp, tg, blk, vf, li, lh);
+      mma_rows<T, DT, NP, TS, true>(s, tq, blk, kf, li, lh);
+      mma_rows<T, DT, NP, TS, true>(dp, tg, blk, vf, li, lh);
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
@@ -920,32 +1023,31 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) >= 512 ? 1 : DT * sizeof(T) >=
         }
       }
       __builtin_amdgcn_s_setprio(1);
-      mma_cols<T, DT>(dv, tg, blk, s, lane);
-      mma_cols<T, DT>(dk, tq, blk, dp, lane);
+      mma_cols<T, DT, NP, TS>(dv, tg, blk, s, lane);
+      mma_cols<T, DT, NP, TS>(dk, tq, blk, dp, lane);
       __builtin_amdgcn_s_setprio(0);
     }
     if (t + 1 < t1) put_stat(buf ^ 1);
     wait_tiles();
   }
   if constexpr (RW == 2) {                               // the second half of the rows joins the first
-    add_from(dk, smem + kwv * 32 * DT * 4, lane, rwv == 1);
-    add_from(dv, smem + kwv * 32 * DT * 4, lane, rwv == 1);
+    add_from(dk, smem + kwv * SHARE, lane, rwv == 1);
+    add_from(dv, smem + kwv * SHARE, lane, rwv == 1);
     if (rwv == 1) return;
   }
   const int kw = kt * 32 * KW + kwv * 32;
   if (a.splits > 1) {
     float* pk = a.part + sp * 2 * krows * a.D;
     float* pv = pk + krows * a.D;
-    static_assert(32 * DT * 4 <= TILE, "");
     auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; }; };
-    store_tile<float, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(pk));
-    store_tile<float, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(pv));
+    store_tile<float, DT>(smem + wave * SHARE, dk, a.D, lane, a.scale, seen, at(pk));
+    store_tile<float, DT>(smem + wave * SHARE, dv, a.D, lane, 1.f, seen, at(pv));
   } else {
     auto at = [&](void* base) {
-      return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<T*>(base) + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; };
+      return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<O*>(base) + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; };
     };
-    store_tile<T, DT>(smem + wave * TILE, dk, a.D, lane, a.scale, seen, at(a.dk));
-    store_tile<T, DT>(smem + wave * TILE, dv, a.D, lane, 1.f, seen, at(a.dv));
+    store_tile<O, DT>(smem + wave * SHARE, dk, a.D, lane, a.scale, seen, at(a.dk));
+    store_tile<O, DT>(smem + wave * SHARE, dv, a.D, lane, 1.f, seen, at(a.dv));
   }
 }
 
@@ -976,6 +1078,40 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a) {
   else *reinterpret_cast<float4*>(p) = x;
 }
 
+// fp32 [B, L, Hn, D] -> bf16 planes [3][B][Hn][L][W], features D .. W - 1 zero; rows at or past len[b] are left out (no tile reads
+// them).  Up to four tensors a launch (grid z); 10 bytes of memory traffic an element.
+struct SplitArgs {
+  const float* src[4];
+  uint16_t* dst[4];
+  const int64_t* len[4];
+  int64_t sb[4], sl[4], sh[4];
+  int L[4], Hn[4];
+  int B, D, W;
+};
+__global__ __launch_bounds__(256) void xattn_split_kernel(SplitArgs a) {
+  const int z = blockIdx.z, L = a.L[z], Hn = a.Hn[z], ppr = a.W / 8;         // 8-feature pieces per row
+  const int64_t plane = (int64_t)a.B * Hn * L * a.W;
+  for (int bh = blockIdx.y; bh < a.B * Hn; bh += gridDim.y) {
+    const int b = bh / Hn, h = bh - b * Hn, n = clamp_len(a.len[z], b, L);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)n * ppr; i += (int64_t)gridDim.x * 256) {
+      const int64_t l = i / ppr;
+      const int d = (int)(i - l * ppr) * 8;
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+      if (d < a.D) {
+        const float* p = a.src[z] + b * a.sb[z] + l * a.sl[z] + h * a.sh[z] + d;
+        u = *reinterpret_cast<const float4*>(p);
+        v = *reinterpret_cast<const float4*>(p + 4);
+      }
+      const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      bf16x8 q[3];
+      split8(x, q);
+      uint16_t* o = a.dst[z] + ((int64_t)bh * L + l) * a.W + d;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(o + k * plane) = q[k];
+    }
+  }
+}
+
 // How many shares of a long axis (n tiles) give the launch about `want` blocks, each with at least `least` tiles.
 int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   int64_t s = (want + blocks - 1) / blocks;
@@ -984,26 +1120,33 @@ int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : (int)s;
 }
-struct Plan { int kg, nrt, fwd, dq, kw, nkt, dkv; };
-// Sizes alone decide.  512 blocks are two per CU.  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
+struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; };
+// Sizes alone decide.  512 blocks are two per CU, and shares are cut to reach that (2 x 65537 keys of one token: 256 blocks, one per CU,
+// 110 us, 512 113, 1024 118).  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
 // 81 us (every share writes its part once more); two key groups from 512 blocks of 128 rows down: 8 x 500 x 700 49 us, from 1024: the
-// fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).
+// fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).  fp32 with more than 64 rows a key head goes through
+// planes (their making pays from there on); with fewer it is bound by reading the keys, which planes would do twice.
 Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   Plan p;
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
-  const int rb = (D <= 32 ? 32 : D <= 64 ? 64 : 128) * (bf16 ? 2 : 4);
-  p.kg = M <= 32 ? 4 : M <= 64 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
+  p.width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+  p.planes = !bf16 && M > 64 ? 3 : 1;
+  const int row = p.width * (bf16 || p.planes == 3 ? 2 : 4) * p.planes;
+  p.kg = p.planes == 3 ? 1 : M <= 32 ? 4 : M <= 64 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
   const int rows = 128 / p.kg;
   p.nrt = (int)((M + rows - 1) / rows);
-  const int KT = 32 * p.kg * (p.kg == 1 && rb < 512 ? 2 : 1);
+  const int KT = 32 * p.kg * (p.kg == 1 && row <= 256 ? 2 : 1);
   const int64_t kt = (Lk + KT - 1) / KT;
-  p.fwd = split_count(BG * p.nrt, kt, 512, 2);
-  p.dq = split_count(BG * p.nrt, kt, 512, 4);
-  p.kw = BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
+  const int want = row >= 512 || (p.kg == 4 && row >= 256) ? 256 : 512;        // (LDS holds one block of these per CU)
+  p.fwd = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 2 : 128 / KT);
+  p.dq = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 4 : 256 / KT);
+  p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
-  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + 63) / 64) * (H / G), 512, 8);
+  const int RT = p.planes == 3 ? 32 : 64;
+  p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), row >= 512 ? 256 : 512, 512 / RT);
   return p;
 }
+int64_t plane_bytes(const Plan& p, int B, int L, int Hn) { return p.planes == 3 ? (int64_t)6 * B * L * Hn * p.width : 0; }
 
 // Runs of logical blocks per XCD (see xcd_block): as long as the blocks of one (item, key head), but never fewer than 64 runs
 // -- eight per XCD, so that ragged items even out.
@@ -1017,24 +1160,32 @@ dim3 grid_for(XArgs& a) {
 }
 
 template <typename T, int DT>
-void launch_fwd(XArgs& a, int kg, hipStream_t st) {
+void launch_fwd(XArgs& a, const Plan& p, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (kg == 4) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
-  else if (kg == 2) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1>), g, dim3(256), 0, st, a);
+  if (p.kg == 4) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 4, 1>), g, dim3(256), 0, st, a);
+  else if (p.kg == 2) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2, 1>), g, dim3(256), 0, st, a);
+  else if constexpr (sizeof(T) == 2) {
+    if (p.planes == 3) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 3>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 1>), g, dim3(256), 0, st, a);
+  }
 }
 template <typename T, int DT>
-void launch_dq(XArgs& a, int kg, hipStream_t st) {
+void launch_dq(XArgs& a, const Plan& p, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (kg == 4) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
-  else if (kg == 2) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1>), g, dim3(256), 0, st, a);
+  if (p.kg == 4) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 4, 1>), g, dim3(256), 0, st, a);
+  else if (p.kg == 2) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2, 1>), g, dim3(256), 0, st, a);
+  else if constexpr (sizeof(T) == 2) {
+    if (p.planes == 3) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 3>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 1>), g, dim3(256), 0, st, a);
+  }
 }
 template <typename T, int DT>
-void launch_dkv(XArgs& a, int kw, hipStream_t st) {
+void launch_dkv(XArgs& a, const Plan& p, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (kw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 4>), g, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 2>), g, dim3(256), 0, st, a);
+  if (p.planes == 3) {
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 4, 3>), g, dim3(256), 0, st, a);
+  } else if (p.kw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 4, 1>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_dkv_kernel<T, DT, 2, 1>), g, dim3(256), 0, st, a);
 }
 #define BY_WIDTH(T, CALL)              \
   do {                                 \
@@ -1080,12 +1231,42 @@ extern "C" int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk,
   if (B < 1 || Lq < 1 || Lk < 1 || G < 1 || H < G || H % G || D < 8 || D > 128) return 0;
   const Plan p = make_plan(B, Lq, Lk, H, G, D, bf16);
   const int64_t qrows = (int64_t)B * H * Lq, krows = (int64_t)B * G * Lk;
-  if (!bwd) return p.fwd > 1 ? 4 * p.fwd * qrows * (D + 2) : 0;
+  const int64_t kv = 2 * plane_bytes(p, B, Lk, G);
+  if (!bwd) return (p.fwd > 1 ? (4 * p.fwd * qrows * (D + 2) + 15) / 16 * 16 : 0) + kv;
   int64_t part = p.dq > 1 ? p.dq * qrows * D : 0;
-  const int64_t kv = p.dkv > 1 ? 2 * p.dkv * krows * D : 0;
-  if (kv > part) part = kv;                              // the two gradients' launches follow each other: one buffer
-  return 4 * (part + (qrows + 3) / 4 * 4);
+  const int64_t pkv = p.dkv > 1 ? 2 * p.dkv * krows * D : 0;
+  if (pkv > part) part = pkv;                            // the two gradients' launches follow each other: one buffer
+  return 4 * (part + (qrows + 3) / 4 * 4) + kv + 2 * plane_bytes(p, B, Lq, H);
 }
+
+namespace {
+// the tensors' planes, one after the other at `at`
+struct SplitJob { const void* src; int64_t sb, sl, sh; int L, Hn; const int64_t* len; };
+void launch_split(const SplitJob* job, int n, uint16_t* at, const XArgs& a, const Plan& p, hipStream_t st) {
+  SplitArgs s = {};
+  s.B = a.B; s.D = a.D; s.W = p.width;
+  int most = 0, heads = 0;
+  for (int i = 0; i < n; ++i) {
+    s.src[i] = (const float*)job[i].src; s.dst[i] = at; s.len[i] = job[i].len;
+    s.sb[i] = job[i].sb; s.sl[i] = job[i].sl; s.sh[i] = job[i].sh; s.L[i] = job[i].L; s.Hn[i] = job[i].Hn;
+    at += (int64_t)3 * a.B * job[i].L * job[i].Hn * p.width;
+    if (job[i].L > most) most = job[i].L;
+    if (job[i].Hn > heads) heads = job[i].Hn;
+  }
+  const int64_t x = ((int64_t)most * (p.width / 8) + 255) / 256, y = (int64_t)a.B * heads;
+  hipLaunchKernelGGL(xattn_split_kernel, dim3((unsigned)(x < 1024 ? x : 1024), (unsigned)(y < 65535 ? y : 65535), n), dim3(256), 0, st, s);
+}
+// tiles come from the tensors themselves, or from their planes
+void tiles_from(XArgs& a, const void* x0, int64_t b0, int64_t l0, int64_t h0, const void* x1, int64_t b1, int64_t l1, int64_t h1) {
+  a.t0 = x0; a.t0b = b0; a.t0l = l0; a.t0h = h0; a.t0p = 0;
+  a.t1 = x1; a.t1b = b1; a.t1l = l1; a.t1h = h1; a.t1p = 0;
+}
+void tiles_from_planes(XArgs& a, const uint16_t* x0, int L, int Hn, int W) {
+  const int64_t plane = (int64_t)a.B * Hn * L * W;
+  tiles_from(a, x0, (int64_t)Hn * L * W, W, (int64_t)L * W, x0 + 3 * plane, (int64_t)Hn * L * W, W, (int64_t)L * W);
+  a.t0p = a.t1p = plane;
+}
+}  // namespace
 
 extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check(x, false)) return rc;
@@ -1095,8 +1276,16 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   a.nrt = p.nrt; a.splits = p.fwd; a.part = p.fwd > 1 ? (float*)workspace : nullptr;
-#define FWD(T, W) launch_fwd<T, W>(a, p.kg, st)
-  if (x->bf16) BY_WIDTH(uint16_t, FWD); else BY_WIDTH(float, FWD);
+  if (p.planes == 3) {
+    uint16_t* planes = (uint16_t*)((char*)workspace + need - 2 * plane_bytes(p, x->B, x->Lk, x->G));
+    const SplitJob job[2] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, x->len}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, x->len}};
+    launch_split(job, 2, planes, a, p, st);
+    tiles_from_planes(a, planes, x->Lk, x->G, p.width);
+  } else {
+    tiles_from(a, x->k, x->kb, x->kl, x->kh, x->v, x->vb, x->vl, x->vh);
+  }
+#define FWD(T, W) launch_fwd<T, W>(a, p, st)
+  if (x->bf16 || p.planes == 3) BY_WIDTH(uint16_t, FWD); else BY_WIDTH(float, FWD);
 #undef FWD
   if (p.fwd > 1) {
     const unsigned blocks = (unsigned)(((int64_t)x->B * x->H * x->Lq + 3) / 4);
@@ -1117,18 +1306,30 @@ extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspa
   const int64_t qrows = (int64_t)x->B * x->H * x->Lq, krows = (int64_t)x->B * x->G * x->Lk;
   a.delta = (float*)workspace;
   a.part = (float*)workspace + (qrows + 3) / 4 * 4;
+  const int64_t kvb = 2 * plane_bytes(p, x->B, x->Lk, x->G), qb = 2 * plane_bytes(p, x->B, x->Lq, x->H);
+  uint16_t* planes = (uint16_t*)((char*)workspace + need - kvb - qb);        // k, v, q, dout
+  if (p.planes == 3) {
+    const SplitJob job[4] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, x->len}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, x->len},
+                             {x->q, x->qb, x->ql, x->qh, x->Lq, x->H, x->q_len}, {x->dout, x->gb, x->gl, x->gh, x->Lq, x->H, x->q_len}};
+    launch_split(job, 4, planes, a, p, st);
+    tiles_from_planes(a, planes, x->Lk, x->G, p.width);
+  } else {
+    tiles_from(a, x->k, x->kb, x->kl, x->kh, x->v, x->vb, x->vl, x->vh);
+  }
   a.nrt = p.nrt; a.splits = p.dq;
-#define DQ(T, W) launch_dq<T, W>(a, p.kg, st)
-  if (x->bf16) BY_WIDTH(uint16_t, DQ); else BY_WIDTH(float, DQ);
+#define DQ(T, W) launch_dq<T, W>(a, p, st)
+  if (x->bf16 || p.planes == 3) BY_WIDTH(uint16_t, DQ); else BY_WIDTH(float, DQ);
 #undef DQ
   if (p.dq > 1) {
     const unsigned blocks = (unsigned)((qrows * (x->D / 4) + 255) / 256);
     if (x->bf16) hipLaunchKernelGGL((xattn_sum_kernel<uint16_t, true>), dim3(blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((xattn_sum_kernel<float, true>), dim3(blocks), dim3(256), 0, st, a);
   }
+  if (p.planes == 3) tiles_from_planes(a, planes + kvb / 2, x->Lq, x->H, p.width);
+  else tiles_from(a, x->q, x->qb, x->ql, x->qh, x->dout, x->gb, x->gl, x->gh);
   a.nrt = p.nkt; a.splits = p.dkv;
-#define DKV(T, W) launch_dkv<T, W>(a, p.kw, st)
-  if (x->bf16) BY_WIDTH(uint16_t, DKV); else BY_WIDTH(float, DKV);
+#define DKV(T, W) launch_dkv<T, W>(a, p, st)
+  if (x->bf16 || p.planes == 3) BY_WIDTH(uint16_t, DKV); else BY_WIDTH(float, DKV);
 #undef DKV
   if (p.dkv > 1) {
     const unsigned blocks = (unsigned)((2 * krows * (x->D / 4) + 255) / 256);
