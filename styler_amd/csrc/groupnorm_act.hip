@@ -229,16 +229,16 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       }
     col_sums<V, T>(s, q, red, sa, sb, cv, RL, on);
     // a wave per group: channel c has mean K + s / n and M2 = q - s^2 / n; all its channels have n values
-    const float fn = (float)n, inv = n > 0 ? 1.f / fn : 0.f, icg = 1.f / (float)a.cg;
+    const float fn = (float)n;
     for (int g = tid >> 6; g < ng; g += T / 64) {
       float m = 0.f, m2 = 0.f;
-      for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) m += sk[j] + sa[j] * inv;
-      const float mean = wave_sum(m) * icg;
+      for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) m += n > 0 ? sk[j] + sa[j] / fn : 0.f;
+      const float mean = wave_sum(m) / (float)a.cg;
       for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) {
-        const float sm = sa[j] * inv, d = (sk[j] + sm) - mean;
+        const float sm = n > 0 ? sa[j] / fn : 0.f, d = (sk[j] + sm) - mean;
         m2 += fmaxf(0.f, sb[j] - sa[j] * sm) + fn * d * d;
       }
-      const float var = wave_sum(m2) * (inv * icg), rstd = n > 0 ? rsqrtf(var + a.eps) : 0.f;
+      const float var = wave_sum(m2) / (fn * (float)a.cg), rstd = n > 0 ? 1.f / sqrtf(var + a.eps) : 0.f;
       if (lane == 0) {
         gm[2 * g] = n > 0 ? mean : 0.f;
         gm[2 * g + 1] = rstd;
@@ -294,13 +294,13 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
     col_sums<V, T>(s, q, red, sa, sb, cv, RL, on);
     for (int j = tid; j < W; j += T)                     // this item's share of the parameter gradients
       *reinterpret_cast<float2*>(a.pw + ((int64_t)b * a.C + c0 + j) * 2) = make_float2(sa[j], sb[j]);
-    const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
+    const float count = (float)max(n, 1) * (float)a.cg;
     for (int g = tid >> 6; g < ng; g += T / 64) {
       float m1 = 0.f, m2 = 0.f;
       for (int j = g * a.cg + lane; j < (g + 1) * a.cg; j += 64) { m1 = fmaf(sa[j], a.gamma[c0 + j], m1); m2 = fmaf(sb[j], a.gamma[c0 + j], m2); }
       m1 = wave_sum(m1);
       m2 = wave_sum(m2);
-      if (lane == 0) { gm[2 * g] = m1 * inv; gm[2 * g + 1] = m2 * inv; }
+      if (lane == 0) { gm[2 * g] = m1 / count; gm[2 * g + 1] = m2 / count; }
     }
     __syncthreads();
     if (!on) return;
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw, float*
   const int n = gn_len(a.len, b, a.L), live = (n + a.rows - 1) / a.rows;
   const int cl = min(a.cg, 256), RL = 256 / cl, r0 = tid / cl, c = tid - r0 * cl;
   const float* ws = a.ws + (int64_t)b * a.chunks * a.C * 2;
-  const float inv = n > 0 ? 1.f / ((float)n * a.cg) : 0.f;
+  const float count = (float)max(n, 1) * (float)a.cg;
   float x = 0.f, y = 0.f;
   for (int c0 = 0; c0 < a.cg; c0 += cl) {                // (one turn unless a group has more than 256 channels)
     const int ch = g * a.cg + c0 + c;
@@ -454,9 +454,9 @@ __global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw, float*
     }
   }
   __syncthreads();
-  x = block_sum256(x, red[0]) * inv;
+  x = block_sum256(x, red[0]) / count;
   if constexpr (BWD) {
-    y = block_sum256(y, red[1]) * inv;
+    y = block_sum256(y, red[1]) / count;
   } else {
     for (int c0 = 0; c0 < a.cg; c0 += cl) {
       if (r0 >= RL || c0 + c >= a.cg) continue;
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw, float*
         y += fmaf((float)(min(n, (i + 1) * a.rows) - i * a.rows), d * d, p.y);
       }
     }
-    y = rsqrtf(block_sum256(y, red[1]) * inv + a.eps);
+    y = 1.f / sqrtf(block_sum256(y, red[1]) / count + a.eps);
   }
   if (tid == 0) {
     float* st = (BWD ? gw : a.stats) + ((int64_t)b * a.G + g) * 2;
