@@ -1243,7 +1243,8 @@ int check(const styler_xattn_t* x, bool bwd) {
   if (bwd && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse)) return STYLER_EINVAL;
   const Plan pl = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
   const int64_t bg = (int64_t)x->B * x->G;
-  if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0x60000000 || bg * pl.nkt * pl.dkv > 0x60000000) return STYLER_EINVAL;
+  // a launch has fewer than 2^32 threads, the padding of the runs (grid_for: one eighth at most) among them
+  if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0xe00000 || (bwd && bg * pl.nkt * pl.dkv > 0xe00000)) return STYLER_EINVAL;
   return 0;
 }
 XArgs args(const styler_xattn_t* x) {

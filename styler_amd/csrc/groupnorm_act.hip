@@ -607,7 +607,8 @@ int gn_vec(const styler_gn_t* x, bool bwd) {
 }
 int gn_check(const styler_gn_t* x, bool bwd) {
   if (!x || !x->x || !x->out || !x->gamma || !x->beta || x->B < 1 || x->L < 1 || x->C < 1 || x->G < 1 || x->C % x->G) return STYLER_EINVAL;
-  if (x->B > 65535 || x->L > (1 << 30) || !(x->eps >= 0.f)) return STYLER_EINVAL;
+  if (x->L > (1 << 30) || !(x->eps >= 0.f)) return STYLER_EINVAL;
+  if (x->G > 1 << 22 || (x->C + 63) / 64 > 65535) return STYLER_EINVAL;                  // (grids: 65535 slabs, 2^32 threads)
   if (x->act != STYLER_ACT_NONE && x->act != STYLER_ACT_RELU && x->act != STYLER_ACT_SILU && x->act != STYLER_ACT_GELU) return STYLER_EINVAL;
   if (bwd && (!x->dy || !x->dgamma || !x->dbeta || !x->stats)) return STYLER_EINVAL;
   const uintptr_t es = x->bf16 ? 2 : 4;
@@ -663,6 +664,22 @@ void gn_dispatch(const GArgs& a, const GPlan& p, int bf16, int act, float* gw, h
     else gn_by_act<false, 1, BWD>(a, p, act, gw, st);
   }
 }
+// as many items a launch as a grid holds: 65535 in y and z, 2^32 threads in x
+template <bool BWD>
+void gn_run(const GArgs& all, const GPlan& p, int bf16, int act, float* gw, hipStream_t st) {
+  const int64_t es = bf16 ? 2 : 4, step = p.fused ? ((int64_t)1 << 31) / ((int64_t)p.T * p.slabs) : 65528;
+  for (int64_t b0 = 0; b0 < all.B; b0 += step) {
+    GArgs a = all;
+    a.B = (int)(all.B - b0 < step ? all.B - b0 : step);
+    a.x = (const char*)all.x + b0 * all.xb * es;
+    a.out = (char*)all.out + b0 * all.ob * es;
+    if (BWD) { a.dy = (const char*)all.dy + b0 * all.db * es; a.pw = all.pw + 2 * b0 * all.C; }
+    if (all.stats) a.stats = all.stats + 2 * b0 * all.G;
+    if (!p.fused) a.ws = all.ws + 2 * b0 * p.chunks * all.C;
+    if (all.len) a.len = all.len + b0;
+    gn_dispatch<BWD>(a, p, bf16, act, BWD ? gw + 2 * b0 * all.G : nullptr, st);
+  }
+}
 
 }  // namespace
 
@@ -689,7 +706,7 @@ extern "C" int styler_groupnorm_act(const styler_gn_t* x, void* workspace, int64
   GArgs a = gn_args(x, p);
   if (!a.stats && !p.fused) a.stats = (float*)workspace;
   a.ws = workspace ? (float*)workspace + 2 * (int64_t)x->B * x->G : nullptr;
-  gn_dispatch<false>(a, p, x->bf16, x->act, nullptr, (hipStream_t)stream);
+  gn_run<false>(a, p, x->bf16, x->act, nullptr, (hipStream_t)stream);
   return launch_status();
 }
 
@@ -701,7 +718,7 @@ extern "C" int styler_groupnorm_act_bwd(const styler_gn_t* x, void* workspace, i
   GArgs a = gn_args(x, p);
   a.pw = (float*)workspace + 2 * (int64_t)x->B * x->G;
   a.ws = a.pw + 2 * (int64_t)x->B * x->C;
-  gn_dispatch<true>(a, p, x->bf16, x->act, (float*)workspace, (hipStream_t)stream);
+  gn_run<true>(a, p, x->bf16, x->act, (float*)workspace, (hipStream_t)stream);
   hipLaunchKernelGGL(gn_params_kernel, dim3((x->C + 255) / 256), dim3(256), 0, (hipStream_t)stream, a, (const float*)a.pw);
   return launch_status();
 }

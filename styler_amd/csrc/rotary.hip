@@ -188,6 +188,7 @@ extern "C" int styler_rotary(const styler_rotary_t* p, void* stream) {
   if (rpb < 1) rpb = 1;
   a.rpb = (int)rpb;
   const int64_t blocks = (a.rows + rpb - 1) / rpb;
+  if (blocks > 0xffffff) return STYLER_EINVAL;                             // (2^32 threads a launch; 512 items a block: 17 GB of bf16 pairs)
   const size_t lds = (size_t)rpb * (rot / 2 * 8 + 16);
   hipStream_t s = (hipStream_t)stream;
 #define GO(B16, I, V) hipLaunchKernelGGL((rotary_kernel<B16, I, V>), dim3((unsigned)blocks), dim3(256), lds, s, a)

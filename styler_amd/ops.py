@@ -1969,6 +1969,8 @@ def _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, writes):
         _like(name, out, "out", qs, q.dtype, device)
         if writes and not (_rows_ok(qs, out.stride()) and _heads(out, 2 if bf16 else 4)[0] is out):
             _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
+        if writes and out.numel() and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+            _refuse(name, "out shares memory with an input")
     if not q.is_cuda:
         _refuse(name, "there is no CPU form")
     return (B, Lq, Lk, H, G, D, bf16), scale, lens, q_lens, mask, maskb
@@ -1979,7 +1981,8 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
     reads key head h // (H // G).  fp32 or bf16 (all alike), D a multiple of 8 up to 128, scale 1 / sqrt(D) unless given.
 
     lens int64 [B]: keys at or past it are not seen; mask bool [B or 1, Lk]: True = not seen.  What stands in rows that are not
-    seen is never used.  q_lens int64 [B]: queries at or past it, like queries that see no key, give zeros and lse = -inf.
+    seen is never used; what is seen is finite.  q_lens int64 [B]: queries at or past it, like queries that see no key, give zeros
+    and lse = -inf.
     lse (optional, fp32 [B, H, Lq]) receives the logarithm of the softmax's denominator, which cross_attention_bwd needs.
     out (optional): the result's tensor, which shares no memory with the inputs."""
     name = "cross_attention"
@@ -2080,6 +2083,8 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
         _refuse(name, f"gain {gain}: a finite number expected")
     if out is not None and not _rows_ok(_like(name, out, "out", shape, x.dtype, device).shape, out.stride()):
         _refuse(name, "out must have contiguous features and distinct rows")
+    if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel():
+        _refuse(name, "out shares memory with x in another layout")
     if not x.is_cuda:
         _refuse(name, "there is no CPU form")
     if x.stride(3) != 1:
@@ -2145,6 +2150,8 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
     groupnorm_act_bwd.  out (optional) may be x."""
     name = "groupnorm_act"
+    if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel():
+        _refuse(name, "out shares memory with x in another layout")
     sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, out, "out")
     B, L, C, _ = sizes
     if out is None:
@@ -2152,6 +2159,8 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     elif not _rows_ok(out.shape, out.stride()):
         _refuse(name, "out must have contiguous channels and distinct rows")
     if out.numel() == 0:
+        if stats is not None:
+            stats.zero_()
         return out
     (x, xb, xl), (_, ob, ol) = _gn_rows(x, B, L, C), _gn_rows(out, B, L, C)
     n = _gn_ws(*sizes, bf16, 0)

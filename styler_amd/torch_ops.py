@@ -538,3 +538,104 @@ OPS = ("conv_gemm", "conv_gemm_bwd", "attention", "attention_bwd", "add_layernor
        "length_regulate_bwd", "stft_mel", "groupnorm_relu", "groupnorm_relu_bwd", "batchnorm_act", "batchnorm_act_bwd", "lstm_bidir",
        "lstm_bidir_bwd", "linear_ln", "masked_err_mean", "masked_err_mean_bwd", "nll3", "nll3_bwd", "dropout", "embed_pos",
        "embed_pos_bwd", "mel_calibrate", "mel_calibrate_bwd", "aug_classifier_tail", "aug_classifier_tail_bwd", "clip_adam_step")
+
+
+# =====================================================================================================================================
+# Operators of a decoder block that reads an encoder's states (ops.cross_attention, ops.rotary, ops.groupnorm_act), forward + backward
+# =====================================================================================================================================
+#     cross_attention / _bwd       attention of queries over another sequence's keys and values -> (out, lse)
+#     rotary                       rotary positions (its own backward, the opposite turn)
+#     groupnorm_act / _bwd         group norm over channels-last rows + activation -> (y, stats)
+#
+# lse and stats are what the backward operators take; they carry no gradient of their own (using one raises).
+def _no_grad_of(name, g):
+    if g is not None:
+        raise ops.StylerHipError(f"styler::{name}: its second output has no gradient")
+
+
+# ---- cross_attention -------------------------------------------------------------------------------------------------------------------
+def _xattn_fwd(q, k, v, lens=None, q_lens=None, mask=None, scale=None):
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
+    return ops.cross_attention(q, k, v, lens, q_lens=q_lens, mask=mask, scale=scale, lse=lse), lse
+
+
+_pair("cross_attention", "(Tensor q, Tensor k, Tensor v, Tensor? lens=None, Tensor? q_lens=None, Tensor? mask=None, float? scale=None) -> "
+      "(Tensor, Tensor)", _xattn_fwd,
+      lambda q, k, v, lens=None, q_lens=None, mask=None, scale=None: (
+          q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)))
+_pair("cross_attention_bwd", "(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, Tensor? lens, Tensor? q_lens, Tensor? mask, "
+      "float? scale) -> (Tensor, Tensor, Tensor)",
+      lambda q, k, v, out, dout, lse, lens, q_lens, mask, scale: ops.cross_attention_bwd(q, k, v, out, dout, lse, lens, q_lens=q_lens,
+                                                                                          mask=mask, scale=scale),
+      lambda q, k, v, out, dout, lse, lens, q_lens, mask, scale: (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)))
+
+
+def _xattn_setup(ctx, inputs, output):
+    q, k, v, lens, q_lens, mask, ctx.scale = inputs
+    ctx.save_for_backward(q, k, v, output[0], output[1], lens, q_lens, mask)
+    ctx.set_materialize_grads(False)
+
+
+def _xattn_backward(ctx, dout, dlse):
+    _no_grad_of("cross_attention", dlse)
+    if dout is None:
+        return (None,) * 7
+    q, k, v, out, lse, lens, q_lens, mask = ctx.saved_tensors
+    return (*torch.ops.styler.cross_attention_bwd(q, k, v, out, dout, lse, lens, q_lens, mask, ctx.scale), None, None, None, None)
+
+
+register_autograd("styler::cross_attention", _xattn_backward, setup_context=_xattn_setup)
+
+# ---- rotary ------------------------------------------------------------------------------------------------------------------------------
+_pair("rotary", "(Tensor x, Tensor freqs, Tensor? pos=None, bool interleaved=False, float gain=1.0, bool inverse=False) -> Tensor",
+      lambda x, freqs, pos=None, interleaved=False, gain=1.0, inverse=False: ops.rotary(x, freqs, pos, interleaved=interleaved, gain=gain,
+                                                                                         inverse=inverse),
+      lambda x, freqs, pos=None, interleaved=False, gain=1.0, inverse=False: x.new_empty(x.shape))
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, freqs, pos, ctx.interleaved, ctx.gain, ctx.inverse = inputs
+    ctx.save_for_backward(freqs, pos)
+
+
+def _rotary_backward(ctx, dy):
+    freqs, pos = ctx.saved_tensors
+    return torch.ops.styler.rotary(dy, freqs, pos, ctx.interleaved, ctx.gain, not ctx.inverse), None, None, None, None, None
+
+
+register_autograd("styler::rotary", _rotary_backward, setup_context=_rotary_setup)
+
+
+# ---- groupnorm_act -----------------------------------------------------------------------------------------------------------------------
+def _gna_fwd(x, gamma, beta, groups, act, eps=1e-5, lens=None):
+    stats = torch.empty(x.shape[0], groups, 2, device=x.device, dtype=torch.float32)
+    return ops.groupnorm_act(x, gamma, beta, groups, act, eps=eps, lens=lens, stats=stats), stats
+
+
+_pair("groupnorm_act", "(Tensor x, Tensor gamma, Tensor beta, int groups, int act, float eps=1e-5, Tensor? lens=None) -> (Tensor, Tensor)",
+      _gna_fwd,
+      lambda x, gamma, beta, groups, act, eps=1e-5, lens=None: (
+          x.new_empty(x.shape), x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)))
+_pair("groupnorm_act_bwd", "(Tensor x, Tensor dy, Tensor gamma, Tensor beta, Tensor stats, int groups, int act, Tensor? lens) -> "
+      "(Tensor, Tensor, Tensor)",
+      lambda x, dy, gamma, beta, stats, groups, act, lens: ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, groups, act, lens=lens),
+      lambda x, dy, gamma, beta, stats, groups, act, lens: (x.new_empty(x.shape), torch.empty_like(gamma), torch.empty_like(beta)))
+
+
+def _gna_setup(ctx, inputs, output):
+    x, gamma, beta, ctx.groups, ctx.act, _, lens = inputs
+    ctx.save_for_backward(x, gamma, beta, output[1], lens)
+    ctx.set_materialize_grads(False)
+
+
+def _gna_backward(ctx, dy, dstats):
+    _no_grad_of("groupnorm_act", dstats)
+    if dy is None:
+        return (None,) * 7
+    x, gamma, beta, stats, lens = ctx.saved_tensors
+    return (*torch.ops.styler.groupnorm_act_bwd(x, dy, gamma, beta, stats, ctx.groups, ctx.act, lens), None, None, None, None)
+
+
+register_autograd("styler::groupnorm_act", _gna_backward, setup_context=_gna_setup)
+
+BLOCK_OPS = ("cross_attention", "cross_attention_bwd", "rotary", "groupnorm_act", "groupnorm_act_bwd")

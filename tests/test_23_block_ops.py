@@ -126,6 +126,30 @@ def test_cross_attention_against_definition(dev, B, Lq, Lk, H, G, D, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D,lens,q_lens", [
+    (3, 530, 500, 2, 1, 32, [500, 3, 260], [530, 530, 100]),              # long ragged items: the most work first
+    (4, 600, 450, 1, 1, 128, [17, 0, 450, 450], [600, 1, 0, 599]),
+    (5, 520, 510, 2, 2, 80, [510, 64, 65, 1, 509], [1, 520, 519, 520, 0]),
+    (3, 1, 5000, 4, 1, 64, [5000, 3, 0], None),                           # shares of which some see nothing
+    (3, 2, 4097, 16, 4, 128, [4097, 4096, 65], [2, 1, 2]),
+    (2, 9, 1500, 8, 1, 32, [1500, 700], None),                            # 72 rows of one key head
+    (20, 2, 33, 4, 4, 64, None, None),                                    # many items of few rows
+    (300, 130, 5, 2, 1, 8, None, None),                                   # more blocks than the chip holds at once
+    (520, 70, 90, 1, 1, 64, [90 - i % 91 for i in range(520)], [i % 71 for i in range(520)]),
+    (1, 2500, 33, 2, 1, 64, [32], [2499]),                                # the key gradient's rows shared out, few keys
+])
+def test_cross_attention_sizes_and_lengths(dev, B, Lq, Lk, H, G, D, lens, q_lens, dtype):
+    t = lambda x: None if x is None else torch.tensor(x)
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, dtype, seed=21)
+    got = check_attention(q, k, v, do, t(lens), t(q_lens))
+    for b, n in enumerate(lens or []):
+        assert not got[2][b, n:].any() and not got[3][b, n:].any()
+    for b, n in enumerate(q_lens or []):
+        assert not got[0][b, n:].any() and not got[1][b, n:].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("Lq", [1, 45])
 def test_cross_attention_masks(dev, dtype, Lq):
     """Lengths of zero, one, all and beyond; whole rows and whole tiles dropped by the mask; queries past their length.  What stands
@@ -618,3 +642,354 @@ def test_groupnorm_act_of_single_values(dev, dtype):
     assert torch.equal(y, beta.to(dtype).expand(8, 1, 128))
     dx, dgamma, dbeta = ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, 128, ops.ACT_NONE)
     assert not dx.any() and not dgamma.any()
+
+
+# ------------------------------------------------------------------------------------------------------------ together
+def test_block_operators_have_schemas_and_fake_kernels():
+    import styler_amd.torch_ops as T
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    assert all(hasattr(torch.ops.styler, n) for n in T.BLOCK_OPS)
+    with FakeTensorMode():
+        q, k = torch.empty(2, 7, 8, 64, dtype=torch.bfloat16), torch.empty(2, 9, 2, 64, dtype=torch.bfloat16)
+        out, lse = torch.ops.styler.cross_attention(q, k, k)
+        assert out.shape == q.shape and out.dtype == q.dtype and tuple(lse.shape) == (2, 8, 7) and lse.dtype == torch.float32
+        g = torch.ops.styler.cross_attention_bwd(q, k, k, out, out, lse, None, None, None, None)
+        assert [tuple(t.shape) for t in g] == [(2, 7, 8, 64), (2, 9, 2, 64), (2, 9, 2, 64)]
+        assert torch.ops.styler.rotary(q, torch.empty(32, dtype=torch.float64)).shape == q.shape
+        x, w = torch.empty(2, 5, 48, dtype=torch.bfloat16), torch.empty(48)
+        y, stats = torch.ops.styler.groupnorm_act(x, w, w, 3, 6)
+        assert y.shape == x.shape and tuple(stats.shape) == (2, 3, 2)
+        dx, dg, db = torch.ops.styler.groupnorm_act_bwd(x, y, w, w, stats, 3, 6, None)
+        assert dx.shape == x.shape and dg.shape == w.shape and dg.dtype == torch.float32
+
+
+def block_case(dev, dtype, seed=0):
+    """A decoder block over an encoder's states: norm -> query projection -> rotary queries and keys -> attention."""
+    g = torch.Generator().manual_seed(seed)
+    B, Lq, Lk, C, H, G, D = 3, 70, 41, 256, 4, 2, 64
+    r = lambda *s: torch.randn(*s, generator=g)
+    t = dict(x=r(B, Lq, C).to(dtype), enc=r(B, Lk, 2, G, D).to(dtype), w=(r(H * D, C) / 16), gamma=1 + 0.1 * r(C), beta=0.1 * r(C),
+             dout=r(B, Lq, H, D).to(dtype))
+    return {k: v.to(dev) for k, v in t.items()}, torch.tensor([70, 1, 33], device=dev), torch.tensor([41, 20, 7], device=dev)
+
+
+def block_forward(ops_, x, enc, w, gamma, beta, q_lens, lens, freqs, native):
+    B, Lq, C = x.shape
+    H, G, D = 4, 2, 64
+    pos_q = (torch.arange(Lq, device=x.device) / 1.7).float()
+    if native:
+        y, _ = torch.ops.styler.groupnorm_act(x, gamma, beta, 16, 6, 1e-5, q_lens)
+        q = torch.ops.styler.conv_gemm(y.float(), w, None, 0, 0).to(x.dtype).view(B, Lq, H, D)
+        q = torch.ops.styler.rotary(q, freqs, pos_q)
+        k = torch.ops.styler.rotary(enc[:, :, 0], freqs, None)
+        return torch.ops.styler.cross_attention(q, k, enc[:, :, 1], lens, q_lens)[0]
+    on = (torch.arange(Lq, device=x.device)[None] < q_lens[:, None])[..., None]
+    out = torch.zeros(B, Lq, H, D, dtype=torch.float64, device=x.device)
+    turn = lambda t, p: torch.cat([t[..., :32] * p.cos()[:, None] - t[..., 32:] * p.sin()[:, None],
+                                   t[..., 32:] * p.cos()[:, None] + t[..., :32] * p.sin()[:, None]], -1)
+    for b in range(B):
+        n, m = int(q_lens[b]), int(lens[b])
+        xb = x[b, :n].view(n, 16, C // 16)
+        z = ((xb - xb.mean((0, 2), keepdim=True)) * (xb.var((0, 2), correction=0, keepdim=True) + 1e-5).rsqrt()).reshape(n, C) * gamma + beta
+        q = turn((z * torch.sigmoid(z) @ w.T).view(n, H, D), pos_q[:n, None].double() * freqs)
+        k = turn(enc[b, :m, 0], torch.arange(m, device=x.device)[:, None].double() * freqs)
+        for h in range(H):
+            out[b, :n, h] = torch.softmax(q[:, h] @ k[:, h // 2].T / 8, -1) @ enc[b, :m, 1, h // 2]
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 2e-5), (torch.bfloat16, 4e-2)])
+def test_decoder_block_over_encoder_states(dev, dtype, tol):
+    """The operators one after the other through the dispatcher, gradients by the registered formulas, against 64-bit math.  fp32: a
+    chain of some thirty 32-bit roundings over sums of up to 256 terms, relative to the largest value; bf16: five roundings to bf16
+    on the way (2^-8 each, twice that through the softmax's logits)."""
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    t, q_lens, lens = block_case(dev, dtype)
+    freqs = ops.rotary_freqs(64, dev)
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items() if k != "dout"}
+    out = block_forward(ops, *(leaves[k] for k in ("x", "enc", "w", "gamma", "beta")), q_lens, lens, freqs, True)
+    grads = torch.autograd.grad(out, list(leaves.values()), t["dout"])
+    ref_leaves = {k: v.double().clone().requires_grad_() for k, v in t.items() if k != "dout"}
+    ref = block_forward(None, *(ref_leaves[k] for k in ("x", "enc", "w", "gamma", "beta")), q_lens, lens, freqs, False)
+    on = (torch.arange(70, device=dev)[None] < q_lens[:, None])[..., None, None]
+    ref_grads = torch.autograd.grad(ref, list(ref_leaves.values()), torch.where(on, t["dout"].double(), 0.0))
+    assert float((out.double() - ref).detach().abs().max()) <= tol * float(ref.detach().abs().max())
+    for (k, _), a, b in zip(leaves.items(), grads, ref_grads):
+        assert float((a.double() - b).abs().max()) <= tol * float(b.abs().max()), k
+
+
+@gpu
+def test_block_operators_opcheck(dev):
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    q, k, v, do = attention_case(dev, 2, 7, 9, 4, 2, 32, torch.float32)
+    lens = torch.tensor([9, 4], device=dev)
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor")
+    torch.library.opcheck(torch.ops.styler.cross_attention, (q.requires_grad_(), k.requires_grad_(), v.requires_grad_(), lens), test_utils=tests)
+    torch.library.opcheck(torch.ops.styler.rotary, (torch.randn(2, 5, 3, 64, device=dev, requires_grad=True), ops.rotary_freqs(32, dev)), test_utils=tests)
+    x, dy, gamma, beta = gn_case(dev, 2, 9, 32, torch.float32)
+    torch.library.opcheck(torch.ops.styler.groupnorm_act, (x.requires_grad_(), gamma.requires_grad_(), beta.requires_grad_(), 4, 6), test_utils=tests)
+
+
+@gpu
+def test_block_operators_refuse_gradients_they_do_not_have(dev):
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    q, k, v, do = attention_case(dev, 1, 7, 9, 2, 2, 32, torch.float32)
+    out, lse = torch.ops.styler.cross_attention(q.requires_grad_(), k, v)
+    with pytest.raises(ops.StylerHipError, match="no gradient"):
+        (out.sum() + lse.sum()).backward()
+    x, dy, gamma, beta = gn_case(dev, 2, 9, 32, torch.float32)
+    y, stats = torch.ops.styler.groupnorm_act(x.requires_grad_(), gamma, beta, 4, 6)
+    with pytest.raises(ops.StylerHipError, match="no gradient"):
+        stats.sum().backward()
+
+
+@gpu
+def test_block_operators_gradients_of_broadcast_inputs(dev):
+    """Keys that a batch shares, a channel-expanded gradient (a sum's) and an expanded x: autograd sums what broadcasting spread."""
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    q, k, v, _ = attention_case(dev, 3, 20, 50, 4, 2, 32, torch.float32)
+    k1, v1 = (t[:1].clone().requires_grad_() for t in (k, v))
+    torch.ops.styler.cross_attention(q, k1.expand(3, -1, -1, -1), v1.expand(3, -1, -1, -1))[0].sum().backward()
+    k2, v2 = (t[:1].expand(3, -1, -1, -1).contiguous() for t in (k, v))
+    lse = torch.empty(3, 4, 20, device=dev)
+    out = ops.cross_attention(q, k2, v2, lse=lse)
+    _, dk, dv = ops.cross_attention_bwd(q, k2, v2, out, torch.ones_like(out), lse)
+    for got, ref in ((k1.grad, dk), (v1.grad, dv)):
+        assert float((got - ref.sum(0, keepdim=True)).abs().max()) <= 8 * half_step(torch.float32) * float(ref.abs().sum(0).max())
+    x, _, gamma, beta = gn_case(dev, 1, 30, 32, torch.float32)
+    x1 = x.clone().requires_grad_()
+    torch.ops.styler.groupnorm_act(x1.expand(4, -1, -1), gamma, beta, 4, 6)[0][:, 3:].sum().backward()
+    x2 = x.clone().requires_grad_()
+    (4 * torch.ops.styler.groupnorm_act(x2, gamma, beta, 4, 6)[0][:, 3:]).sum().backward()
+    assert float((x1.grad - x2.grad).abs().max()) <= 64 * half_step(torch.float32) * float(x2.grad.abs().max())
+    f = ops.rotary_freqs(32, dev)
+    x1 = torch.randn(1, 9, 1, 32, device=dev, requires_grad=True)
+    torch.ops.styler.rotary(x1.expand(2, 9, 3, 32), f).sum().backward()
+    one = ops.rotary(torch.ones(1, 9, 1, 32, device=dev), f, inverse=True)
+    assert float((x1.grad - 6 * one).abs().max()) <= 6 * 8 * half_step(torch.float32) * 2
+
+
+@gpu
+def test_groupnorm_act_gradient_by_differences(dev):
+    """Central differences of sum(y dy) in fp32 on a few directions.  With a step of h the quotient is off by the third derivative's
+    h^2 / 6 and by y's rounding over 2 h: 600 values of about 2^-24 each add up to less than 1e-5, so h = 1e-2 leaves 1e-3; both are far below
+    the 2e-2 allowed of derivatives around 1."""
+    from styler_amd import ops
+    for act in (ops.ACT_NONE, ops.ACT_SILU, ops.ACT_GELU):
+        x, dy, gamma, beta = gn_case(dev, 2, 10, 30, torch.float32, offset=0.5)
+        lens = torch.tensor([10, 6], device=dev)
+        stats = torch.empty(2, 3, 2, device=dev)
+        f = lambda x, g, b: float((ops.groupnorm_act(x, g, b, 3, act, lens=lens, stats=stats).double() * dy.double()).sum())
+        f(x, gamma, beta)
+        grads = ops.groupnorm_act_bwd(x, dy, gamma, beta, stats.clone(), 3, act, lens=lens)
+        gen = torch.Generator().manual_seed(5)
+        for i in range(3):
+            t = [x, gamma, beta]
+            d = torch.randn(t[i].shape, generator=gen).to(dev)
+            d /= d.norm()
+            up, down = list(t), list(t)
+            up[i], down[i] = t[i] + 1e-2 * d, t[i] - 1e-2 * d
+            assert abs((f(*up) - f(*down)) / 2e-2 - float((grads[i].double() * d).sum())) < 2e-2, (act, i)
+
+
+@gpu
+def test_block_operators_in_a_graph(dev):
+    """Captured once, replayed with new inputs in the same buffers and eager calls of the same operators in between; two graphs that
+    share a pool are replayed in turn.  Every replay equals the eager result."""
+    from styler_amd import ops
+    freqs = ops.rotary_freqs(64, dev)
+    lens = torch.tensor([300, 120], device=dev)
+
+    def make(Lq, dtype):
+        q, k, v, do = attention_case(dev, 2, Lq, 300, 4, 2, 64, dtype, seed=Lq)
+        x, dy, gamma, beta = gn_case(dev, 2, 900 + Lq, 64, dtype, seed=Lq)
+        bufs = [q, k, v, do, x, dy]
+
+        def step():
+            qr, kr = ops.rotary(q, freqs), ops.rotary(k, freqs)
+            lse = torch.empty(2, 4, Lq, device=dev)
+            out = ops.cross_attention(qr, kr, v, lens, lse=lse)
+            g = ops.cross_attention_bwd(qr, kr, v, out, do, lse, lens)
+            stats = torch.empty(2, 4, 2, device=dev)
+            y = ops.groupnorm_act(x, gamma, beta, 4, stats=stats)
+            return [out, *g, ops.rotary(g[0], freqs, inverse=True), y, *ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, 4)]
+        return bufs, step
+
+    sets = [make(1, torch.bfloat16), make(70, torch.float32), make(150, torch.bfloat16)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _, step in sets:
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for bufs, step in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            got = step()
+        graphs.append((g, got, bufs, step))
+    gen = torch.Generator().manual_seed(99)
+    for turn in range(4):
+        for g, got, bufs, step in graphs:
+            for t in bufs:
+                t.copy_(torch.randn(t.shape, generator=gen).to(t.dtype))
+            want = [t.clone() for t in step()]
+            g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), turn
+
+
+@gpu
+def test_block_operators_on_another_stream(dev):
+    """Two streams at once, each with its own workspaces: the results of either are those of one alone."""
+    from styler_amd import ops
+    cases = [attention_case(dev, 2, Lq, 4000, 8, 2, 64, dt, seed=s) for s, (Lq, dt) in enumerate([(1, torch.bfloat16), (90, torch.float32)])]
+
+    def step(q, k, v, do):
+        lse = torch.empty(2, 8, q.shape[1], device=dev)
+        out = ops.cross_attention(q, k, v, lse=lse)
+        return [out, *ops.cross_attention_bwd(q, k, v, out, do, lse)]
+
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(step(*c))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2]))
+
+
+@gpu
+def test_block_operators_past_32_bit_offsets(dev):
+    """Tensors of more than 2^31 elements: what stands at their end is what is read and written."""
+    from styler_amd import ops
+    Lk = (1 << 21) + 77
+    k, v = (torch.zeros(1, Lk, 8, 128, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    assert k.numel() > 1 << 31
+    q, kt, vt, _ = attention_case(dev, 1, 2, 100, 16, 8, 128, torch.bfloat16, seed=2)
+    k[:, -100:], v[:, -100:] = kt, vt
+    mask = torch.ones(1, Lk, dtype=torch.bool, device=dev)
+    mask[:, -100:] = False
+    a, b = ops.cross_attention(q, k, v, mask=mask), ops.cross_attention(q, kt, vt)
+    assert float((a.float() - b.float()).abs().max()) <= 2 * half_step(torch.bfloat16) * float(b.float().abs().max())
+    x = k.view(1, Lk, 8, 128)
+    f = ops.rotary_freqs(128, dev)
+    pos = torch.arange(Lk, device=dev)
+    y = ops.rotary(x, f, pos, out=v)
+    assert torch.equal(y[:, -100:], ops.rotary(kt, f, pos[-100:])) and not y[:, :-100].any()
+    y.zero_()
+    rows = x.view(1, Lk, 1024)
+    w = torch.ones(1024, device=dev)
+    ops.groupnorm_act(rows, w, 0 * w, 8, ops.ACT_NONE, out=y.view(1, Lk, 1024))
+    t = kt.double().view(100, 8, 128)
+    mean = t.sum((0, 2)) / (Lk * 128)
+    var = (t ** 2).sum((0, 2)) / (Lk * 128) - mean ** 2
+    ref = ((t - mean[:, None]) * (var[:, None] + 1e-5).rsqrt()).view(1, 100, 1024)
+    assert float((y.view(1, Lk, 1024)[:, -100:].double() - ref).abs().max()) <= 2 * half_step(torch.bfloat16) * float(ref.abs().max())
+
+
+def test_block_operators_refuse_shared_outputs():
+    """An output in an input's place would be read after it was written; only the elementwise operators work in place, in one layout."""
+    from styler_amd import ops
+    q, k = torch.zeros(2, 4, 4, 32), torch.zeros(2, 4, 4, 32)
+    for out in (q, k):
+        with pytest.raises(ops.StylerHipError, match="shares memory"):
+            ops.cross_attention(q, k, k, out=out)
+    with pytest.raises(ops.StylerHipError, match="shares memory"):
+        ops.rotary(q, ops.rotary_freqs(32, "cpu"), out=q.transpose(1, 2))
+    with pytest.raises(ops.StylerHipError, match="no CPU form"):
+        ops.rotary(q, ops.rotary_freqs(32, "cpu"), out=q)
+    x, w = torch.zeros(4, 4, 32), torch.ones(32)
+    with pytest.raises(ops.StylerHipError, match="shares memory"):
+        ops.groupnorm_act(x, w, w, 4, out=x.transpose(0, 1))
+    with pytest.raises(ops.StylerHipError, match="no CPU form"):
+        ops.groupnorm_act(x, w, w, 4, out=x)
+
+
+@gpu
+def test_groupnorm_act_of_many_items(dev):
+    """More items than a grid's third axis holds, in both forms; items are alike, so each must equal a small batch's."""
+    from styler_amd import ops
+    for L, C, G in ((1, 16, 4), (2, 2056, 1), (130, 64, 64)):
+        B, n = 70001, 7
+        x, dy, gamma, beta = gn_case(dev, n, L, C, torch.bfloat16, seed=6)
+        at = torch.arange(B, device=dev) % n
+        xs, dys = x[at], dy[at]
+        lens = torch.tensor([L, L, 0, 1, L, (L + 1) // 2, L], device=dev)
+        s1, s2 = torch.empty(n, G, 2, device=dev), torch.empty(B, G, 2, device=dev)
+        y1, y2 = ops.groupnorm_act(x, gamma, beta, G, lens=lens, stats=s1), ops.groupnorm_act(xs, gamma, beta, G, lens=lens[at], stats=s2)
+        assert float((y1[at].float() - y2.float()).abs().max()) <= 4 * half_step(torch.bfloat16) * float(y1.float().abs().max())
+        assert float((s1[at] - s2).abs().max()) <= 1e-5 * float(s1.abs().max())
+        g1, g2 = ops.groupnorm_act_bwd(x, dy, gamma, beta, s1, G, lens=lens), ops.groupnorm_act_bwd(xs, dys, gamma, beta, s2, G, lens=lens[at])
+        assert float((g1[0][at].float() - g2[0].float()).abs().max()) <= 4 * half_step(torch.bfloat16) * float(g1[0].float().abs().max())
+        # the parameters' gradients add B / n of each item, in 32 bits one after the other: B steps of half a unit at most
+        w = torch.bincount(at, minlength=n).double()
+        each = [ops.groupnorm_act_bwd(x[i:i + 1], dy[i:i + 1], gamma, beta, s1[i:i + 1], G, lens=lens[i:i + 1])[1:] for i in range(n)]
+        for j, got in enumerate(g2[1:]):
+            ref = sum(w[i] * e[j].double() for i, e in enumerate(each))
+            size = sum(w[i] * e[j].double().abs() for i, e in enumerate(each))
+            assert float(((got.double() - ref).abs() / (size + 1e-3)).max()) <= B * half_step(torch.float32) * 0.5
+
+
+# ------------------------------------------------------------------------------------------------------------ the C entries
+def test_block_entry_points_refuse_before_any_launch():
+    """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
+    from styler_amd._lib import GN, ROTARY, XATTN, lib
+    EINVAL, EALIGN = -1, -2
+    P = 4096
+
+    def xattn(bwd=False, ws=P, nbytes=1 << 40, **kw):
+        f = dict(q=P, k=P, v=P, out=P, dout=P, dq=P, dk=P, dv=P, lse=P, len=0, q_len=0, mask=0, qb=512, ql=256, qh=64, kb=512, kl=128, kh=64,
+                 vb=512, vl=128, vh=64, ob=512, ol=256, oh=64, gb=512, gl=256, gh=64, maskb=0, B=2, Lq=2, Lk=4, H=4, G=2, D=64, bf16=1,
+                 scale=0.125)
+        f.update(kw)
+        fn = lib.styler_cross_attention_bwd if bwd else lib.styler_cross_attention
+        return fn(XATTN.pack(*f.values()), ws, nbytes, None)
+
+    for kw in (dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(B=0), dict(Lq=0), dict(Lk=-1), dict(H=3), dict(G=0), dict(D=60), dict(D=136),
+               dict(scale=0.0), dict(scale=math.nan), dict(scale=-1.0), dict(ql=1 << 23), dict(kl=1 << 23), dict(B=1 << 23)):
+        assert xattn(**kw) == EINVAL, kw
+    for kw in (dict(q=P + 2), dict(ql=250), dict(kh=4), dict(vb=-64), dict(out=P + 8)):
+        assert xattn(**kw) == EALIGN, kw
+    for kw in (dict(dout=0), dict(dq=0), dict(dk=0), dict(dv=0), dict(lse=0), dict(ws=0), dict(nbytes=8), dict(ws=P + 4)):
+        assert xattn(bwd=True, **kw) == EINVAL, kw
+    assert xattn(bwd=True, gl=12) == EALIGN
+    assert xattn(Lk=100000, kb=0, vb=0, ws=0) == EINVAL                      # shares of a long axis need their workspace
+    assert lib.styler_cross_attention(None, None, 0, None) == EINVAL
+
+    def rotary(**kw):
+        f = dict(x=P, y=P, freqs=P, pos=0, xb=64, xl=64, xh=64, yb=64, yl=64, yh=64, posb=0, B=1, L=1, H=1, D=64, rot=64, pos_kind=0,
+                 interleaved=0, inverse=0, bf16=1, gain=1.0)
+        f.update(kw)
+        return lib.styler_rotary(ROTARY.pack(*f.values()), None)
+
+    for kw in (dict(x=0), dict(y=0), dict(freqs=0), dict(B=0), dict(H=0), dict(rot=0), dict(rot=3), dict(rot=66), dict(D=16384, rot=2),
+               dict(pos_kind=3), dict(pos_kind=1), dict(B=1 << 20, L=1 << 12)):
+        assert rotary(**kw) == EINVAL, kw
+    assert rotary(x=P + 1) == EALIGN
+    assert lib.styler_rotary(None, None) == EINVAL
+
+    def gn(bwd=False, ws=P, nbytes=1 << 40, **kw):
+        f = dict(x=P, dy=P, out=P, gamma=P, beta=P, stats=P, dgamma=P, dbeta=P, len=0, xb=640, xl=64, db=640, dl=64, ob=640, ol=64, B=2, L=10,
+                 C=64, G=4, act=6, bf16=0, eps=1e-5)
+        f.update(kw)
+        return (lib.styler_groupnorm_act_bwd if bwd else lib.styler_groupnorm_act)(GN.pack(*f.values()), ws, nbytes, None)
+
+    for kw in (dict(x=0), dict(out=0), dict(gamma=0), dict(beta=0), dict(B=0), dict(L=0), dict(C=0), dict(G=0), dict(G=3), dict(act=2),
+               dict(act=99), dict(eps=-1.0), dict(eps=math.nan), dict(L=1 << 30 | 1)):
+        assert gn(**kw) == EINVAL, kw
+    for kw in (dict(dy=0), dict(stats=0), dict(dgamma=0), dict(dbeta=0), dict(ws=0), dict(nbytes=16)):
+        assert gn(bwd=True, **kw) == EINVAL, kw
+    assert gn(x=P + 2) == EALIGN
+    assert gn(L=1 << 20, xb=0, ob=0, ws=0) == EINVAL
+    assert lib.styler_groupnorm_act(None, None, 0, None) == EINVAL
