@@ -905,7 +905,7 @@ int styler_adam_step(float* p, const float* g, float* m, float* v, int64_t n, co
  * elements, multiples of 16 bytes, features contiguous, 16-byte aligned bases; out / dq [B, Lq, H, D] and dk / dv
  * [B, Lk, G, D]: `out` by its strides, the gradients contiguous.  The backward takes the forward's out and lse; unseen keys and
  * queries past their length get zero gradients.  No atomics: both directions are deterministic.  The workspace
- * (styler_cross_attention_workspace_bytes, 16-byte aligned) belongs to the call until it has run on its stream. */
+ * (styler_cross_attention_workspace_bytes, masked: with a mask; 16-byte aligned) belongs to the call until it has run on its stream. */
 typedef struct {
   const void *q, *k, *v;
   void* out;
@@ -919,7 +919,7 @@ typedef struct {
   int32_t B, Lq, Lk, H, G, D, bf16;
   float scale;
 } styler_xattn_t;
-int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int bwd);
+int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int masked, int bwd);
 int styler_cross_attention(const styler_xattn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
 int styler_cross_attention_bwd(const styler_xattn_t* host_args, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -147,7 +147,7 @@ _SIGS = {
     "styler_ds_rows": [P, P, I, I, I, I, I, I, I, P],
     "styler_ds_crelu_add": [P, P, P, I64, P],
     "styler_l2_normalize_rows": [P, P, I, I, P],
-    "styler_cross_attention_workspace_bytes": [I, I, I, I, I, I, I, I],
+    "styler_cross_attention_workspace_bytes": [I, I, I, I, I, I, I, I, I],
     "styler_cross_attention": [P, P, I64, P],
     "styler_cross_attention_bwd": [P, P, I64, P],
     "styler_rotary": [P, P],

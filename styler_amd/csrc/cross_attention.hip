@@ -32,10 +32,11 @@ struct XArgs {
   const void *q, *k, *v, *o, *dout;                    // dout / o: backward
   void *out, *dq, *dk, *dv;
   float* lse;                                          // [B, H, Lq]
-  float* delta;                                        // [B, H, Lq] (backward workspace)
+  float *delta, *lse2;                                 // [B, H, Lq] (backward workspace); lse2: lse / ln 2, +inf for -inf
   float* part;                                         // partial results of a split launch
   const int64_t *len, *qlen;
   const uint8_t* mask;
+  const int* order;                                    // [B, Lk] or null: the keys in the order of xattn_order_kernel
   int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh, gb, gl, gh;   // strides (elements): item, row, head; g: dout
   const void *t0, *t1;                                 // what tiles are made of: k and v, or (dk, dv) q and dout
   int64_t t0b, t0l, t0h, t0p, t1b, t1l, t1h, t1p;      // item, row, head, plane
@@ -61,8 +62,8 @@ __device__ __forceinline__ int xcd_block(int total, int chunk) {
 
 // Ragged batches are walked from the item with the most work (keys times queries) to the least, so that the last blocks are the
 // shortest: item number `r` in that order.  Every wave finds it by itself -- lane i counts the items that come before item i,
-// 3 B instructions.  Only for up to 16 items whose blocks' walks are
-// long against that (8 x 1203 x 1001 fp32: 620 -> 570 us; 48 x 1000 x 133, sorted all the same: 74 -> 82).
+// 3 B instructions.  Only for up to 16 items whose blocks' walks are long against that (8 x 1203 x 1001 fp32: 620 -> 570 us;
+// 48 x 1000 x 133, sorted all the same: 74 -> 82).
 __device__ __forceinline__ int item_at(const XArgs& a, int r, int lane) {
   if (!a.sort) return r;
   const int i = lane < a.B ? lane : 0;
@@ -97,19 +98,31 @@ template <int RB> struct DmaLane {
   static constexpr int RPI = 1024 / RB, VAR = RPI * 4 >= 16 ? 1 : 16 / (RPI * 4);
   uint32_t off[VAR];
   int row;
-  __device__ __forceinline__ void init(int64_t ldbytes, int dbytes, int wave, int lane) {
+  // pick: rows are found by their numbers (RowNumbers), off holds the piece alone
+  __device__ __forceinline__ void init(int64_t ldbytes, int dbytes, int wave, int lane, bool pick = false) {
     row = wave * RPI + lane / (RB / 16);
 #pragma unroll
     for (int i = 0; i < VAR; ++i) {
       const uint32_t c = ((lane % (RB / 16)) ^ Swz<RB>::of(i * 4 * RPI + row)) * 16;
-      off[i] = c < (uint32_t)dbytes ? (uint32_t)(row * (int)ldbytes) + c : OOB;
+      off[i] = c < (uint32_t)dbytes ? (pick ? 0u : (uint32_t)(row * (int)ldbytes)) + c : OOB;
     }
   }
 };
-template <int RB, int ROWS, int NW>
+template <int RB, int ROWS> constexpr int dma_count() { return ROWS >= 4 * (1024 / RB) ? ROWS * RB / 4096 : 1; }      // instructions per wave
+// The numbers of the rows that a lane's instructions fill, where a tile's rows are any rows of the tensor; fetched a tile ahead.
+template <int N> struct RowNumbers { uint32_t n[N]; };
+template <int RB, int ROWS>
+__device__ __forceinline__ void order_fetch(RowNumbers<dma_count<RB, ROWS>()>& rn, const int* order, int k0, int L, const DmaLane<RB>& dl) {
+#pragma unroll
+  for (int i = 0; i < dma_count<RB, ROWS>(); ++i) {
+    const int k = k0 + i * 4 * DmaLane<RB>::RPI + dl.row;
+    rn.n[i] = k < L ? order[k] : 0;
+  }
+}
+template <int RB, int ROWS, int NW, bool PICK = false>
 __device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* base, int64_t ldbytes, const DmaLane<RB>& dl, int wave,
-                                         const uint32_t (&w)[NW]) {
-  constexpr int RPI = DmaLane<RB>::RPI, N = ROWS >= 4 * RPI ? ROWS / (4 * RPI) : 1;        // instructions per wave
+                                         const uint32_t (&w)[NW], const RowNumbers<dma_count<RB, ROWS>()>* rn = nullptr) {
+  constexpr int RPI = DmaLane<RB>::RPI, N = dma_count<RB, ROWS>();
   static_assert(NW == ROWS / 32, "");
   if (ROWS < 4 * RPI && wave * RPI >= ROWS) return;                  // (narrow rows: two waves fill the tile)
   const uint64_t at = reinterpret_cast<uint64_t>(base);
@@ -121,11 +134,13 @@ __device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* b
     uint32_t word = w[r0 / 32];
     int bit = r0 % 32 + dl.row;
     if constexpr (4 * RPI > 32 && ROWS > 32) { if (dl.row >= 32) word = w[r0 / 32 + 1]; bit &= 31; }
-    const uint32_t off = (word >> bit) & 1u ? dl.off[i % DmaLane<RB>::VAR] : OOB;
+    uint32_t off = dl.off[i % DmaLane<RB>::VAR];
+    if constexpr (PICK) off = off == OOB ? OOB : off + rn->n[i] * (uint32_t)ldbytes;
+    off = (word >> bit) & 1u ? off : OOB;
     // asm: the compiler lets no transposing LDS read start before the DMA it knows of has landed (it cannot tell the buffers
     // apart), i.e. it would wait for the NEXT tile in the middle of this one.  wait_tiles orders the DMA; the asm has no outputs.
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
-                 :: "v"(off), "s"(rs), "s"(l0 + i * 4096), "s"(r0 * (int)ldbytes) : "memory");
+                 :: "v"(off), "s"(rs), "s"(l0 + i * 4096), "s"(PICK ? 0 : r0 * (int)ldbytes) : "memory");
   }
 }
 // This wave's DMA has landed and its LDS reads are done; then all waves'.  The builtin, not asm: the compiler has to know that
@@ -135,6 +150,14 @@ __device__ __forceinline__ void wait_tiles() {
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
+}
+
+// 64 floats of a row statistic, one a lane: base[lane], or 0 where lane >= n
+__device__ __forceinline__ void dma_floats(char* smem, uint32_t lds, const float* base, int n, int lane) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const i32x4 rs = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32), 0x7fffffff, 0x00020000};
+  const uint32_t off = lane < n ? lane * 4u : OOB, l0 = (uint32_t)(uintptr_t)(lds_void*)smem + lds;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" :: "v"(off), "s"(rs), "s"(l0) : "memory");
 }
 
 // the other half wave's value joined in: lane and lane ^ 32 hold the same row
@@ -503,7 +526,7 @@ template <int KG, int LDO> __device__ __forceinline__ float4 group_sum(const flo
 }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DT, int KG, int NP>
+template <typename T, int DT, int KG, int NP, bool PICK>
 __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : DT * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
   constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
@@ -550,15 +573,20 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : DT 
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
   DmaLane<RB> kdl, vdl;
-  kdl.init(klb, dbytes, wave, lane);
-  vdl.init(vlb, dbytes, wave, lane);
+  kdl.init(klb, dbytes, wave, lane, PICK);
+  vdl.init(vlb, dbytes, wave, lane, PICK);
+  const int* order = PICK ? a.order + (int64_t)b * a.Lk : nullptr;
+  RowNumbers<dma_count<RB, KT>()> rn;
+  if constexpr (PICK) order_fetch<RB, KT>(rn, order, t0 * KT, a.Lk, kdl);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
+    const int64_t first = PICK ? 0 : (int64_t)t * KT;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      dma_tile<RB, KT>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + (int64_t)t * KT * a.t0l, klb, kdl, wave, kw.w);
-      dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + (int64_t)t * KT * a.t1l, vlb, vdl, wave, kw.w);
+      dma_tile<RB, KT, KT / 32, PICK>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + first * a.t0l, klb, kdl, wave, kw.w, &rn);
+      dma_tile<RB, KT, KT / 32, PICK>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + first * a.t1l, vlb, vdl, wave, kw.w, &rn);
     }
     start_put(start + buf * KT, kw, tid);
+    if constexpr (PICK) order_fetch<RB, KT>(rn, order, (t + 1) * KT, a.Lk, kdl);
   };
   fill(t0, 0, cur);
   Rows<T, DT, NP> qf;
@@ -755,9 +783,10 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
 //
 // delta = do . o is off by the rounding of a bf16 o, which weighs where a query sees a few keys (o is as large as a value then, and
-// the scores' gradient a difference of few terms: 3 keys gave dq an error of 0.0037, 100 keys 0.0024).  Items of up to 32 keys take delta + sum_j P_j (do . v_j - delta)
-// instead: the exact sum, at the price of the tile's products once more.  (0 stays 0 where one key is seen.)
-template <typename T, int DT, int KG, int NP>
+// the scores' gradient a difference of few terms: 3 keys gave dq an error of 0.0037, 100 keys 0.0024).  Items of up to 32 keys take
+// delta + sum_j P_j (do . v_j - delta) instead: the exact sum, at the price of the tile's products once more.  (0 stays 0 where one
+// key is seen.)
+template <typename T, int DT, int KG, int NP, bool PICK>
 __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
   constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
@@ -791,7 +820,10 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * s
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
   }
-  if (!few && sp == 0 && m < M && lh == 0 && kg == 0) a.delta[srow] = dl;
+  if (sp == 0 && m < M && lh == 0 && kg == 0) {
+    a.lse2[srow] = lse2;
+    if (!few) a.delta[srow] = dl;
+  }
   int t0, t1;
   tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
   if (m0 >= Mv || t0 >= t1) {
@@ -810,15 +842,20 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * s
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
   DmaLane<RB> kdl, vdl;
-  kdl.init(klb, dbytes, wave, lane);
-  vdl.init(vlb, dbytes, wave, lane);
+  kdl.init(klb, dbytes, wave, lane, PICK);
+  vdl.init(vlb, dbytes, wave, lane, PICK);
+  const int* order = PICK ? a.order + (int64_t)b * a.Lk : nullptr;
+  RowNumbers<dma_count<RB, KT>()> rn;
+  if constexpr (PICK) order_fetch<RB, KT>(rn, order, t0 * KT, a.Lk, kdl);
   auto fill = [&](int t, int buf, const KeyWords<KT>& kw) {
+    const int64_t first = PICK ? 0 : (int64_t)t * KT;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      dma_tile<RB, KT>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + (int64_t)t * KT * a.t0l, klb, kdl, wave, kw.w);
-      dma_tile<RB, KT>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + (int64_t)t * KT * a.t1l, vlb, vdl, wave, kw.w);
+      dma_tile<RB, KT, KT / 32, PICK>(smem, buf * 2 * TILE + k * TS, kbase + k * a.t0p + first * a.t0l, klb, kdl, wave, kw.w, &rn);
+      dma_tile<RB, KT, KT / 32, PICK>(smem, buf * 2 * TILE + TILE + k * TS, vbase + k * a.t1p + first * a.t1l, vlb, vdl, wave, kw.w, &rn);
     }
     start_put(start + buf * KT, kw, tid);
+    if constexpr (PICK) order_fetch<RB, KT>(rn, order, (t + 1) * KT, a.Lk, kdl);
   };
   fill(t0, 0, cur);
   load_rows(qf, a.q, b * a.qb + qi * a.ql + head * a.qh, a.D, lh, live);
@@ -959,7 +996,8 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
   constexpr int RB = DT * sizeof(T), RT = NP == 3 ? 32 : 64, TS = RT * RB, TILE = NP * TS, RW = 4 / KW, NBLK = RT / 32 / RW;
   constexpr int SHARE = 32 * DT * 4;                     // LDS of a wave for its results, once the tiles are done with
   static_assert(NBLK >= 1 && 4 * SHARE <= 4 * TILE, "");
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE + 4 * RT * 4];
+  constexpr int STAT = 4 * TILE;                         // [buf][lse2 | delta][64]
+  __shared__ __attribute__((aligned(1024))) char smem[STAT + 2 * 512];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
   const int kwv = wave / RW, rwv = wave % RW;
   const int v = xcd_block(a.nrt * a.splits * a.G * a.B, a.chunk);
@@ -969,7 +1007,10 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
   const int key = kt * 32 * KW + kwv * 32 + li;
   const bool seen = key < klen && !(a.mask && a.mask[b * a.maskb + key]);
   const bool some = __builtin_amdgcn_ballot_w64(seen) != 0;
-  const int64_t krow = ((int64_t)b * a.Lk + key) * a.G + g, krows = (int64_t)a.B * a.Lk * a.G;
+  // the block's p-th key is key number order[p] of the item, its row of k, v and of the gradients
+  const int* order = a.order ? a.order + (int64_t)b * a.Lk : nullptr;
+  const int knum = order && key < a.Lk ? order[key] : key;
+  const int64_t krow = ((int64_t)b * a.Lk + knum) * a.G + g, krows = (int64_t)a.B * a.Lk * a.G;
   const int nt = (qv + RT - 1) / RT, total = nt * a.R;
   int t0, t1;
   tile_range(total, sp, a.splits, t0, t1);
@@ -987,8 +1028,6 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
   }
   const int dbytes = (NP == 3 ? DT : a.D) * (int)sizeof(T);
   const int64_t qlb = a.t0l * (int64_t)sizeof(T), glb = a.t1l * (int64_t)sizeof(T);
-  float* stat = reinterpret_cast<float*>(smem + 4 * TILE);         // [buf][lse2 | delta][RT]
-  float sreg = 0.f;
   DmaLane<RB> qdl, gdl;
   qdl.init(qlb, dbytes, wave, lane);
   gdl.init(glb, dbytes, wave, lane);
@@ -1004,33 +1043,26 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
       dma_tile<RB, RT>(smem, buf * 2 * TILE + k * TS, qp + k * a.t0p, qlb, qdl, wave, w);
       dma_tile<RB, RT>(smem, buf * 2 * TILE + TILE + k * TS, gp + k * a.t1p, glb, gdl, wave, w);
     }
-    if (tid < 2 * RT) {
-      const int q = q0 + tid % RT;
-      const int64_t s = ((int64_t)b * a.H + head) * a.Lq + q;
-      sreg = tid < RT ? INFINITY : 0.f;                             // rows past the queries: P = exp2(s - inf) = 0
-      if (q < qv) {
-        sreg = tid < RT ? a.lse[s] * LOG2E : a.delta[s];
-        if (tid < RT && sreg == -INFINITY) sreg = INFINITY;
-      }
+    if (wave < 2) {                                      // (rows past the queries are zeros throughout: they add 0, whatever P is)
+      const float* st = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.H + head) * a.Lq + q0;
+      dma_floats(smem, STAT + buf * 512 + wave * 256, st, left < RT ? left : RT, lane);
     }
   };
-  auto put_stat = [&](int buf) { if (tid < 2 * RT) stat[buf * 2 * RT + tid] = sreg; };
   fill(t0, 0);
   Rows<T, DT, NP> kf, vf;
-  load_rows(kf, a.k, b * a.kb + (int64_t)key * a.kl + g * a.kh, a.D, lh, seen);
-  load_rows(vf, a.v, b * a.vb + (int64_t)key * a.vl + g * a.vh, a.D, lh, seen);
+  load_rows(kf, a.k, b * a.kb + (int64_t)knum * a.kl + g * a.kh, a.D, lh, seen);
+  load_rows(vf, a.v, b * a.vb + (int64_t)knum * a.vl + g * a.vh, a.D, lh, seen);
   f32x16 dk[DT / 32], dv[DT / 32];
 #pragma unroll
   for (int i = 0; i < DT / 32; ++i) { zero16(dk[i]); zero16(dv[i]); }
   const float SC = a.scale * LOG2E;
-  put_stat(0);
   wait_tiles();
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     if (t + 1 < t1) fill(t + 1, buf ^ 1);
     const char* tq = smem + buf * 2 * TILE;
     const char* tg = tq + TILE;
-    const float* st = stat + buf * 2 * RT;
+    const float* st = reinterpret_cast<const float*>(smem + STAT + buf * 512);
     if (some)                                            // (a wave whose keys are all unseen only helps to load)
 #pragma unroll DKV_UNROLL<T, DT, NP>
     for (int hb = 0; hb < NBLK; ++hb) {
@@ -1045,7 +1077,7 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
         const float4 L = *reinterpret_cast<const float4*>(st + blk * 32 + gq * 8 + lh * 4);
-        const float4 E = *reinterpret_cast<const float4*>(st + RT + blk * 32 + gq * 8 + lh * 4);
+        const float4 E = *reinterpret_cast<const float4*>(st + 64 + blk * 32 + gq * 8 + lh * 4);
         const float ls[4] = {L.x, L.y, L.z, L.w}, de[4] = {E.x, E.y, E.z, E.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1059,7 +1091,6 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
       mma_cols<T, DT, NP, TS>(dk, tq, blk, dp, lane);
       __builtin_amdgcn_s_setprio(0);
     }
-    if (t + 1 < t1) put_stat(buf ^ 1);
     wait_tiles();
   }
   if constexpr (RW == 2) {                               // the second half of the rows joins the first
@@ -1068,15 +1099,16 @@ __global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(
     if (rwv == 1) return;
   }
   const int kw = kt * 32 * KW + kwv * 32;
+  auto row_of = [&](int r) { return ((int64_t)b * a.Lk + (order ? order[kw + r] : kw + r)) * a.G + g; };
   if (a.splits > 1) {
     float* pk = a.part + sp * 2 * krows * a.D;
     float* pv = pk + krows * a.D;
-    auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; }; };
+    auto at = [&](float* base) { return [=](int r) { return kw + r < a.Lk ? base + row_of(r) * a.D : nullptr; }; };
     store_tile<float, DT>(smem + wave * SHARE, dk, a.D, lane, a.scale, seen, at(pk));
     store_tile<float, DT>(smem + wave * SHARE, dv, a.D, lane, 1.f, seen, at(pv));
   } else {
     auto at = [&](void* base) {
-      return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<O*>(base) + (((int64_t)b * a.Lk + kw + r) * a.G + g) * a.D : nullptr; };
+      return [=](int r) { return kw + r < a.Lk ? reinterpret_cast<O*>(base) + row_of(r) * a.D : nullptr; };
     };
     store_tile<O, DT>(smem + wave * SHARE, dk, a.D, lane, a.scale, seen, at(a.dk));
     store_tile<O, DT>(smem + wave * SHARE, dv, a.D, lane, 1.f, seen, at(a.dv));
@@ -1116,6 +1148,7 @@ struct SplitArgs {
   const float* src[4];
   uint16_t* dst[4];
   const int64_t* len[4];
+  const int* order[4];                                   // rows are taken in this order ([B, L]), or as they stand
   int64_t sb[4], sl[4], sh[4];
   int L[4], Hn[4];
   int B, D, W;
@@ -1130,7 +1163,8 @@ __global__ __launch_bounds__(256) void xattn_split_kernel(SplitArgs a) {
       const int d = (int)(i - l * ppr) * 8;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
       if (d < a.D) {
-        const float* p = a.src[z] + b * a.sb[z] + l * a.sl[z] + h * a.sh[z] + d;
+        const int64_t from = a.order[z] ? a.order[z][(int64_t)b * L + l] : l;
+        const float* p = a.src[z] + b * a.sb[z] + from * a.sl[z] + h * a.sh[z] + d;
         u = *reinterpret_cast<const float4*>(p);
         v = *reinterpret_cast<const float4*>(p + 4);
       }
@@ -1144,6 +1178,57 @@ __global__ __launch_bounds__(256) void xattn_split_kernel(SplitArgs a) {
   }
 }
 
+// The keys of an item in a new order: those that are seen first, in their own order, then the others.  order [B, Lk], count [B].
+// The other kernels then walk the first count[b] keys, without a mask: keys that it drops cost nothing instead of a whole product
+// (8 x 2048 x 1500 x 16 heads, training, one key in four dropped: 541 -> 461 us).  A block orders 2048 keys; those before it, it counts.
+__device__ __forceinline__ int zero_bytes(uint32_t x) { return 4 - __builtin_popcount((((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u); }
+__global__ __launch_bounds__(256) void xattn_order_kernel(const uint8_t* mask, int64_t maskb, const int64_t* len, int Lk, int* order, int64_t* count) {
+  __shared__ int red[8];
+  const int chunks = (Lk + 2047) / 2048, b = blockIdx.x / chunks, k0 = blockIdx.x % chunks * 2048, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = clamp_len(len, b, Lk);
+  mask += b * maskb;
+  order += (int64_t)b * Lk;
+  // seen keys in front of the block: single bytes up to a 16-byte border, then pieces
+  const int end = min(k0, n), head = min(end, (int)(-(intptr_t)mask & 15)), pieces = (end - head) / 16;
+  int before = 0;
+  if (tid < head) before += mask[tid] == 0;
+  for (int i = tid; i < pieces; i += 256) {
+    const uint4 u = *reinterpret_cast<const uint4*>(mask + head + i * 16);
+    before += zero_bytes(u.x) + zero_bytes(u.y) + zero_bytes(u.z) + zero_bytes(u.w);
+  }
+  if (head + pieces * 16 + tid < end) before += mask[head + pieces * 16 + tid] == 0;
+  // a thread's eight keys, and the seen ones among those of the lower lanes
+  uint32_t seen = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = k0 + tid * 8 + i;
+    seen |= k < n && mask[k] == 0 ? 1u << i : 0u;
+  }
+  const int mine = __builtin_popcount(seen);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += x;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o, 64);
+  if (lane == 63) { red[wave] = upto; red[4 + wave] = before; }
+  __syncthreads();
+  int at = red[4] + red[5] + red[6] + red[7] + upto - mine;
+  for (int w = 0; w < wave; ++w) at += red[w];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = k0 + tid * 8 + i;
+    if (k < Lk) {
+      const bool s = (seen >> i) & 1u;
+      order[s ? at : Lk - 1 - (k - at)] = k;             // k - at unseen keys stand before an unseen one
+      at += s ? 1 : 0;
+    }
+  }
+  if (k0 + 2048 >= Lk && tid == 255) count[b] = at;
+}
+
 // How many shares of a long axis (n tiles) give the launch about `want` blocks, each with at least `least` tiles.
 int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   int64_t s = (want + blocks - 1) / blocks;
@@ -1152,12 +1237,17 @@ int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : (int)s;
 }
-struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; };
+struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; bool order; };
 // Sizes alone decide.  512 blocks are two per CU, and shares are cut to reach that (2 x 65537 keys of one token: 256 blocks, one per CU,
 // 110 us, 512 113, 1024 118).  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
 // 81 us (every share writes its part once more); two key groups from 512 blocks of 128 rows down: 8 x 500 x 700 49 us, from 1024: the
 // fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).  fp32 with more than 64 rows a key head goes through
 // planes (their making pays from there on); with fewer it is bound by reading the keys, which planes would do twice.
+// A mask's keys are put in order from here on (rows x keys x width, six times that with planes): the ordering is a launch of 3 us.
+// One key in four dropped, without / with it, at 1.4e9 (8 x 8 heads x 500 x 700 x 64) 16.5 / 19.1 us, at 4.3e9 (8 x 8 x 1024 x 1024 x
+// 64) 28.5 / 28.1 and 107 / 102 (training), at 5.9e9 (4 x 8 x 1024 x 1400 x 128) 37 / 36, at 5.5e9 in planes 171 / 162.  (The rows
+// that a mask leaves out are zeros in the tiles otherwise: they cost the product, but little power.)
+constexpr double ORDER_FROM = 4294967296.;
 Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   Plan p;
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
@@ -1174,10 +1264,12 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   p.dq = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 4 : 256 / KT);
   p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
+  p.order = M > 64 && (double)BG * M * Lk * p.width * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
   const int RT = p.planes == 3 ? 32 : 64;
   p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), row >= 512 ? 256 : 512, 128 / RT);
   return p;
 }
+int64_t order_bytes(const Plan& p, int B, int Lk) { return p.order ? ((int64_t)4 * B * Lk + 15) / 16 * 16 + ((int64_t)8 * B + 15) / 16 * 16 : 0; }
 int64_t plane_bytes(const Plan& p, int B, int L, int Hn) { return p.planes == 3 ? (int64_t)6 * B * L * Hn * p.width : 0; }
 
 // Runs of logical blocks per XCD (see xcd_block): as long as the blocks of one (item, key head), but never fewer than 64 runs
@@ -1194,22 +1286,32 @@ dim3 grid_for(XArgs& a) {
 template <typename T, int DT>
 void launch_fwd(XArgs& a, const Plan& p, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (p.kg == 4) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 4, 1>), g, dim3(256), 0, st, a);
-  else if (p.kg == 2) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2, 1>), g, dim3(256), 0, st, a);
-  else if constexpr (sizeof(T) == 2) {
-    if (p.planes == 3) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 3>), g, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 1>), g, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    if (p.planes == 3) { hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 3, false>), g, dim3(256), 0, st, a); return; }       // (planes are made in order)
+    if (p.kg == 1) {
+      if (a.order) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 1, true>), g, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 1, 1, false>), g, dim3(256), 0, st, a);
+      return;
+    }
+    if (a.order) { hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2, 1, true>), g, dim3(256), 0, st, a); return; }
   }
+  if (p.kg == 4) hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 4, 1, false>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_fwd_kernel<T, DT, 2, 1, false>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
 void launch_dq(XArgs& a, const Plan& p, hipStream_t st) {
   const dim3 g = grid_for(a);
-  if (p.kg == 4) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 4, 1>), g, dim3(256), 0, st, a);
-  else if (p.kg == 2) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2, 1>), g, dim3(256), 0, st, a);
-  else if constexpr (sizeof(T) == 2) {
-    if (p.planes == 3) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 3>), g, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 1>), g, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    if (p.planes == 3) { hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 3, false>), g, dim3(256), 0, st, a); return; }
+    if (p.kg == 1) {
+      if (a.order) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 1, true>), g, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 1, 1, false>), g, dim3(256), 0, st, a);
+      return;
+    }
+    if (a.order) { hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2, 1, true>), g, dim3(256), 0, st, a); return; }
   }
+  if (p.kg == 4) hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 4, 1, false>), g, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((xattn_dq_kernel<T, DT, 2, 1, false>), g, dim3(256), 0, st, a);
 }
 template <typename T, int DT>
 void launch_dkv(XArgs& a, const Plan& p, hipStream_t st) {
@@ -1260,27 +1362,37 @@ XArgs args(const styler_xattn_t* x) {
 
 }  // namespace
 
-extern "C" int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int bwd) {
+extern "C" int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int masked, int bwd) {
   if (B < 1 || Lq < 1 || Lk < 1 || G < 1 || H < G || H % G || D < 8 || D > 128) return 0;
   const Plan p = make_plan(B, Lq, Lk, H, G, D, bf16);
   const int64_t qrows = (int64_t)B * H * Lq, krows = (int64_t)B * G * Lk;
-  const int64_t kv = 2 * plane_bytes(p, B, Lk, G);
+  const int64_t kv = 2 * plane_bytes(p, B, Lk, G) + (masked ? order_bytes(p, B, Lk) : 0);
   if (!bwd) return (p.fwd > 1 ? (4 * p.fwd * qrows * (D + 2) + 15) / 16 * 16 : 0) + kv;
   int64_t part = p.dq > 1 ? p.dq * qrows * D : 0;
   const int64_t pkv = p.dkv > 1 ? 2 * p.dkv * krows * D : 0;
   if (pkv > part) part = pkv;                            // the two gradients' launches follow each other: one buffer
-  return 4 * (part + (qrows + 3) / 4 * 4) + kv + 2 * plane_bytes(p, B, Lq, H);
+  return (4 * (part + (qrows + 3) / 4 * 8) + 15) / 16 * 16 + kv + 2 * plane_bytes(p, B, Lq, H);
 }
 
 namespace {
 // the tensors' planes, one after the other at `at`
-struct SplitJob { const void* src; int64_t sb, sl, sh; int L, Hn; const int64_t* len; };
+// the seen keys first, if that pays: order and count at `at` (order_bytes), and the rest of the call sees a batch of lengths without a mask
+void put_in_order(XArgs& a, const Plan& p, char* at, hipStream_t st) {
+  if (!a.mask || !p.order || a.Lk * a.kl * 4 >= (int64_t)1 << 31 || a.Lk * a.vl * 4 >= (int64_t)1 << 31) return;      // (32-bit offsets)
+  int* order = (int*)at;
+  int64_t* count = (int64_t*)(at + ((int64_t)4 * a.B * a.Lk + 15) / 16 * 16);
+  hipLaunchKernelGGL(xattn_order_kernel, dim3((a.Lk + 2047) / 2048 * a.B), dim3(256), 0, st, a.mask, a.maskb, a.len, a.Lk, order, count);
+  a.order = order;
+  a.len = count;
+  a.mask = nullptr;
+}
+struct SplitJob { const void* src; int64_t sb, sl, sh; int L, Hn; const int64_t* len; const int* order; };
 void launch_split(const SplitJob* job, int n, uint16_t* at, const XArgs& a, const Plan& p, hipStream_t st) {
   SplitArgs s = {};
   s.B = a.B; s.D = a.D; s.W = p.width;
   int most = 0, heads = 0;
   for (int i = 0; i < n; ++i) {
-    s.src[i] = (const float*)job[i].src; s.dst[i] = at; s.len[i] = job[i].len;
+    s.src[i] = (const float*)job[i].src; s.dst[i] = at; s.len[i] = job[i].len; s.order[i] = job[i].order;
     s.sb[i] = job[i].sb; s.sl[i] = job[i].sl; s.sh[i] = job[i].sh; s.L[i] = job[i].L; s.Hn[i] = job[i].Hn;
     at += (int64_t)3 * a.B * job[i].L * job[i].Hn * p.width;
     if (job[i].L > most) most = job[i].L;
@@ -1303,15 +1415,17 @@ void tiles_from_planes(XArgs& a, const uint16_t* x0, int L, int Hn, int W) {
 
 extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check(x, false)) return rc;
-  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, 0);
+  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, x->mask != nullptr, 0);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return STYLER_EINVAL;
   const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   a.nrt = p.nrt; a.splits = p.fwd; a.part = p.fwd > 1 ? (float*)workspace : nullptr;
+  char* end = (char*)workspace + need;                   // from the end: the order, the planes
+  if (x->mask) put_in_order(a, p, end -= order_bytes(p, x->B, x->Lk), st);
   if (p.planes == 3) {
-    uint16_t* planes = (uint16_t*)((char*)workspace + need - 2 * plane_bytes(p, x->B, x->Lk, x->G));
-    const SplitJob job[2] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, x->len}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, x->len}};
+    uint16_t* planes = (uint16_t*)(end - 2 * plane_bytes(p, x->B, x->Lk, x->G));
+    const SplitJob job[2] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, a.len, a.order}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, a.len, a.order}};
     launch_split(job, 2, planes, a, p, st);
     tiles_from_planes(a, planes, x->Lk, x->G, p.width);
   } else {
@@ -1331,19 +1445,23 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
 
 extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check(x, true)) return rc;
-  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, 1);
+  const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, x->mask != nullptr, 1);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return STYLER_EINVAL;
   const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   const int64_t qrows = (int64_t)x->B * x->H * x->Lq, krows = (int64_t)x->B * x->G * x->Lk;
   a.delta = (float*)workspace;
-  a.part = (float*)workspace + (qrows + 3) / 4 * 4;
+  a.lse2 = a.delta + (qrows + 3) / 4 * 4;
+  a.part = a.lse2 + (qrows + 3) / 4 * 4;
   const int64_t kvb = 2 * plane_bytes(p, x->B, x->Lk, x->G), qb = 2 * plane_bytes(p, x->B, x->Lq, x->H);
-  uint16_t* planes = (uint16_t*)((char*)workspace + need - kvb - qb);        // k, v, q, dout
+  char* end = (char*)workspace + need;
+  if (x->mask) put_in_order(a, p, end -= order_bytes(p, x->B, x->Lk), st);
+  uint16_t* planes = (uint16_t*)(end - kvb - qb);        // k, v, q, dout
   if (p.planes == 3) {
-    const SplitJob job[4] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, x->len}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, x->len},
-                             {x->q, x->qb, x->ql, x->qh, x->Lq, x->H, x->q_len}, {x->dout, x->gb, x->gl, x->gh, x->Lq, x->H, x->q_len}};
+    const SplitJob job[4] = {{x->k, x->kb, x->kl, x->kh, x->Lk, x->G, a.len, a.order}, {x->v, x->vb, x->vl, x->vh, x->Lk, x->G, a.len, a.order},
+                             {x->q, x->qb, x->ql, x->qh, x->Lq, x->H, x->q_len, nullptr},
+                             {x->dout, x->gb, x->gl, x->gh, x->Lq, x->H, x->q_len, nullptr}};
     launch_split(job, 4, planes, a, p, st);
     tiles_from_planes(a, planes, x->Lk, x->G, p.width);
   } else {

@@ -1995,7 +1995,7 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
             lse.fill_(-math.inf)
         return out.zero_()
     (q, qt), (k, kt), (v, vt) = _heads(q, es), _heads(k, es), _heads(v, es)
-    n = _xattn_ws(*sizes, 0)
+    n = _xattn_ws(*sizes, mask is not None, 0)
     with _on(q.device):
         ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
         args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _addr(lse), _addr(lens),
@@ -2018,7 +2018,7 @@ def cross_attention_bwd(q, k, v, out, dout, lse, lens=None, *, q_lens=None, mask
     if dq.numel() == 0 or dk.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, qt), (k, kt), (v, vt), (out, ot), (dout, gt) = (_heads(t, es) for t in (q, k, v, out, dout))
-    n = _xattn_ws(*sizes, 1)
+    n = _xattn_ws(*sizes, mask is not None, 1)
     with _on(q.device):
         ws = torch.empty(n, device=q.device, dtype=torch.uint8)
         args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),

@@ -180,6 +180,72 @@ def test_cross_attention_masks(dev, dtype, Lq):
 
 @gpu
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D,shared", [
+    (5, 130, 2101, 8, 4, 96, False),         # two blocks of keys in the ordering, few rows: two key groups
+    (4, 520, 1203, 4, 2, 64, True),          # one mask for all items
+    (3, 1030, 700, 6, 6, 128, False),
+    (9, 1100, 4100, 1, 1, 32, False),        # blocks of 128 rows, three blocks of keys
+])
+def test_cross_attention_long_masks(dev, B, Lq, Lk, H, G, D, shared, dtype):
+    """Masks long enough that the seen keys are put in front: every key, none, one, a run, every other, at random; with lengths, and
+    what stands in the unseen rows is NaN."""
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, dtype, seed=31)
+    mask = torch.rand(B, Lk + 3, generator=torch.Generator().manual_seed(6))[:, 3:] < 0.4         # rows on odd addresses
+    mask[1] = False
+    mask[2] = True
+    mask[2, Lk - 30] = False
+    if B > 3:
+        mask[3] = torch.arange(Lk) % 2 == 0
+        mask[3, :600] = True
+    lens = torch.randint(Lk // 2, Lk + 50, (B,), generator=torch.Generator().manual_seed(7))
+    lens[1], lens[2] = Lk, Lk
+    if B > 4:
+        lens[4] = 0
+    if shared:
+        mask = mask[:1]
+    seen = (torch.arange(Lk)[None] < lens[:, None]) & ~mask
+    k2, v2 = k.clone(), v.clone()
+    k2[~seen.to(dev)] = math.nan
+    v2[~seen.to(dev)] = math.nan
+    got = check_attention(q, k2, v2, do, lens, torch.randint(1, Lq + 1, (B,)), mask, oracle=(q, k, v, do))
+    assert not got[2][~seen.to(dev)].any() and not got[3][~seen.to(dev)].any()
+    check_attention(q, k2, v2, do, lens, None, mask, oracle=(q, k, v, do))
+
+
+@gpu
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D,dtype", [
+    (5, 1100, 2101, 16, 8, 32, torch.bfloat16), (16, 2050, 2200, 2, 2, 32, torch.bfloat16),
+    (2, 2050, 4097, 4, 2, 64, torch.bfloat16), (8, 1030, 1025, 8, 8, 64, torch.bfloat16),
+    (2, 1100, 4200, 4, 4, 128, torch.bfloat16), (9, 1000, 530, 8, 8, 80, torch.bfloat16),
+    (5, 1100, 2101, 4, 2, 32, torch.float32), (3, 600, 1500, 8, 4, 64, torch.float32), (2, 300, 6000, 2, 2, 72, torch.float32),
+])
+def test_cross_attention_masked_keys_are_left_out(dev, B, Lq, Lk, H, G, D, dtype):
+    """A mask that is put in order gives, bit for bit, what the seen keys give that stand at the front of each item by themselves."""
+    from styler_amd import ops
+    g = torch.Generator(device=dev).manual_seed(B + Lk)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(dtype)
+    q, kv, do = r(B, Lq, H, D), r(B, Lk, 2, G, D), r(B, Lq, H, D)
+    mask = torch.rand(B, Lk, generator=g, device=dev) < torch.linspace(0.1, 0.9, B, device=dev)[:, None]
+    lens = torch.full((B,), Lk - 5, device=dev)
+    seen = ~mask & (torch.arange(Lk, device=dev)[None] < lens[:, None])
+    order = torch.argsort((~seen).int(), dim=1, stable=True)
+    front = torch.gather(kv, 1, order.view(B, Lk, 1, 1, 1).expand(-1, -1, 2, G, D))
+    count = seen.sum(1)
+
+    def both(k, v, n, m):
+        lse = torch.empty(B, H, Lq, device=dev)
+        out = ops.cross_attention(q, k, v, n, mask=m, lse=lse)
+        return out, lse, *ops.cross_attention_bwd(q, k, v, out, do, lse, n, mask=m)
+
+    a, b = both(kv[:, :, 0], kv[:, :, 1], lens, mask), both(front[:, :, 0], front[:, :, 1], count, None)
+    assert all(torch.equal(x, y) for x, y in zip(a[:3], b[:3]))
+    for x, y in zip(a[3:], b[3:]):
+        assert torch.equal(torch.gather(x, 1, order.view(B, Lk, 1, 1).expand(-1, -1, G, D)), y)
+        assert not x[~seen].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("Lq,Lk", [(1, 2048), (200, 96), (6, 700)])
 def test_cross_attention_layouts(dev, dtype, Lq, Lk):
     """Slices of fused projections, heads before rows, one encoder output shared by all items, a gradient with stride zero, rows
