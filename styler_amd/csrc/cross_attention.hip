@@ -1260,7 +1260,9 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   const int KT = 32 * p.kg * (p.kg == 1 && row <= 256 ? 2 : 1);
   const int64_t kt = (Lk + KT - 1) / KT;
   const int want = row >= 512 || (p.kg == 4 && row >= 256) ? 256 : 512;        // (LDS holds one block of these per CU)
-  p.fwd = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 2 : 128 / KT);
+  // (a token over under eight tiles of up to 32 KB is one share: the join is a launch more, 4 us of the host's time.  700 keys of 64 bf16
+  // features, shared out / not: 32 x 4 heads 14 / 10 us a call, 10.1 / 8.9 in a graph; 8 x 4 heads 13.5 / 10.9, 9.6 / 10.5)
+  p.fwd = p.kg == 4 && row <= 128 && kt < 8 ? 1 : split_count(BG * p.nrt, kt, want, p.kg == 4 ? 2 : 128 / KT);
   p.dq = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 4 : 256 / KT);
   p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
