@@ -4,7 +4,6 @@ PyTorch supplies device memory (caching allocator), the current HIP stream and n
 function here hands raw device pointers + sizes to libstyler_hip.so.  Activations are fp32
 channels-last [B, L, C]; a channel slice `x[..., a:b]` of a wider buffer is a legal argument (the row
 stride travels as `ld`), which is how torch.cat / torch.split copies of the reference disappear."""
-import contextlib
 import functools
 import math
 import os
@@ -1870,18 +1869,13 @@ def adam_step(p, g, m, v, sumsq_buf, max_norm, lr, beta1, beta2, eps, step, grad
 # fp32 or bf16 tensors with their own strides; what a kernel cannot read in place (features not contiguous, rows not on 16 bytes) is
 # copied first.  They run on the current stream of the tensors' device, whichever device is current.  A token's call is bound by this
 # file: shapes, strides and types are looked at once each, and the arguments go over as one packed structure.
-_ON_CURRENT = contextlib.nullcontext()
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _refuse(name, what):
     raise StylerHipError(f"{name}: {what}")
-
-
-def _on(device):
-    """Makes `device` the current one for the launches inside."""
-    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _like(name, t, what, shape, dtype, device):
@@ -1987,6 +1981,10 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
     out (optional): the result's tensor, which shares no memory with the inputs."""
     name = "cross_attention"
     sizes, scale, lens, q_lens, mask, maskb = _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, True)
+    device = q.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return cross_attention(q, k, v, lens, q_lens=q_lens, mask=mask, scale=scale, out=out, lse=lse)
     es = 2 if sizes[6] else 4
     if out is None:
         out = _new(q)
@@ -1996,11 +1994,10 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
         return out.zero_()
     (q, qt), (k, kt), (v, vt) = _heads(q, es), _heads(k, es), _heads(v, es)
     n = _xattn_ws(*sizes, mask is not None, 0)
-    with _on(q.device):
-        ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-        args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _addr(lse), _addr(lens),
-                          _addr(q_lens), _addr(mask), *qt, *kt, *vt, *_heads(out, es)[1], 0, 0, 0, maskb, *sizes, scale)
-        _chk(lib.styler_cross_attention(args, _addr(ws), n, _raw_stream(q.device.index)), "styler_cross_attention")
+    ws = torch.empty(n, device=device, dtype=torch.uint8) if n else None
+    args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _addr(lse), _addr(lens), _addr(q_lens),
+                      _addr(mask), *qt, *kt, *vt, *_heads(out, es)[1], 0, 0, 0, maskb, *sizes, scale)
+    _chk(lib.styler_cross_attention(args, _addr(ws), n, _raw_stream(device.index)), "styler_cross_attention")
     return out
 
 
@@ -2013,18 +2010,21 @@ def cross_attention_bwd(q, k, v, out, dout, lse, lens=None, *, q_lens=None, mask
         _refuse(name, "the forward's lse is needed")
     _like(name, dout, "dout", q.shape, q.dtype, q.device)
     sizes, scale, lens, q_lens, mask, maskb = _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, False)
+    device = q.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return cross_attention_bwd(q, k, v, out, dout, lse, lens, q_lens=q_lens, mask=mask, scale=scale)
     es = 2 if sizes[6] else 4
     dq, dk, dv = _new(q), _new(k), _new(k)
     if dq.numel() == 0 or dk.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, qt), (k, kt), (v, vt), (out, ot), (dout, gt) = (_heads(t, es) for t in (q, k, v, out, dout))
     n = _xattn_ws(*sizes, mask is not None, 1)
-    with _on(q.device):
-        ws = torch.empty(n, device=q.device, dtype=torch.uint8)
-        args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                          dv.data_ptr(), lse.data_ptr(), _addr(lens), _addr(q_lens), _addr(mask), *qt, *kt, *vt, *ot, *gt, maskb,
-                          *sizes, scale)
-        _chk(lib.styler_cross_attention_bwd(args, ws.data_ptr(), n, _raw_stream(q.device.index)), "styler_cross_attention_bwd")
+    ws = torch.empty(n, device=device, dtype=torch.uint8)
+    args = XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                      dv.data_ptr(), lse.data_ptr(), _addr(lens), _addr(q_lens), _addr(mask), *qt, *kt, *vt, *ot, *gt, maskb,
+                      *sizes, scale)
+    _chk(lib.styler_cross_attention_bwd(args, ws.data_ptr(), n, _raw_stream(device.index)), "styler_cross_attention_bwd")
     return dq, dk, dv
 
 
@@ -2087,6 +2087,9 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
         _refuse(name, "out shares memory with x in another layout")
     if not x.is_cuda:
         _refuse(name, "there is no CPU form")
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return rotary(x, freqs, pos, interleaved=interleaved, gain=gain, inverse=inverse, out=out)
     if x.stride(3) != 1:
         x = x.contiguous()
     if freqs.stride(0) != 1:
@@ -2103,10 +2106,9 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
         xl = yl = 0
     if H == 1:
         xh = yh = 0
-    with _on(device):
-        args = ROTARY.pack(x.data_ptr(), out.data_ptr(), freqs.data_ptr(), _addr(pos), xb, xl, xh, yb, yl, yh, posb, B, L, H, D, 2 * n,
-                           kind, 1 if interleaved else 0, 1 if inverse else 0, bf16, gain)
-        _chk(lib.styler_rotary(args, _raw_stream(device.index)), "styler_rotary")
+    args = ROTARY.pack(x.data_ptr(), out.data_ptr(), freqs.data_ptr(), _addr(pos), xb, xl, xh, yb, yl, yh, posb, B, L, H, D, 2 * n,
+                       kind, 1 if interleaved else 0, 1 if inverse else 0, bf16, gain)
+    _chk(lib.styler_rotary(args, _raw_stream(device.index)), "styler_rotary")
     return out
 
 
@@ -2154,6 +2156,10 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
         _refuse(name, "out shares memory with x in another layout")
     sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, out, "out")
     B, L, C, _ = sizes
+    device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return groupnorm_act(x, gamma, beta, groups, act, eps=eps, lens=lens, out=out, stats=stats)
     if out is None:
         out = _new(x)
     elif not _rows_ok(out.shape, out.stride()):
@@ -2164,11 +2170,10 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
         return out
     (x, xb, xl), (_, ob, ol) = _gn_rows(x, B, L, C), _gn_rows(out, B, L, C)
     n = _gn_ws(*sizes, bf16, 0)
-    with _on(x.device):
-        ws = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
-        args = GN.pack(x.data_ptr(), 0, out.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _addr(stats), 0, 0, _addr(lens),
-                       xb, xl, 0, 0, ob, ol, *sizes, act, bf16, eps)
-        _chk(lib.styler_groupnorm_act(args, _addr(ws), n, _raw_stream(x.device.index)), "styler_groupnorm_act")
+    ws = torch.empty(n, device=device, dtype=torch.uint8) if n else None
+    args = GN.pack(x.data_ptr(), 0, out.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _addr(stats), 0, 0, _addr(lens),
+                   xb, xl, 0, 0, ob, ol, *sizes, act, bf16, eps)
+    _chk(lib.styler_groupnorm_act(args, _addr(ws), n, _raw_stream(device.index)), "styler_groupnorm_act")
     return out
 
 
@@ -2180,14 +2185,17 @@ def groupnorm_act_bwd(x, dy, gamma, beta, stats, groups, act=ACT_SILU, *, lens=N
         _refuse(name, "the forward's stats are needed")
     sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, 0.0, lens, stats, dy, "dy")
     B, L, C, _ = sizes
+    device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return groupnorm_act_bwd(x, dy, gamma, beta, stats, groups, act, lens=lens)
     dx, dgamma, dbeta = _new(x), _new(gamma), _new(gamma)
     if dx.numel() == 0:
         return dx, dgamma.zero_(), dbeta.zero_()
     (x, xb, xl), (dy, db, dl), (_, ob, ol) = _gn_rows(x, B, L, C), _gn_rows(dy, B, L, C), _gn_rows(dx, B, L, C)
     n = _gn_ws(*sizes, bf16, 1)
-    with _on(x.device):
-        ws = torch.empty(n, device=x.device, dtype=torch.uint8)
-        args = GN.pack(x.data_ptr(), dy.data_ptr(), dx.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
-                       dgamma.data_ptr(), dbeta.data_ptr(), _addr(lens), xb, xl, db, dl, ob, ol, *sizes, act, bf16, 0.0)
-        _chk(lib.styler_groupnorm_act_bwd(args, ws.data_ptr(), n, _raw_stream(x.device.index)), "styler_groupnorm_act_bwd")
+    ws = torch.empty(n, device=device, dtype=torch.uint8)
+    args = GN.pack(x.data_ptr(), dy.data_ptr(), dx.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
+                   dgamma.data_ptr(), dbeta.data_ptr(), _addr(lens), xb, xl, db, dl, ob, ol, *sizes, act, bf16, 0.0)
+    _chk(lib.styler_groupnorm_act_bwd(args, ws.data_ptr(), n, _raw_stream(device.index)), "styler_groupnorm_act_bwd")
     return dx, dgamma, dbeta

@@ -936,6 +936,36 @@ def test_block_operators_on_another_stream(dev):
 
 
 @gpu
+def test_block_operators_make_their_device_current(dev, monkeypatch):
+    """Called with another device current: the call is made again with the tensors' own, with every argument."""
+    from styler_amd import ops
+    q, k, v, do = attention_case(dev, 2, 20, 30, 4, 2, 64, torch.float32)
+    x, dy, gamma, beta = gn_case(dev, 2, 40, 64, torch.float32)
+    lens, q_lens, gl = (torch.tensor(t, device=dev) for t in ([30, 11], [7, 20], [33, 40]))
+    mask = torch.arange(30, device=dev)[None] == 4
+    f = ops.rotary_freqs(64, dev)
+    pos = torch.arange(20, device=dev).float() * 0.7
+
+    def calls():
+        lse, stats = torch.empty(2, 4, 20, device=dev), torch.empty(2, 4, 2, device=dev)
+        out = ops.cross_attention(q, k, v, lens, q_lens=q_lens, mask=mask, scale=0.2, out=torch.empty_like(q), lse=lse)
+        return [out, lse, *ops.cross_attention_bwd(q, k, v, out, do, lse, lens, q_lens=q_lens, mask=mask, scale=0.2),
+                ops.rotary(q, f, pos, interleaved=True, gain=1.5, inverse=True, out=torch.empty_like(q)),
+                ops.groupnorm_act(x, gamma, beta, 4, ops.ACT_GELU, eps=0.1, lens=gl, out=torch.empty_like(x), stats=stats), stats,
+                *ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, 4, ops.ACT_GELU, lens=gl)]
+
+    want, real, turn = calls(), ops._current_device, [0]
+
+    def other_first():
+        turn[0] += 1
+        return -1 if turn[0] % 2 else real()
+
+    monkeypatch.setattr(ops, "_current_device", other_first)
+    got = calls()
+    assert turn[0] == 10 and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
 def test_block_operators_past_32_bit_offsets(dev):
     """Tensors of more than 2^31 elements: what stands at their end is what is read and written."""
     from styler_amd import ops
