@@ -5,7 +5,7 @@
 //   backward: dz = dy act'(z);  dbeta = sum dz, dgamma = sum dz xh;  with d = dz gamma and the group's means m1 = mean d,
 //   m2 = mean d xh:  dx = rstd (d - m1 - xh m2)
 //
-// Bound by memory.  Two forms (16 x 1000 x 320 bf16, fused: 11 us forward, 17 + 2 backward, one generation of blocks each; 8 x 16384 x
+// Bound by memory.  Two forms (16 x 1000 x 320 bf16, fused: 11 us forward, 14 + 2 backward, one generation of blocks each; 8 x 16384 x
 // 512 fp32, split: 61 + 7 + 86 us forward, 119 + 7 + 137 backward, i.e. 5.1 TB/s over what the two passes move):
 //   * fused: a block owns a slab of whole groups of one item and keeps its values in registers between the statistics and the
 //     output, so x (and dy) is read once;
@@ -281,15 +281,16 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
       s[j] = 0.f;
       q[j] = 0.f;
     }
+    float dz[IT][V];                                     // kept for the output: formed again there, 18.1 us instead of 16.2 (16 x 1000 x 320)
 #pragma unroll
     for (int i = 0; i < IT; ++i)
       if (on && rl + i * RL < n) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float xh = (xr[i].get(j) - S[j]) * R[j];
-          const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
-          s[j] += dz;
-          q[j] = fmaf(dz, xh, q[j]);
+          dz[i][j] = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
+          s[j] += dz[i][j];
+          q[j] = fmaf(dz[i][j], xh, q[j]);
         }
       }
     col_sums<V, T>(s, q, red, sa, sb, cv, RL, on);
@@ -316,8 +317,7 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xh = (xr[i].get(j) - S[j]) * R[j];
-        const float dz = gr[i].get(j) * act_slope<ACT>(fmaf(xh, ga[j], be[j]));
-        y[j] = t < n ? R[j] * (mul_rounded(dz, ga[j]) - m1[j] - xh * m2[j]) : 0.f;
+        y[j] = t < n ? R[j] * (mul_rounded(dz[i][j], ga[j]) - m1[j] - xh * m2[j]) : 0.f;
       }
       put<B16, V>(a.out, o0 + t * a.ol, y);
     }
@@ -566,14 +566,15 @@ GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
   p.v = v;
   // fused: a slab is whole groups and whole pieces, a memory line (128 bytes) wide where that gives 128 blocks, else down to 32
   // bytes (the lines that slabs share are then shared in one XCD's cache).  16 x 1000 x 320 bf16, forward / backward: 80 blocks
-  // 13.7 / 16.6 us, 160 blocks 11.0 / 16.6, 320 blocks 13.3 / 23.5
+  // 13.7 / 16.3 us, 160 blocks 10.7 / 16.2, 320 blocks 12.9 / 22.8.  Blocks of 256 threads first, several of which share a CU: 12 x
+  // 300 x 768 bf16, 384 blocks of 256 9.5 / 14.1, 132 blocks of 1024 10.9 / 17.6
   const int64_t unit = (int64_t)cg / gcd(cg, v) * v;
-  for (int line = 128; line >= 32 && !p.fused; line >>= 1) {
-    int64_t slab = unit * ((line / es + unit - 1) / unit);
-    if (slab > C) slab = C;
-    const int64_t cv = slab / v, slabs = (C + slab - 1) / slab;
-    if (line > 32 && B * slabs < 128 && slab > unit) continue;
-    for (int T = 256; T <= 1024 && !p.fused; T *= 4) {
+  for (int T = 256; T <= 1024 && !p.fused; T *= 4)
+    for (int line = 128; line >= 32 && !p.fused; line >>= 1) {
+      int64_t slab = unit * ((line / es + unit - 1) / unit);
+      if (slab > C) slab = C;
+      const int64_t cv = slab / v, slabs = (C + slab - 1) / slab;
+      if (line > 32 && B * slabs < 128 && slab > unit) continue;
       if (cv > T || slab > 1024) continue;
       const int64_t it = (L + T / cv - 1) / (T / cv);
       if (it <= (T == 256 ? 4 : it_max(bf16 != 0, v, bwd))) {
@@ -584,7 +585,6 @@ GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {
         p.slabs = (int)slabs;
       }
     }
-  }
   if (p.fused) return p;
   const int wide = 256 * v;
   p.slab = C < wide ? C : wide;
