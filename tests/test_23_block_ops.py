@@ -215,7 +215,7 @@ def test_cross_attention_long_masks(dev, B, Lq, Lk, H, G, D, shared, dtype):
 @gpu
 @pytest.mark.parametrize("B,Lq,Lk,H,G,D,dtype", [
     (5, 1100, 2101, 16, 8, 32, torch.bfloat16), (16, 2050, 2200, 2, 2, 32, torch.bfloat16),
-    (2, 2050, 4097, 4, 2, 64, torch.bfloat16), (8, 1030, 1025, 8, 8, 64, torch.bfloat16),
+    (2, 2100, 8200, 4, 4, 32, torch.bfloat16), (2, 2050, 4097, 4, 2, 64, torch.bfloat16), (8, 1030, 1025, 8, 8, 64, torch.bfloat16),
     (2, 1100, 4200, 4, 4, 128, torch.bfloat16), (9, 1000, 530, 8, 8, 80, torch.bfloat16),
     (5, 1100, 2101, 4, 2, 32, torch.float32), (3, 600, 1500, 8, 4, 64, torch.float32), (2, 300, 6000, 2, 2, 72, torch.float32),
 ])
@@ -226,6 +226,7 @@ def test_cross_attention_masked_keys_are_left_out(dev, B, Lq, Lk, H, G, D, dtype
     r = lambda *s: torch.randn(*s, generator=g, device=dev).to(dtype)
     q, kv, do = r(B, Lq, H, D), r(B, Lk, 2, G, D), r(B, Lq, H, D)
     mask = torch.rand(B, Lk, generator=g, device=dev) < torch.linspace(0.1, 0.9, B, device=dev)[:, None]
+    mask[1] = True                                            # an item without keys
     lens = torch.full((B,), Lk - 5, device=dev)
     seen = ~mask & (torch.arange(Lk, device=dev)[None] < lens[:, None])
     order = torch.argsort((~seen).int(), dim=1, stable=True)
