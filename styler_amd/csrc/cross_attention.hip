@@ -1252,20 +1252,24 @@ struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; bool order; };
 // Sizes alone decide.  512 blocks are two per CU, and shares are cut to reach that (2 x 65537 keys of one token: 256 blocks, one per CU,
 // 110 us, 512 113, 1024 118).  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
 // 81 us (every share writes its part once more); two key groups from 512 blocks of 128 rows down: 8 x 500 x 700 49 us, from 1024: the
-// fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).  fp32 with more than 64 rows a key head goes through
-// planes (their making pays from there on); with fewer it is bound by reading the keys, which planes would do twice.
+// fp32 forward at 608 blocks 137 -> 155 us (each row of blocks reads all keys).
+// fp32 goes through planes where their making (10 bytes of traffic a value, a launch) pays, the fp32 instruction / planes: forward 15 x
+// 8 heads of 128, 378 keys, 70 rows 54 / 66 us, 130 rows 71 / 79, 260 rows 104 / 98; 8 x 4 heads of 64, 2000 keys, 200 rows 48.5 / 48.9,
+// 400 rows 109 / 70; backward, with the same planes for two kernels more, 15 x 8 x 378 x 128, 70 rows 151 / 142, 8 x 4 x 2000 x 64, 100
+// rows 83 / 77; but 30 x 8 heads of 64, 60 keys, 100 rows (9e7 rows x keys x width) 35 / 45, 2 x 4 x 300 x 64, 400 rows (6e7) 50 / 57.
+constexpr double PLANES_FROM = 1 << 27;
 // A mask's keys are put in order from here on (rows x keys x width, six times that with planes): the ordering is a launch of 3 us.
 // One key in four dropped, without / with it, at 1.4e9 (8 x 8 heads x 500 x 700 x 64) 16.5 / 19.1 us, at 4.3e9 (8 x 8 x 1024 x 1024 x
 // 64) 28.5 / 28.1 and 107 / 102 (training), at 5.9e9 (4 x 8 x 1024 x 1400 x 128) 37 / 36, at 5.5e9 in planes 171 / 162.  (The rows
 // that a mask leaves out are zeros in the tiles otherwise: they cost the product, but little power.)
 constexpr double ORDER_FROM = 4294967296.;
-Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
+Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16, bool bwd) {
   Plan p;
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
   p.width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
-  p.planes = !bf16 && M > 64 ? 3 : 1;
+  p.planes = !bf16 && M > (bwd ? 64 : 192) && (double)BG * M * Lk * p.width >= PLANES_FROM ? 3 : 1;
   const int row = p.width * (bf16 || p.planes == 3 ? 2 : 4) * p.planes;
-  p.kg = p.planes == 3 ? 1 : M <= 32 ? 4 : M <= 64 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
+  p.kg = p.planes == 3 ? 1 : M <= 32 ? 4 : M <= 64 || !bf16 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
   const int rows = 128 / p.kg;
   p.nrt = (int)((M + rows - 1) / rows);
   const int KT = 32 * p.kg * (p.kg == 1 && row <= 256 ? 2 : 1);
@@ -1277,7 +1281,7 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16) {
   p.dq = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 4 : 256 / KT);
   p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
-  p.order = M > 64 && (double)BG * M * Lk * p.width * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
+  p.order = M > 64 && (bf16 || p.planes == 3) && (double)BG * M * Lk * p.width * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
   const int RT = p.planes == 3 ? 32 : 64;
   p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), row >= 512 ? 256 : 512, 128 / RT);
   return p;
@@ -1356,7 +1360,7 @@ int check(const styler_xattn_t* x, bool bwd) {
   const void* p[] = {x->q, x->k, x->v, x->out, bwd ? x->dout : nullptr, bwd ? x->dq : nullptr, bwd ? x->dk : nullptr, bwd ? x->dv : nullptr};
   for (const void* q : p) if ((uintptr_t)q & 15) return STYLER_EALIGN;
   if (bwd && (!x->dout || !x->dq || !x->dk || !x->dv || !x->lse)) return STYLER_EINVAL;
-  const Plan pl = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  const Plan pl = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, bwd);
   const int64_t bg = (int64_t)x->B * x->G;
   // a launch has fewer than 2^32 threads, the padding of the runs (grid_for: one eighth at most) among them
   if (bg * pl.nrt * (pl.fwd > pl.dq ? pl.fwd : pl.dq) > 0xe00000 || (bwd && bg * pl.nkt * pl.dkv > 0xe00000)) return STYLER_EINVAL;
@@ -1377,7 +1381,7 @@ XArgs args(const styler_xattn_t* x) {
 
 extern "C" int64_t styler_cross_attention_workspace_bytes(int B, int Lq, int Lk, int H, int G, int D, int bf16, int masked, int bwd) {
   if (B < 1 || Lq < 1 || Lk < 1 || G < 1 || H < G || H % G || D < 8 || D > 128) return 0;
-  const Plan p = make_plan(B, Lq, Lk, H, G, D, bf16);
+  const Plan p = make_plan(B, Lq, Lk, H, G, D, bf16, bwd != 0);
   const int64_t qrows = (int64_t)B * H * Lq, krows = (int64_t)B * G * Lk;
   const int64_t kv = 2 * plane_bytes(p, B, Lk, G) + (masked ? order_bytes(p, B, Lk) : 0);
   if (!bwd) return (p.fwd > 1 ? (4 * p.fwd * qrows * (D + 2) + 15) / 16 * 16 : 0) + kv;
@@ -1430,7 +1434,7 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
   if (const int rc = check(x, false)) return rc;
   const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, x->mask != nullptr, 0);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return STYLER_EINVAL;
-  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, false);
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   a.nrt = p.nrt; a.splits = p.fwd; a.part = p.fwd > 1 ? (float*)workspace : nullptr;
@@ -1460,7 +1464,7 @@ extern "C" int styler_cross_attention_bwd(const styler_xattn_t* x, void* workspa
   if (const int rc = check(x, true)) return rc;
   const int64_t need = styler_cross_attention_workspace_bytes(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, x->mask != nullptr, 1);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return STYLER_EINVAL;
-  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16);
+  const Plan p = make_plan(x->B, x->Lq, x->Lk, x->H, x->G, x->D, x->bf16, true);
   hipStream_t st = (hipStream_t)stream;
   XArgs a = args(x);
   const int64_t qrows = (int64_t)x->B * x->H * x->Lq, krows = (int64_t)x->B * x->G * x->Lk;

@@ -130,6 +130,8 @@ def test_cross_attention_against_definition(dev, B, Lq, Lk, H, G, D, dtype):
     (3, 530, 500, 2, 1, 32, [500, 3, 260], [530, 530, 100]),              # long ragged items: the most work first
     (4, 600, 450, 1, 1, 128, [17, 0, 450, 450], [600, 1, 0, 599]),
     (5, 520, 510, 2, 2, 80, [510, 64, 65, 1, 509], [1, 520, 519, 520, 0]),
+    (4, 1100, 1000, 1, 1, 32, [1000, 33, 0, 999], [1100, 1099, 5, 64]),   # (fp32: through planes from here on)
+    (3, 1030, 1020, 2, 2, 64, [1020, 640, 31], [1030, 0, 1]),
     (3, 1, 5000, 4, 1, 64, [5000, 3, 0], None),                           # shares of which some see nothing
     (3, 2, 4097, 16, 4, 128, [4097, 4096, 65], [2, 1, 2]),
     (2, 9, 1500, 8, 1, 32, [1500, 700], None),                            # 72 rows of one key head
