@@ -1248,6 +1248,22 @@ int split_count(int64_t blocks, int64_t n, int64_t want, int64_t least) {
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : (int)s;
 }
+// The same for blocks of 64 and 128 rows, whose shares write (and the join reads) whole tiles of partial results: the count with the
+// least expected time, in us -- tile_us a tile of the share, more where blocks wait for a CU (LDS holds one block) or share it (two
+// blocks take 1.4 times one's time together), 4 for the launch of the join and 0.8 a MB of partial results.  Measured at 1 / 2 / 4 / 8 shares: 29 x 8 heads of 128, 54 rows x
+// 451 keys 17 / 26 / 32 / 47 us, 16 x 8 heads of 64, 60 x 2000 28 / 25 / 23 / 25, 4 x 8 x 64, 60 x 4000 48 / 31 / 21 / 17, 2 x 4 x
+// 128, 1000 x 4000 62 / 43 / 35 / 45, fp32 3 x 4 x 64, 400 x 2000 106 / 67 / 46 / 40.
+int share_count(int64_t blocks, int64_t n, int at_once, double tile_us, double part_mb) {
+  static const int counts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  int best = 1;
+  double least = 1e30;
+  for (const int s : counts) {
+    if (s > n) break;
+    const double load = (double)blocks * s / (at_once == 256 ? 256 : 366), t = (double)((n + s - 1) / s) * tile_us * (load > 1 ? load : 1) + (s > 1 ? 4 + 0.8 * part_mb * s : 0);
+    if (t < least) { least = t; best = s; }
+  }
+  return best;
+}
 struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; bool order; };
 // Sizes alone decide.  512 blocks are two per CU, and shares are cut to reach that (2 x 65537 keys of one token: 256 blocks, one per CU,
 // 110 us, 512 113, 1024 118).  48 x 1000 x 133 bf16 training with shares for 512 / 1024 / 2048 blocks: 74 / 79 /
@@ -1277,8 +1293,15 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16, bool bwd) {
   const int want = row >= 512 || (p.kg == 4 && row >= 256) ? 256 : 512;        // (LDS holds one block of these per CU)
   // (a token over under eight tiles of up to 32 KB is one share: the join is a launch more, 4 us of the host's time.  700 keys of 64 bf16
   // features, shared out / not: 32 x 4 heads 14 / 10 us a call, 10.1 / 8.9 in a graph; 8 x 4 heads 13.5 / 10.9, 9.6 / 10.5)
-  p.fwd = p.kg == 4 && row <= 128 && kt < 8 ? 1 : split_count(BG * p.nrt, kt, want, p.kg == 4 ? 2 : 128 / KT);
-  p.dq = split_count(BG * p.nrt, kt, want, p.kg == 4 ? 4 : 256 / KT);
+  if (p.kg == 4) {
+    p.fwd = row <= 128 && kt < 8 ? 1 : split_count(BG * p.nrt, kt, want, 2);
+    p.dq = split_count(BG * p.nrt, kt, want, 4);
+  } else {
+    // a tile's two products (the gradient's three) at a CU's share of the matrix rate, 4.5 or 0.6 TFLOP/s, and what is not overlapped
+    const double us = 4e-6 * rows * KT * p.width * (p.planes == 3 ? 6 : 1) / (bf16 || p.planes == 3 ? 4.5 : 0.6), mb = 4e-6 * BG * M * D;
+    p.fwd = share_count(BG * p.nrt, kt, want, 0.4 + 1.15 * us, mb);
+    p.dq = share_count(BG * p.nrt, kt, want, 0.4 + 1.7 * us, mb);
+  }
   p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
   p.order = M > 64 && (bf16 || p.planes == 3) && (double)BG * M * Lk * p.width * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
