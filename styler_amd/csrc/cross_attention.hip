@@ -33,6 +33,10 @@
 
 namespace {
 
+// Heads are padded to DT = 32, 64, 96 or 128 features; LDS rows are powers of two wide (banks, DMA).  96 leaves out a quarter of the
+// products of 128 (heads of 80: training 8 x 16 heads, 2048 x 1500 bf16 890 -> 755 us, 11 x 2, 1059 x 699 fp32 254 -> 218; forward 4 x 16 /
+// 4, 4096 x 4096 bf16 470 -> 420).
+constexpr int stored(int dt) { return dt == 96 ? 128 : dt; }
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
@@ -257,7 +261,7 @@ __device__ __forceinline__ void zero16(f32x16& a) {
 // s[32 tile rows][32 lane rows] += tile(rows blk * 32 ..) . lane rows      (TS: bytes from plane to plane of the tile)
 template <typename T, int DT, int NP, int TS, bool SWAP = false>
 __device__ __forceinline__ void mma_rows(f32x16& s, const char* tile, int blk, const Rows<T, DT, NP>& f, int li, int lh) {
-  constexpr int RB = DT * sizeof(T);
+  constexpr int RB = stored(DT) * sizeof(T);
   const char* row = tile + (blk * 32 + li) * RB;
   const uint32_t x = (lh ^ Swz<RB>::of(li)) * 16;
   if constexpr (NP == 3) {
@@ -330,7 +334,7 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& a, int s2) {
 // rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain; planes: split like the operands)
 template <typename T, int DT, int NP, int TS>
 __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* tile, int blk, const f32x16& p, int lane) {
-  constexpr int RB = DT * sizeof(T);
+  constexpr int RB = stored(DT) * sizeof(T);
   const int li = lane & 31, lh = lane >> 5;
   if constexpr (sizeof(T) == 2) {
     const int tq = lane & 15, tc = (lane >> 4) & 1, r0 = lh * 4 + (tq >> 2);
@@ -411,7 +415,7 @@ __device__ __forceinline__ void store_zero(T* row, int D, int lh) {
 // keep = false store zeros (whatever their accumulators hold).
 template <typename To, int DT, typename At>
 __device__ __forceinline__ void store_tile(char* lds, const f32x16 (&acc)[DT / 32], int D, int lane, float c, bool keep, At at) {
-  constexpr int RB = DT * sizeof(To), LPR = RB / 16, RPI = 64 / LPR;         // lanes per row, rows per instruction
+  constexpr int RB = stored(DT) * sizeof(To), LPR = RB / 16, RPI = 64 / LPR;       // lanes per row, rows per instruction
   const int li = lane & 31, lh = lane >> 5;
 #pragma unroll
   for (int dt = 0; dt < DT / 32; ++dt)
@@ -509,11 +513,11 @@ __device__ __forceinline__ void mma_rows_seen(f32x16& s, const char* tile, int b
 // at most 32 of them, 2 between (and where blocks of 128 rows would be too few, or too uneven, to fill it).  A tile holds NB blocks
 // of 32 keys for each key group: two where two tiles of K and V fit in 64 KB (two blocks a CU), so that the softmax's bookkeeping is
 // shared by 64 keys.
-template <typename T, int DT, int KG, int NP> constexpr int key_blocks() { return KG == 1 && DT * sizeof(T) * NP <= 256 ? 2 : 1; }
+template <typename T, int DT, int KG, int NP> constexpr int key_blocks() { return KG == 1 && stored(DT) * sizeof(T) * NP <= 256 ? 2 : 1; }
 
 // Waves per SIMD to ask registers for: `most` where rows are shared out alone, as far as LDS lets them in; two with key groups.
 template <typename T, int DT, int KG, int NP> constexpr int waves_wanted(int most) {
-  return DT * sizeof(T) * NP >= 512 || (KG == 4 && DT * sizeof(T) >= 256) ? 1 : (KG == 1 ? most : 2);
+  return stored(DT) * sizeof(T) * NP >= 512 || (KG == 4 && stored(DT) * sizeof(T) >= 256) ? 1 : (KG == 1 ? most : 2);
 }
 template <typename T, int NP> struct OutOf { typedef T type; };
 template <typename T> struct OutOf<T, 3> { typedef float type; };
@@ -538,14 +542,14 @@ template <int KG, int LDO> __device__ __forceinline__ float4 group_sum(const flo
 
 // ------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DT, int KG, int NP, bool PICK>
-__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : DT * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : stored(DT) * sizeof(T) <= 128 ? 4 : 2))) void xattn_fwd_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
-  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
+  constexpr int RB = stored(DT) * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
   constexpr int TS = KT * RB, TILE = NP * TS;            // a plane of a tile, a tile
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int LDO = DT + 4;                            // rows of the join start 4 banks apart
   constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
-  static_assert(KG > 1 || 4 * 32 * DT * 4 <= SMEM, "");
+  static_assert(KG > 1 || 4 * 32 * stored(DT) * 4 <= SMEM, "");
   __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (KG > 1 ? 1280 : 0)];
   float* start = reinterpret_cast<float*>(smem + SMEM);          // [buffer][KT], see start_put
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
@@ -684,12 +688,12 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : DT 
   if constexpr (KG == 1) {
     const int mw = m0 + wave * 32;
     if (a.splits > 1) {
-      store_tile<float, DT>(smem + wave * 32 * DT * 4, o, a.D, lane, 1.f, true, [&](int r) {
+      store_tile<float, DT>(smem + wave * 32 * stored(DT) * 4, o, a.D, lane, 1.f, true, [&](int r) {
         return mw + r < M ? a.part + (sp * prows + (int64_t)bg * M + mw + r) * a.D : nullptr;
       });
       if (lh == 0 && m < M) { pml[0] = m2; pml[1] = l; }
     } else {
-      store_tile<O, DT>(smem + wave * 32 * DT * sizeof(O), o, a.D, lane, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), true, [&](int r) {
+      store_tile<O, DT>(smem + wave * 32 * stored(DT) * sizeof(O), o, a.D, lane, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), true, [&](int r) {
         return mw + r < M ? reinterpret_cast<O*>(a.out) + b * a.ob + (mw + r) / a.R * a.ol + (g * a.R + (mw + r) % a.R) * a.oh : nullptr;
       });
       if (a.lse && lh == 0 && m < M) a.lse[((int64_t)b * a.H + head) * a.Lq + qi] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * LN2;
@@ -798,14 +802,14 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // delta + sum_j P_j (do . v_j - delta) instead: the exact sum, at the price of the tile's products once more.  (0 stays 0 where one
 // key is seen.)
 template <typename T, int DT, int KG, int NP, bool PICK>
-__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored(DT) * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
-  constexpr int RB = DT * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
+  constexpr int RB = stored(DT) * sizeof(T), RG = 4 / KG, NB = key_blocks<T, DT, KG, NP>(), KT = 32 * KG * NB;
   constexpr int TS = KT * RB, TILE = NP * TS;
   constexpr int NBUF = 4 * TILE <= 131072 ? 2 : 1;
   constexpr int LDO = DT + 4;
   constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
-  static_assert(KG > 1 || 4 * 32 * DT * 4 <= SMEM, "");
+  static_assert(KG > 1 || 4 * 32 * stored(DT) * 4 <= SMEM, "");
   __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (KG > 1 ? 512 : 0)];
   float* start = reinterpret_cast<float*>(smem + SMEM);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
@@ -942,11 +946,11 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && DT * s
   if constexpr (KG == 1) {
     const int mw = m0 + wave * 32;
     if (a.splits > 1)
-      store_tile<float, DT>(smem + wave * 32 * DT * 4, dq, a.D, lane, a.scale, true, [&](int r) {
+      store_tile<float, DT>(smem + wave * 32 * stored(DT) * 4, dq, a.D, lane, a.scale, true, [&](int r) {
         return mw + r < M ? a.part + (sp * prows + (int64_t)bg * M + mw + r) * a.D : nullptr;
       });
     else
-      store_tile<O, DT>(smem + wave * 32 * DT * sizeof(O), dq, a.D, lane, a.scale, true, [&](int r) {
+      store_tile<O, DT>(smem + wave * 32 * stored(DT) * sizeof(O), dq, a.D, lane, a.scale, true, [&](int r) {
         return mw + r < M ? reinterpret_cast<O*>(a.dq) + (((int64_t)b * a.Lq + (mw + r) / a.R) * a.H + g * a.R + (mw + r) % a.R) * a.D : nullptr;
       });
   } else {
@@ -1000,12 +1004,12 @@ template <int N> __device__ __forceinline__ void add_from(f32x16 (&acc)[N], char
 // The block walks tiles of 64 query rows (32 of planes), head after head of the group; with KW = 2 two waves share the keys and each takes half of
 // a tile's rows.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen key computes
 // stays in its own lane; zeros are stored for it.
-template <typename T, int DT, int NP> constexpr int DKV_UNROLL = DT * sizeof(T) * NP >= 256 ? 1 : 2;        // (twice the registers spill)
+template <typename T, int DT, int NP> constexpr int DKV_UNROLL = stored(DT) * sizeof(T) * NP >= 256 ? 1 : 2;        // (twice the registers spill)
 template <typename T, int DT, int KW, int NP>
-__global__ __launch_bounds__(256, (DT * sizeof(T) * NP >= 512 ? 1 : DT * sizeof(T) * NP >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
+__global__ __launch_bounds__(256, (stored(DT) * sizeof(T) * NP >= 512 ? 1 : stored(DT) * sizeof(T) * NP >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
-  constexpr int RB = DT * sizeof(T), RT = NP == 3 ? 32 : 64, TS = RT * RB, TILE = NP * TS, RW = 4 / KW, NBLK = RT / 32 / RW;
-  constexpr int SHARE = 32 * DT * 4;                     // LDS of a wave for its results, once the tiles are done with
+  constexpr int RB = stored(DT) * sizeof(T), RT = NP == 3 ? 32 : 64, TS = RT * RB, TILE = NP * TS, RW = 4 / KW, NBLK = RT / 32 / RW;
+  constexpr int SHARE = 32 * stored(DT) * 4;             // LDS of a wave for its results, once the tiles are done with
   static_assert(NBLK >= 1 && 4 * SHARE <= 4 * TILE, "");
   constexpr int STAT = 4 * TILE;                         // [buf][lse2 | delta][64]
   __shared__ __attribute__((aligned(1024))) char smem[STAT + 2 * 512];
@@ -1274,7 +1278,7 @@ struct Plan { int planes, width, kg, nrt, fwd, dq, kw, nkt, dkv; bool order; };
 // 400 rows 109 / 70; backward, with the same planes for two kernels more, 15 x 8 x 378 x 128, 70 rows 151 / 142, 8 x 4 x 2000 x 64, 100
 // rows 83 / 77; but 30 x 8 heads of 64, 60 keys, 100 rows (9e7 rows x keys x width) 35 / 45, 2 x 4 x 300 x 64, 400 rows (6e7) 50 / 57.
 constexpr double PLANES_FROM = 1 << 27;
-// A mask's keys are put in order from here on (rows x keys x width, six times that with planes): the ordering is a launch of 3 us.
+// A mask's keys are put in order from here on (rows x keys x width of an LDS row, six times that with planes): the ordering is a launch of 3 us.
 // One key in four dropped, without / with it, at 1.4e9 (8 x 8 heads x 500 x 700 x 64) 16.5 / 19.1 us, at 4.3e9 (8 x 8 x 1024 x 1024 x
 // 64) 28.5 / 28.1 and 107 / 102 (training), at 5.9e9 (4 x 8 x 1024 x 1400 x 128) 37 / 36, at 5.5e9 in planes 171 / 162.  (The rows
 // that a mask leaves out are zeros in the tiles otherwise: they cost the product, but little power.)
@@ -1282,9 +1286,9 @@ constexpr double ORDER_FROM = 4294967296.;
 Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16, bool bwd) {
   Plan p;
   const int64_t M = (int64_t)Lq * (H / G), BG = (int64_t)B * G;
-  p.width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+  p.width = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
   p.planes = !bf16 && M > (bwd ? 64 : 192) && (double)BG * M * Lk * p.width >= PLANES_FROM ? 3 : 1;
-  const int row = p.width * (bf16 || p.planes == 3 ? 2 : 4) * p.planes;
+  const int row = stored(p.width) * (bf16 || p.planes == 3 ? 2 : 4) * p.planes;
   p.kg = p.planes == 3 ? 1 : M <= 32 ? 4 : M <= 64 || !bf16 || BG * ((M + 127) / 128) < 512 ? 2 : 1;
   const int rows = 128 / p.kg;
   p.nrt = (int)((M + rows - 1) / rows);
@@ -1304,7 +1308,7 @@ Plan make_plan(int B, int Lq, int Lk, int H, int G, int D, int bf16, bool bwd) {
   }
   p.kw = p.planes == 1 && BG * ((Lk + 127) / 128) < 512 ? 2 : 4;
   p.nkt = (Lk + 32 * p.kw - 1) / (32 * p.kw);
-  p.order = M > 64 && (bf16 || p.planes == 3) && (double)BG * M * Lk * p.width * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
+  p.order = M > 64 && (bf16 || p.planes == 3) && (double)BG * M * Lk * stored(p.width) * (p.planes == 3 ? 6 : 1) >= ORDER_FROM;
   const int RT = p.planes == 3 ? 32 : 64;
   p.dkv = split_count(BG * p.nkt, (int64_t)((Lq + RT - 1) / RT) * (H / G), row >= 512 ? 256 : 512, 128 / RT);
   return p;
@@ -1365,6 +1369,7 @@ void launch_dkv(XArgs& a, const Plan& p, hipStream_t st) {
   do {                                 \
     if (a.D <= 32) { CALL(T, 32); }    \
     else if (a.D <= 64) { CALL(T, 64); } \
+    else if (a.D <= 96) { CALL(T, 96); } \
     else { CALL(T, 128); }             \
   } while (0)
 
@@ -1476,7 +1481,7 @@ extern "C" int styler_cross_attention(const styler_xattn_t* x, void* workspace, 
 #undef FWD
   if (p.fwd > 1) {
     const unsigned blocks = (unsigned)(((int64_t)x->B * x->H * x->Lq + 3) / 4);
-#define JOIN(T, W) hipLaunchKernelGGL((xattn_join_kernel<T, W>), dim3(blocks), dim3(256), 0, st, a)
+#define JOIN(T, W) hipLaunchKernelGGL((xattn_join_kernel<T, stored(W)>), dim3(blocks), dim3(256), 0, st, a)
     if (x->bf16) BY_WIDTH(uint16_t, JOIN); else BY_WIDTH(float, JOIN);
 #undef JOIN
   }
