@@ -5,7 +5,7 @@
 //   backward: dz = dy act'(z);  dbeta = sum dz, dgamma = sum dz xh;  with d = dz gamma and the group's means m1 = mean d,
 //   m2 = mean d xh:  dx = rstd (d - m1 - xh m2)
 //
-// Bound by memory.  Two forms (16 x 1000 x 320 bf16, fused: 11 us forward, 14 + 2 backward, one generation of blocks each; 8 x 16384 x
+// Bound by memory.  Two forms (16 x 1000 x 320 bf16, fused: 11 us forward, 15 + 2 backward, one generation of blocks each; 8 x 16384 x
 // 512 fp32, split: 61 + 7 + 86 us forward, 119 + 7 + 137 backward, i.e. 5.1 TB/s over what the two passes move):
 //   * fused: a block owns a slab of whole groups of one item and keeps its values in registers between the statistics and the
 //     output, so x (and dy) is read once;
