@@ -62,7 +62,7 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
   return z > 0.f ? 1.f - h : h;
 }
 template <int ACT> __device__ __forceinline__ float act_of(float z) {
-  if constexpr (ACT == STYLER_ACT_RELU) return fmaxf(z, 0.f);
+  if constexpr (ACT == STYLER_ACT_RELU) return z < 0.f ? 0.f : z;        // (a maximum would turn NaN into 0)
   if constexpr (ACT == STYLER_ACT_SILU) return z * sigmoid(z);
   if constexpr (ACT == STYLER_ACT_GELU) { float e; return z * normal_cdf(z, e); }
   return z;

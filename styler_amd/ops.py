@@ -2150,7 +2150,7 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     """act(GroupNorm(x)) over channels-last x [B, L, C] (fp32 or bf16), `groups` groups of C / groups channels, gamma and beta fp32
     [C], act one of ACT_NONE / ACT_RELU / ACT_SILU / ACT_GELU.  lens int64 [B]: the statistics cover the rows before it, rows at or
     past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
-    groupnorm_act_bwd.  out (optional) may be x."""
+    groupnorm_act_bwd.  A NaN or an infinity in a group's rows makes the group NaN.  out (optional) may be x."""
     name = "groupnorm_act"
     if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel():
         _refuse(name, "out shares memory with x in another layout")

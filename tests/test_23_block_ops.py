@@ -1040,6 +1040,60 @@ def test_groupnorm_act_of_many_items(dev):
             assert float(((got.double() - ref).abs() / (size + 1e-3)).max()) <= B * half_step(torch.float32) * 0.5
 
 
+# ------------------------------------------------------------------------------------------------------------ values that are not finite
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("L", [60, 3000])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+def test_groupnorm_act_shows_values_that_are_not_finite(dev, act, L, dtype):
+    """A NaN or an infinity among a group's valid rows makes the group NaN, forward and backward, whatever the activation; the other
+    groups and items are what they are without it."""
+    from styler_amd import ops
+    x, dy, gamma, beta = gn_case(dev, 3, L, 64, dtype, seed=17)
+    lens = torch.tensor([L, L - 7, L], device=dev)
+
+    def both(x):
+        stats = torch.empty(3, 4, 2, device=dev)
+        y = ops.groupnorm_act(x, gamma, beta, 4, ACTS[act], lens=lens, stats=stats)
+        return (y, *ops.groupnorm_act_bwd(x, dy, gamma, beta, stats, 4, ACTS[act], lens=lens))
+
+    ref = both(x)
+    for bad in (math.nan, math.inf, -math.inf):
+        x2 = x.clone()
+        x2[1, L // 3, 21] = bad                               # group 1 of item 1
+        got = both(x2)
+        for a, b in zip(got[:2], ref[:2]):
+            a = a.clone()
+            assert bool(a[1, :L - 7, 16:32].isnan().all()), (bad, act)
+            a[1, :L - 7, 16:32] = b[1, :L - 7, 16:32]
+            assert torch.equal(a, b)
+        assert bool(got[2][16:32].isnan().all())              # dgamma
+        for a, b in zip(got[2:], ref[2:]):
+            assert torch.equal(a[:16], b[:16]) and torch.equal(a[32:], b[32:])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("L", [60, 3000])
+@pytest.mark.parametrize("groups", [4, 64])
+def test_groupnorm_act_of_a_variance_past_the_range(dev, groups, L, dtype):
+    """Squares that leave the range of 32 bits make the variance infinite: 1 / sqrt(inf) = 0, so y = act(beta) and dx = 0."""
+    from styler_amd import ops
+    C, cg = 64, 64 // groups
+    x, dy, gamma, beta = gn_case(dev, 2, L, C, dtype, seed=18)
+    g = torch.Generator().manual_seed(1)
+    x2 = x.clone()
+    x2[1, :, :cg] = (1e20 * torch.randn(L, cg, generator=g)).to(dtype).to(dev)
+    stats, clean = (torch.empty(2, groups, 2, device=dev) for _ in range(2))
+    y, ref = ops.groupnorm_act(x2, gamma, beta, groups, stats=stats), ops.groupnorm_act(x, gamma, beta, groups, stats=clean)
+    assert not stats[1, 0, 1].any() and torch.equal(stats[1, 1:], clean[1, 1:]) and torch.equal(stats[0], clean[0])
+    want = beta[:cg].double() * torch.sigmoid(beta[:cg].double())
+    within(y[1, :, :cg].cpu(), want.cpu().expand(L, cg), (half_step(dtype) + 8 * U32) * want.abs().cpu().expand(L, cg) + 1e-30, "y")
+    assert torch.equal(y[1, :, cg:], ref[1, :, cg:]) and torch.equal(y[0], ref[0])
+    dx, dgamma, dbeta = ops.groupnorm_act_bwd(x2, dy, gamma, beta, stats, groups)
+    assert not dx[1, :, :cg].any() and bool(dgamma.isfinite().all()) and bool(dbeta.isfinite().all())
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
