@@ -798,9 +798,65 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // Same walk as the forward; P is rebuilt from lse.  A row without keys has lse = -inf: it takes +inf here, every P is 0.
 //
 // delta = do . o is off by the rounding of a bf16 o, which weighs where a query sees a few keys (o is as large as a value then, and
-// the scores' gradient a difference of few terms: 3 keys gave dq an error of 0.0037, 100 keys 0.0024).  Items of up to 32 keys take
-// delta + sum_j P_j (do . v_j - delta) instead: the exact sum, at the price of the tile's products once more.  (0 stays 0 where one
-// key is seen.)
+// the scores' gradient a difference of few terms: 3 keys gave dq an error of 0.0037, 100 keys 0.0024).  Items of up to FEW seen keys,
+// by their length or by their mask, take delta + sum_j P_j (do . v_j - delta) instead: the exact sum.  Their keys are gathered into
+// one block of 32 tile rows for that, and every wave and share forms the sum by itself.  (0 stays 0 where one key is seen.)
+constexpr int FEW = 32;
+// 16 bytes of the mask from key k on; keys at or past klen count as dropped
+__device__ __forceinline__ uint4 mask16(const uint8_t* mask, int k, int klen) {
+  uint4 u;
+  if (__builtin_amdgcn_ballot_w64(k + 16 > klen) == 0) {
+    __builtin_memcpy(&u, mask + k, 16);
+  } else {
+    uint32_t m[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m[i] = k + i < klen ? mask[k + i] : 1;
+    u = make_uint4(m[0] | m[1] << 8 | m[2] << 16 | m[3] << 24, m[4] | m[5] << 8 | m[6] << 16 | m[7] << 24,
+                   m[8] | m[9] << 8 | m[10] << 16 | m[11] << 24, m[12] | m[13] << 8 | m[14] << 16 | m[15] << 24);
+  }
+  return u;
+}
+// bit 8 j + 7: byte j of x is zero
+__device__ __forceinline__ uint32_t zero_byte_bits(uint32_t x) { return ~(((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u; }
+// The number of seen keys, or FEW + 1 if they are more; where they are not, list[0 ..] receives their numbers (`put`: by this wave).
+// first: mask16 of the lane's first keys, fetched early: most masks are done after those, which costs the backward of 4 x 64 x 4096
+// keys half a us.  Then 8192 keys a step (2 x 8 rows, 65537 keys of which a mask leaves 3: 58 us with the sum, 46 without; 512 keys
+// a step 256).
+__device__ __forceinline__ int few_keys(const uint8_t* mask, const int* order, int klen, int lane, int* list, bool put, const uint4& first) {
+  if (!mask) {
+    if (klen <= FEW && put && lane < klen) list[lane] = order ? order[lane] : lane;
+    return klen <= FEW ? klen : FEW + 1;
+  }
+  int n = 0;
+  auto add = [&](const uint4& u, int k) {
+    const uint32_t z[4] = {zero_byte_bits(u.x), zero_byte_bits(u.y), zero_byte_bits(u.z), zero_byte_bits(u.w)};
+    const int mine = __builtin_popcount(z[0]) + __builtin_popcount(z[1]) + __builtin_popcount(z[2]) + __builtin_popcount(z[3]);
+    if (__builtin_amdgcn_ballot_w64(mine != 0) == 0) return;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += x;
+    }
+    const int before = n + upto - mine;
+    n += __builtin_amdgcn_readlane(upto, 63);
+    if (!put || n > FEW) return;
+    int at = before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      for (uint32_t x = z[i]; x; x &= x - 1) list[at++] = k + 4 * i + __builtin_ctz(x) / 8;
+  };
+  add(first, lane * 16);
+  for (int k0 = 1024; k0 < klen && n <= FEW; k0 += 8192) {
+    uint4 u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = mask16(mask, k0 + i * 1024 + lane * 16, klen);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n <= FEW) add(u[i], k0 + i * 1024 + lane * 16);
+  }
+  return n <= FEW ? n : FEW + 1;
+}
 template <typename T, int DT, int KG, int NP, bool PICK>
 __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored(DT) * sizeof(T) <= 128 ? 3 : 2))) void xattn_dq_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;
@@ -810,7 +866,9 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored
   constexpr int LDO = DT + 4;
   constexpr int JOIN = KG > 1 ? 4 * 32 * LDO * 4 : 0, SMEM = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
   static_assert(KG > 1 || 4 * 32 * stored(DT) * 4 <= SMEM, "");
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (KG > 1 ? 512 : 0)];
+  constexpr bool SUMS = NP == 1 && sizeof(T) == 2;       // (fp32: o is as good as the sums)
+  static_assert(!SUMS || NBUF == 2, "");                 // (the few keys are gathered into the second buffer)
+  __shared__ __attribute__((aligned(1024))) char smem[SMEM + 2 * KT * 4 + (SUMS ? FEW * 4 : 0)];
   float* start = reinterpret_cast<float*>(smem + SMEM);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
   const int rg = wave / KG, kg = wave % KG;
@@ -830,14 +888,13 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored
   load_rows(dof, a.dout, b * a.gb + qi * a.gl + head * a.gh, a.D, lh, live);
   load_rows(qf, a.o, b * a.ob + qi * a.ol + head * a.oh, a.D, lh, live);
   float dl = rows_dot(qf, dof, li, lh);
-  const bool few = NP == 1 && sizeof(T) == 2 && klen <= 32;
   if (live) {
     const float x = a.lse[srow];
     lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
   }
   if (sp == 0 && m < M && lh == 0 && kg == 0) {
     a.lse2[srow] = lse2;
-    if (!few) a.delta[srow] = dl;
+    if (!SUMS) a.delta[srow] = dl;
   }
   int t0, t1;
   tile_range((klen + KT - 1) / KT, sp, a.splits, t0, t1);
@@ -853,6 +910,7 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored
   const uint8_t* mask = a.mask ? a.mask + b * a.maskb : nullptr;
   const int dbytes = (NP == 3 ? DT : a.D) * (int)sizeof(T);
   const int64_t klb = a.t0l * (int64_t)sizeof(T), vlb = a.t1l * (int64_t)sizeof(T);
+  const uint4 first = SUMS && mask ? mask16(mask, lane * 16, klen) : make_uint4(0, 0, 0, 0);
   MaskBytes<KT> mb;
   mask_fetch(mb, mask, t0 * KT, klen, lane);
   KeyWords<KT> cur = key_words(mb, mask != nullptr, t0 * KT, klen, lane), nxt = cur;
@@ -879,33 +937,31 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 1 && stored
 #pragma unroll
   for (int i = 0; i < DT / 32; ++i) zero16(dq[i]);
   const float SC = a.scale * LOG2E;
+  int* list = reinterpret_cast<int*>(start + 2 * KT);
+  const int n = SUMS ? few_keys(mask, order, klen, lane, list, wave == 0, first) : 0;
   wait_tiles();
-  if constexpr (NP == 1 && sizeof(T) == 2) {
-    if (few) {                                           // (one tile: t0 = 0, t1 = 1)
+  if constexpr (SUMS) {
+    if (n <= FEW) {                                      // (the same for the whole block)
+      char* few = smem + 2 * TILE;
+      for (int i = tid; i < 2 * 32 * (RB / 16); i += 256) {
+        const int c = i % (RB / 16), r = i / (RB / 16) % 32, x = i / (RB / 16 * 32);
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < n && c * 16 < dbytes) u = *reinterpret_cast<const uint4*>((x ? vbase : kbase) + list[r] * (x ? a.t1l : a.t0l) + c * (16 / sizeof(T)));
+        *reinterpret_cast<uint4*>(few + x * TILE + r * RB + (c ^ Swz<RB>::of(r)) * 16) = u;
+      }
+      if (tid < 32) start[KT + tid] = tid < n ? 0.f : -INFINITY;
+      wait_tiles();
+      f32x16 s, dp;
+      zero16(dp);
+      mma_rows_seen<T, DT, NP, TS>(s, few, 0, qf, start + KT, n == 32 ? 0xffffffffu : (1u << n) - 1u, li, lh);
+      mma_rows<T, DT, NP, TS>(dp, few + TILE, 0, dof, li, lh);
       float c = 0.f;
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb) {
-        const int blk = kg * NB + kb;
-        if (word_at(cur, blk) == 0) continue;
-        f32x16 s, dp;
-        zero16(dp);
-        mma_rows_seen<T, DT, NP, TS>(s, smem, blk, qf, start + blk * 32, word_at(cur, blk), li, lh);
-        mma_rows<T, DT, NP, TS>(dp, smem + TILE, blk, dof, li, lh);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) c = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)), dp[r] - dl, c);
-      }
-      c = both_sum(c);
-      if constexpr (KG > 1) {                            // the row group's key groups
-        float* red = start + 2 * KT;
-        if (lh == 0) red[wave * 32 + li] = c;
-        wait_tiles();
-        c = 0.f;
-#pragma unroll
-        for (int w = 0; w < KG; ++w) c += red[(rg * KG + w) * 32 + li];
-      }
-      dl += c;
-      if (m < M && lh == 0 && kg == 0) a.delta[srow] = dl;
+      for (int r = 0; r < 16; ++r) c = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], SC, -lse2)), dp[r] - dl, c);
+      dl += both_sum(c);
+      wait_tiles();                                      // every wave has read the buffer: the second tile may come
     }
+    if (sp == a.splits - 1 && m < M && lh == 0 && kg == 0) a.delta[srow] = dl;       // (the last share of an item with keys has a tile)
   }
   for (int t = t0; t < t1; ++t) {
     const int buf = NBUF == 2 ? (t - t0) & 1 : 0;

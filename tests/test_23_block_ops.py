@@ -1094,6 +1094,78 @@ def test_groupnorm_act_of_a_variance_past_the_range(dev, groups, L, dtype):
     assert not dx[1, :, :cg].any() and bool(dgamma.isfinite().all()) and bool(dbeta.isfinite().all())
 
 
+# ------------------------------------------------------------------------------------------------------------ few seen keys
+def score_gradient_oracle(q, k, v, do, seen, scale):
+    """(dq, dk) in 64 bits over the seen keys [B, Lk], and bounds that leave the rounding of the stored output out of the rows'
+    delta = sum_j P_j (do . v_j): P's relative error e, the 32-bit sums, the roundings of dS and of the result."""
+    B, Lq, H, D = q.shape
+    Lk, G = k.shape[1:3]
+    R, u = H // G, half_step(q.dtype)
+    dq, tq = (torch.zeros(B, Lq, H, D, dtype=torch.float64) for _ in range(2))
+    dk, tk = (torch.zeros(B, Lk, G, D, dtype=torch.float64) for _ in range(2))
+    q, k, v, do = (t.cpu().double() for t in (q, k, v, do))
+    for b in range(B):
+        j = seen[b].nonzero()[:, 0]
+        for h in range(H if len(j) else 0):
+            Q, K, V, dO = q[b, :, h], k[b, j, h // R], v[b, j, h // R], do[b, :, h]
+            S = Q @ K.T * scale
+            lse = torch.logsumexp(S, 1, keepdim=True)
+            P = torch.exp(S - lse)
+            e = (D + 4) * U32 * (Q.abs() @ K.abs().T * scale).max() + 4 * U32 * (S.abs().max() + lse.abs().max()) + (len(j) + 64) * U32
+            O, dP = P @ V, dO @ V.T
+            delta = (dO * O).sum(1, keepdim=True)
+            A = dO.abs() @ V.abs().T                             # what the 32-bit sums of dP go by
+            # delta = dl + sum P (dP - dl): dl (off by the rounding of o) enters with sum P - 1, i.e. e; then the sums
+            dl = (dO.abs() * (1 + u) * O.abs()).sum(1, keepdim=True)
+            E = 2 * e * (dl + (P * dP.abs()).sum(1, keepdim=True)) + (D + len(j) + 40) * U32 * ((P * A).sum(1, keepdim=True) + dl)
+            dS = P * (dP - delta)
+            eS = P * (E + (D + 4) * U32 * A) + (u + 2 * e) * dS.abs()
+            n = (max(len(j), R * Lq) + 16) * U32
+            dq[b, :, h], tq[b, :, h] = scale * dS @ K, scale * (eS + n * dS.abs()) @ K.abs()
+            dk[b, j, h // R] += scale * dS.T @ Q
+            tk[b, j, h // R] += scale * (eS + n * dS.abs()).T @ Q.abs()
+    return dq, tq + u * dq.abs() + 1e-30, dk, tk + u * dk.abs() + 1e-30
+
+
+@gpu
+@pytest.mark.parametrize("by", ["length", "mask", "both"])
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D", [
+    (4, 5, 256, 4, 2, 64),               # a few rows: four key groups
+    (4, 40, 256, 4, 2, 64),              # two key groups
+    (4, 33, 200, 2, 1, 96),
+    (2, 9, 1000, 3, 3, 128),
+    (3, 70, 700, 2, 2, 8),
+    (1, 3, 5000, 4, 2, 64),              # shares of a long axis, most of which see nothing
+    (1, 200, 2000, 2, 2, 40),
+    (64, 130, 300, 4, 4, 32),            # one key group
+    (64, 130, 129, 4, 4, 128),
+])
+def test_cross_attention_score_gradients_over_few_keys(dev, B, Lq, Lk, H, G, D, by):
+    """Values that share an offset of a hundred: the scores' gradients are differences of the offset's size, and the rounding of
+    a stored bf16 output would be as large as they are.  Two to 32 keys are seen, by a length, by a mask, by both."""
+    from styler_amd import ops
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, torch.bfloat16, seed=41)
+    v = (v + 100.0).to(torch.bfloat16)
+    g = torch.Generator().manual_seed(B + Lk)
+    count = [(2, 3, 32, 17, 31, 5)[b % 6] for b in range(B)]
+    if B == 64:                                               # (the oracle's time: three items see keys)
+        count = [c if b in (0, 20, 63) else 0 for b, c in enumerate(count)]
+    masked = torch.ones(B, Lk, dtype=torch.bool)
+    for b, n in enumerate(count):
+        masked[b, torch.randperm(Lk, generator=g)[:n]] = False
+    lens = {"length": torch.tensor(count), "mask": None, "both": torch.full((B,), Lk // 2)}[by]
+    mask = None if by == "length" else masked
+    seen = torch.arange(Lk)[None] < (torch.full((B,), Lk) if lens is None else lens)[:, None]
+    seen = seen if mask is None else seen & ~mask
+    on = lambda t: None if t is None else t.to(dev)
+    lse = torch.empty(B, H, Lq, device=dev)
+    out = ops.cross_attention(q, k, v, on(lens), mask=on(mask), lse=lse)
+    dq, dk, _ = ops.cross_attention_bwd(q, k, v, out, do, lse, on(lens), mask=on(mask))
+    rq, tq, rk, tk = score_gradient_oracle(q, k, v, do, seen, D ** -0.5)
+    within(dq.cpu(), rq, tq, "dq")
+    within(dk.cpu(), rk, tk, "dk")
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
