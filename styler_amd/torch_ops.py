@@ -547,7 +547,8 @@ OPS = ("conv_gemm", "conv_gemm_bwd", "attention", "attention_bwd", "add_layernor
 #     rotary                       rotary positions (its own backward, the opposite turn)
 #     groupnorm_act / _bwd         group norm over channels-last rows + activation -> (y, stats)
 #
-# lse and stats are what the backward operators take; they carry no gradient of their own (using one raises).
+# lse and stats are what the backward operators take; they carry no gradient of their own (using one raises), nor do rotary's
+# positions and angles (a backward pass that would owe them one raises).
 def _no_grad_of(name, g):
     if g is not None:
         raise ops.StylerHipError(f"styler::{name}: its second output has no gradient")
@@ -599,6 +600,8 @@ def _rotary_setup(ctx, inputs, output):
 
 
 def _rotary_backward(ctx, dy):
+    if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+        raise ops.StylerHipError("styler::rotary: positions and angles have no gradient (detach them)")
     freqs, pos = ctx.saved_tensors
     return torch.ops.styler.rotary(dy, freqs, pos, ctx.interleaved, ctx.gain, not ctx.inverse), None, None, None, None, None
 

@@ -1166,6 +1166,23 @@ def test_cross_attention_score_gradients_over_few_keys(dev, B, Lq, Lk, H, G, D, 
     within(dk.cpu(), rk, tk, "dk")
 
 
+# ------------------------------------------------------------------------------------------------------------ gradients that are not there
+@pytest.mark.parametrize("leaf", ["pos", "freqs"])
+def test_rotary_refuses_the_gradient_of_positions_and_angles(leaf):
+    """Fractional positions may come from predicted durations, angles may be a parameter: their gradients are not formed, and a
+    backward pass that would drop them says so."""
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 3, 64, requires_grad=True)
+        pos, freqs = torch.empty(5, requires_grad=leaf == "pos"), torch.empty(32, dtype=torch.float64, requires_grad=leaf == "freqs")
+        with pytest.raises(ops.StylerHipError, match="no gradient"):
+            torch.ops.styler.rotary(x, freqs, pos).sum().backward()
+        torch.ops.styler.rotary(x, freqs.detach(), pos.detach()).sum().backward()
+        assert x.grad.shape == x.shape
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
