@@ -600,7 +600,7 @@ def _rotary_setup(ctx, inputs, output):
 
 
 def _rotary_backward(ctx, dy):
-    if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+    if any(ctx.needs_input_grad[1:3]):                    # (arguments left out are left out here too)
         raise ops.StylerHipError("styler::rotary: positions and angles have no gradient (detach them)")
     freqs, pos = ctx.saved_tensors
     return torch.ops.styler.rotary(dy, freqs, pos, ctx.interleaved, ctx.gain, not ctx.inverse), None, None, None, None, None

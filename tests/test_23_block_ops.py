@@ -1181,6 +1181,7 @@ def test_rotary_refuses_the_gradient_of_positions_and_angles(leaf):
             torch.ops.styler.rotary(x, freqs, pos).sum().backward()
         torch.ops.styler.rotary(x, freqs.detach(), pos.detach()).sum().backward()
         assert x.grad.shape == x.shape
+        torch.ops.styler.rotary(x, freqs.detach()).sum().backward()          # (without positions)
 
 
 # ------------------------------------------------------------------------------------------------------------ the C entries
