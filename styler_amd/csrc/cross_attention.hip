@@ -154,17 +154,21 @@ __device__ __forceinline__ void dma_tile(char* smem, uint32_t lds, const void* b
     off = (word >> bit) & 1u ? off : OOB;
     // asm: the compiler lets no transposing LDS read start before the DMA it knows of has landed (it cannot tell the buffers
     // apart), i.e. it would wait for the NEXT tile in the middle of this one.  wait_tiles orders the DMA; the asm has no outputs.
+    // (m0 is reserved: the compiler keeps nothing in it, and takes no clobber of it.)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
                  :: "v"(off), "s"(rs), "s"(l0 + i * 4096), "s"(PICK ? 0 : r0 * (int)ldbytes) : "memory");
   }
 }
 // This wave's DMA has landed and its LDS reads are done; then all waves'.  The builtin, not asm: the compiler has to know that
-// nothing is outstanding, or it waits for everything where a value loaded before the loop is first used in it.
+// nothing is outstanding, or it waits for everything where a value loaded before the loop is first used in it.  The barrier itself
+// touches no memory as far as the optimiser is told: the empty asm on either side keeps LDS reads and writes on theirs.
 __device__ __forceinline__ void wait_tiles() {
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0)
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
 }
 
 // 64 floats of a row statistic, one a lane: base[lane], or 0 where lane >= n
