@@ -200,8 +200,11 @@ template <int DT> struct Frag<uint16_t, DT> { bf16x8 v[DT / 16]; };
 template <int DT> struct Frag<float, DT> { float4 v[DT / 8]; };
 template <typename T, int DT, int NP> struct Rows { Frag<T, DT> p[NP]; };
 
-// 8 values -> their planes
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[3]) {
+// 8 values -> their planes.  WHOLE: for all of fp32 (inputs): what a plane would round to infinity is cut to the largest bf16, so
+// that finite values stay finite (3.39e38 .. 3.40e38), and an infinity, handed down to the last plane, has products of one sign.  NaN
+// goes through the cut into the next plane's remainder.
+template <bool WHOLE = false> __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[3]) {
+  constexpr float TOP = 3.3895313892515355e38f;          // bf16 0x7f7f
   float r[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = x[e];
@@ -210,7 +213,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[3]) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      w[e] = cvt_pk_bf16_rne(r[2 * e], r[2 * e + 1]);
+      float a = r[2 * e], b = r[2 * e + 1];
+      if constexpr (WHOLE) if (k < 2) { a = fminf(fmaxf(a, -TOP), TOP); b = fminf(fmaxf(b, -TOP), TOP); }
+      w[e] = cvt_pk_bf16_rne(a, b);
       r[2 * e] -= __uint_as_float(w[e] << 16);
       r[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
     }
@@ -244,7 +249,7 @@ __device__ __forceinline__ void load_rows(Rows<T, DT, NP>& f, const void* base, 
       }
       const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       bf16x8 q[3];
-      split8(x, q);
+      split8<true>(x, q);
       f.p[0].v[i] = q[0]; f.p[1].v[i] = q[1]; f.p[2].v[i] = q[2];
     }
   }
@@ -349,7 +354,7 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* til
       bf16x8 pb[3];
       if constexpr (NP == 3) {
         const float v[8] = {p[s2 * 8], p[s2 * 8 + 1], p[s2 * 8 + 2], p[s2 * 8 + 3], p[s2 * 8 + 4], p[s2 * 8 + 5], p[s2 * 8 + 6], p[s2 * 8 + 7]};
-        split8(v, pb);
+        split8<>(v, pb);
       } else {
         pb[0] = pack8(p, s2);
       }
@@ -1245,7 +1250,7 @@ __global__ __launch_bounds__(256) void xattn_split_kernel(SplitArgs a) {
       }
       const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
       bf16x8 q[3];
-      split8(x, q);
+      split8<true>(x, q);
       uint16_t* o = a.dst[z] + ((int64_t)bh * L + l) * a.W + d;
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(o + k * plane) = q[k];

@@ -1184,6 +1184,97 @@ def test_rotary_refuses_the_gradient_of_positions_and_angles(leaf):
         torch.ops.styler.rotary(x, freqs.detach()).sum().backward()          # (without positions)
 
 
+@gpu
+@pytest.mark.parametrize("Lq,Lk", [(3, 40), (300, 2000)])
+def test_cross_attention_fp32_to_the_ends_of_the_range(dev, Lq, Lk):
+    """fp32 values up to the largest, in both arithmetics (few rows; many): what rounds to infinity in bf16 is finite here.  A key of
+    infinite distance (a score of -inf) is a key that is not seen."""
+    from styler_amd import ops
+    B, H, G, D = 2, 8, 4, 64
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, torch.float32, seed=51)
+    top = torch.finfo(torch.float32).max
+    v2 = v.clone()
+    v2[:, 7, :, 3], v2[:, 11, :, 5] = top, -top
+    got, ref = ops.cross_attention(q, k, v2), ops.cross_attention(q, k, v)
+    s = torch.matmul(q.double().transpose(1, 2), k.double().repeat_interleave(H // G, 2).permute(0, 2, 3, 1).contiguous()) / 8
+    p = torch.softmax(s, -1)
+    for d in (3, 5):
+        w = torch.matmul(p, v2[..., d].double().repeat_interleave(H // G, 2).transpose(1, 2)[..., None].contiguous())[..., 0].transpose(1, 2)
+        a = torch.matmul(p, v2[..., d].double().abs().repeat_interleave(H // G, 2).transpose(1, 2)[..., None].contiguous())[..., 0].transpose(1, 2)
+        # P's relative error: the scores' sums, the exponent's argument, the sum (as in attention_oracle, with its largest terms)
+        e = (D + 4) * U32 * 64 + 8 * U32 * float(s.abs().max()) + (Lk + 64) * U32
+        within(got[..., d].cpu(), w.cpu(), (2 * e * a).cpu(), d)
+    rest = [d for d in range(D) if d not in (3, 5)]
+    assert torch.equal(got[..., rest], ref[..., rest])
+    k3, mask = k.clone(), torch.zeros(B, Lk, dtype=torch.bool, device=dev)
+    q3 = q.clone()
+    q3[..., 0] = q3[..., 0].abs() + 1e-3
+    k3[:, 5, :, 0] = -math.inf
+    mask[:, 5] = True
+    a, b = ops.cross_attention(q3, k3, v), ops.cross_attention(q3, k, v, mask=mask)
+    assert bool(a.isfinite().all())
+    assert float((a - b).abs().max()) <= 2 * ((D + 4) * U32 * 64 + 8 * U32 * float(s.abs().max() + 8) + (Lk + 64) * U32) * float(v.abs().max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("Lq,Lk", [(1, 700), (45, 200), (300, 2000)])
+def test_cross_attention_shows_a_seen_nan(dev, Lq, Lk, dtype):
+    """A NaN among what is seen shows in everything that depends on it and in nothing else."""
+    from styler_amd import ops
+    B, H, G, D = 3, 4, 2, 64
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, dtype, seed=52)
+
+    def both(q, k, v, do):
+        lse = torch.empty(B, H, Lq, device=dev)
+        out = ops.cross_attention(q, k, v, lse=lse)
+        return (out, *ops.cross_attention_bwd(q, k, v, out, do, lse))
+
+    ref = both(q, k, v, do)
+    for i in range(4):
+        t = [q.clone(), k.clone(), v.clone(), do.clone()]
+        t[i][1, 0 if i in (0, 3) else Lk - 3, 1, 17] = math.nan              # query head 1 and key head 1: the key heads 0 and 1
+        got = both(*t)
+        g = 0 if i in (0, 3) else 1
+        heads = [1] if i in (0, 3) else [2, 3]
+        nan = [a.isnan() for a in got]
+        if i == 0:
+            assert bool(nan[0][1, 0, 1].all()) and not nan[0][1, 1:].any()
+        elif i == 1:
+            assert bool(nan[0][1][:, heads].all())
+        elif i == 2:
+            assert bool(nan[0][1][:, heads][..., 17].all()) and not nan[0][1][:, heads][..., :17].any()
+        if i == 3:
+            assert not nan[0].any()
+        assert bool(nan[1][1, 0, heads].any()) and bool(nan[2][1, :, g].any())
+        for a, b, own in zip(got, ref, (heads, heads, [g], [g])):
+            other = [h for h in range(a.shape[2]) if h not in own]
+            assert torch.equal(a[[0, 2]], b[[0, 2]]) and torch.equal(a[1][:, other], b[1][:, other])
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_shows_values_that_are_not_finite(dev, interleaved):
+    from styler_amd import ops
+    f = ops.rotary_freqs(48, dev)
+    for dtype in DT:
+        x = torch.randn(2, 9, 3, 64, generator=torch.Generator().manual_seed(3)).to(dtype).to(dev)
+        ref = ops.rotary(x, f, interleaved=interleaved)
+        x2 = x.clone()
+        x2[1, 4, 2, 6], x2[0, 3, 0, 60] = math.nan, math.inf                  # one of a pair; a feature that passes through
+        got = ops.rotary(x2, f, interleaved=interleaved)
+        pair = (6, 7) if interleaved else (6, 30)
+        assert all(bool(got[1, 4, 2, d].isnan()) for d in pair) and float(got[0, 3, 0, 60]) == math.inf
+        for d in pair:
+            got[1, 4, 2, d] = ref[1, 4, 2, d]
+        got[0, 3, 0, 60] = ref[0, 3, 0, 60]
+        assert torch.equal(got, ref)
+        pos = torch.arange(9, device=dev).float()
+        pos[5] = math.nan
+        got = ops.rotary(x, f, pos, interleaved=interleaved)
+        assert bool(got[:, 5, :, :48].isnan().all()) and bool(got[:, :5].isfinite().all()) and bool(got[:, 6:].isfinite().all())
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
