@@ -8,6 +8,7 @@ import functools
 import math
 import os
 
+import numpy as np
 import torch
 
 from ._lib import GN, ROTARY, XATTN, lib
@@ -1903,7 +1904,50 @@ def _new(t):
 
 def _rows_ok(shape, st):
     """Inner dimension contiguous, no two rows in the same place (an output)."""
-    return (st[-1] == 1 or shape[-1] == 1) and not any(n > 1 and s == 0 for n, s in zip(shape, st))
+    if st[-1] != 1 and shape[-1] != 1:
+        return False
+    dims, extent = sorted((s, n) for n, s in zip(shape[:-1], st[:-1]) if n > 1), shape[-1]
+    for s, n in dims:
+        if s < extent:
+            break
+        extent += s * (n - 1)
+    else:
+        return True
+    if any(s == 0 for s, _ in dims):
+        return False
+    starts = np.zeros(1, dtype=np.int64)                     # rows that interlock: look at where each one starts
+    for s, n in dims:
+        starts = np.add.outer(starts, np.arange(n, dtype=np.int64) * s).ravel()
+    return bool((np.diff(np.sort(starts)) >= shape[-1]).all())
+
+
+class _Layout:
+    """A tensor's place and strides for numpy's exact test of shared memory (which follows no address)."""
+
+    def __init__(self, t):
+        es = t.element_size()
+        self.__array_interface__ = {"version": 3, "typestr": f"<u{es}", "data": (t.data_ptr(), False), "shape": tuple(t.shape),
+                                    "strides": tuple(s * es for s in t.stride())}
+
+
+def _span(t):
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _shared(out, x):
+    """An element of `out` stands where one of `x` does.  (Slices of one buffer's rows may alternate without that.)"""
+    (a, a1), (b, b1) = _span(out), _span(x)
+    if a1 <= b or b1 <= a:
+        return False
+    try:
+        return np.shares_memory(np.asarray(_Layout(out)), np.asarray(_Layout(x)), max_work=100000)
+    except RuntimeError:                                     # (too many cases to look at)
+        return True
+
+
+def _in_place(out, x):
+    """Element by element in the same place (a stride that no step uses does not count)."""
+    return out is x or out.data_ptr() == x.data_ptr() and all(n < 2 or s == t for n, s, t in zip(x.shape, out.stride(), x.stride()))
 
 
 def _heads(t, es):
@@ -1963,7 +2007,7 @@ def _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, writes):
         _like(name, out, "out", qs, q.dtype, device)
         if writes and not (_rows_ok(qs, out.stride()) and _heads(out, 2 if bf16 else 4)[0] is out):
             _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
-        if writes and out.numel() and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        if writes and out.numel() and (_shared(out, q) or _shared(out, k) or _shared(out, v)):
             _refuse(name, "out shares memory with an input")
     if not q.is_cuda:
         _refuse(name, "there is no CPU form")
@@ -2058,7 +2102,7 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
     2 len(freqs) features of every head turned by pos * freqs (rotary_freqs), times gain; the features behind them pass through.
     Pair i is (2 i, 2 i + 1) if interleaved, else (i, i + len(freqs)).  pos: int64 or fp32 (fractional positions), [L] or
     [B or 1, L]; None: 0 .. L - 1.  Angles are formed in 64 bits.  inverse: the opposite turn, i.e. dx from dy.
-    out (optional): the result's tensor; out=x works in place, any other overlap with x does not."""
+    out (optional): the result's tensor; out=x works in place, any other overlap with x is refused."""
     name = "rotary"
     bf16, shape, device, n = _TYPES.get(x.dtype), x.shape, x.device, freqs.numel()
     if bf16 is None:
@@ -2083,7 +2127,7 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
         _refuse(name, f"gain {gain}: a finite number expected")
     if out is not None and not _rows_ok(_like(name, out, "out", shape, x.dtype, device).shape, out.stride()):
         _refuse(name, "out must have contiguous features and distinct rows")
-    if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel():
+    if out is not None and out.numel() and not _in_place(out, x) and _shared(out, x):
         _refuse(name, "out shares memory with x in another layout")
     if not x.is_cuda:
         _refuse(name, "there is no CPU form")
@@ -2132,6 +2176,8 @@ def _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, other, what):
         _refuse(name, "stats must be contiguous")
     if other is not None:
         _like(name, other, what, shape, x.dtype, device)
+        if what == "out" and other.numel() and not _in_place(other, x) and _shared(other, x):
+            _refuse(name, "out shares memory with x in another layout")
     if not x.is_cuda:
         _refuse(name, "there is no CPU form")
     return (B, L, C, groups), bf16, gamma, beta, lens
@@ -2150,10 +2196,9 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     """act(GroupNorm(x)) over channels-last x [B, L, C] (fp32 or bf16), `groups` groups of C / groups channels, gamma and beta fp32
     [C], act one of ACT_NONE / ACT_RELU / ACT_SILU / ACT_GELU.  lens int64 [B]: the statistics cover the rows before it, rows at or
     past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
-    groupnorm_act_bwd.  A NaN or an infinity in a group's rows makes the group NaN.  out (optional) may be x."""
+    groupnorm_act_bwd.  A NaN or an infinity in a group's rows makes the group NaN.  out (optional) may be x;
+    any other overlap with x is refused."""
     name = "groupnorm_act"
-    if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel():
-        _refuse(name, "out shares memory with x in another layout")
     sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, out, "out")
     B, L, C, _ = sizes
     device = x.device

@@ -1275,6 +1275,41 @@ def test_rotary_shows_values_that_are_not_finite(dev, interleaved):
         assert bool(got[:, 5, :, :48].isnan().all()) and bool(got[:, :5].isfinite().all()) and bool(got[:, 6:].isfinite().all())
 
 
+def test_block_operators_refuse_overlapping_outputs():
+    """Outputs that share some elements with an input, or rows with themselves; alternating slices of one buffer share none."""
+    from styler_amd import ops
+    f = ops.rotary_freqs(32, "cpu")
+    w = torch.ones(32)
+    buf = torch.zeros(2, 6, 12, 32)
+    q, k, v, o = buf[:, :, :4], buf[:, :, 4:6], buf[:, :, 6:8], buf[:, :, 8:]
+    for out in (buf[:, :, 3:7], buf[:, :, 5:9], buf[:, :, 7:11]):           # one head of q; of k and v; of v
+        with pytest.raises(ops.StylerHipError, match="shares memory"):
+            ops.cross_attention(q, k, v, out=out)
+    with pytest.raises(ops.StylerHipError, match="shares memory"):
+        ops.rotary(q, f, out=buf[:, :, 1:5])
+    rows = torch.zeros(2, 9, 32)
+    with pytest.raises(ops.StylerHipError, match="shares memory"):
+        ops.groupnorm_act(rows[:, 1:], w, w, 4, out=rows[:, :-1])           # the next row's place
+    flat = torch.zeros(1000)
+    twice = flat.as_strided((2, 4, 32), (130, 16, 1))                       # every row over half of the next
+    for bad in (lambda: ops.rotary(q, f, out=flat.as_strided(q.shape, (96, 16, 48, 1))),
+                lambda: ops.cross_attention(q, k, v, out=flat.as_strided(q.shape, (96, 16, 32, 1)))):
+        with pytest.raises(ops.StylerHipError, match="distinct rows"):
+            bad()
+    assert not ops._rows_ok(twice.shape, twice.stride())
+    assert ops._rows_ok((2, 4, 32), (32, 64, 1))                            # rows of the items in turn
+    assert ops._rows_ok((3, 2, 32), (64, 96, 1)) and not ops._rows_ok((4, 3, 32), (64, 96, 1))       # (0 64 128 96 160 224; 192 twice)
+    # what shares nothing, and what works in place, goes on to the next check
+    for fine in (lambda: ops.cross_attention(q, k, v, out=o), lambda: ops.rotary(q, f, out=o), lambda: ops.rotary(q, f, out=q),
+                 lambda: ops.groupnorm_act(rows[:, 1:], w, w, 4, out=rows[:, 1:]),
+                 lambda: ops.groupnorm_act(torch.zeros(1, 6, 64)[..., :32], w, w, 4, out=torch.zeros(1, 6, 64)[..., 32:])):
+        with pytest.raises(ops.StylerHipError, match="no CPU form"):
+            fine()
+    one = torch.zeros(1, 4, 2, 32)                                          # a batch of one: its item stride is not used
+    with pytest.raises(ops.StylerHipError, match="no CPU form"):
+        ops.rotary(one, f, out=one.as_strided(one.shape, (7, 64, 32, 1)))
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
