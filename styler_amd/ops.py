@@ -1871,6 +1871,7 @@ def adam_step(p, g, m, v, sumsq_buf, max_norm, lr, beta1, beta2, eps, step, grad
 # copied first.  They run on the current stream of the tensors' device, whichever device is current.  A token's call is bound by this
 # file: shapes, strides and types are looked at once each, and the arguments go over as one packed structure.
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_MOST = (1 << 31) - 1              # sizes travel as 32-bit integers
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 
@@ -1983,6 +1984,8 @@ def _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, writes):
         _refuse(name, "q [B, Lq, H, D] and k, v [B, Lk, G, D] expected")
     B, Lq, H, D = qs
     Lk, G = ks[1], ks[2]
+    if max(*qs, Lk) > _MOST:
+        _refuse(name, f"sizes up to {_MOST} expected")
     _like(name, k, "k", (B, Lk, G, D), q.dtype, device)
     _like(name, v, "v", ks, q.dtype, device)
     if G < 1 or H < 1 or H % G:
@@ -2110,6 +2113,8 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
     if len(shape) != 4:
         _refuse(name, "x [B, L, H, D] expected")
     B, L, H, D = shape
+    if max(shape) > _MOST:
+        _refuse(name, f"sizes up to {_MOST} expected")
     if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != device or not 2 <= 2 * n <= D:
         _refuse(name, f"freqs must be float64 [up to {D // 2}] on {device}")
     kind, posb = 0, 0
@@ -2123,7 +2128,7 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
             pos = pos.contiguous()
         if len(ps) == 2 and ps[0] > 1:
             posb = pos.stride(0)
-    if not math.isfinite(gain):
+    if not -3e38 < gain < 3e38:
         _refuse(name, f"gain {gain}: a finite number expected")
     if out is not None and not _rows_ok(_like(name, out, "out", shape, x.dtype, device).shape, out.stride()):
         _refuse(name, "out must have contiguous features and distinct rows")
@@ -2163,11 +2168,13 @@ def _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, other, what):
     if len(shape) != 3:
         _refuse(name, "x [B, L, C] expected")
     B, L, C = shape
+    if max(shape) > _MOST:
+        _refuse(name, f"sizes up to {_MOST} expected")
     if groups < 1 or C < 1 or C % groups:
         _refuse(name, f"{C} channels do not divide into {groups} groups")
     if act not in (ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU):
         _refuse(name, f"activation {act}: ACT_NONE, ACT_RELU, ACT_SILU or ACT_GELU expected")
-    if not 0.0 <= eps < math.inf:
+    if not 0.0 <= eps < 3e38:
         _refuse(name, f"eps {eps}: a number >= 0 expected")
     gamma = _vector(name, gamma, "gamma", C, torch.float32, device)
     beta = _vector(name, beta, "beta", C, torch.float32, device)

@@ -1310,6 +1310,31 @@ def test_block_operators_refuse_overlapping_outputs():
         ops.rotary(one, f, out=one.as_strided(one.shape, (7, 64, 32, 1)))
 
 
+def test_block_operators_refuse_sizes_and_numbers_past_32_bits():
+    """What the packed arguments cannot hold is refused like any other argument (no memory behind these: one element, expanded)."""
+    from styler_amd import ops
+    z, f, w = torch.zeros(1), ops.rotary_freqs(2, "cpu"), torch.ones(1)
+    wide = lambda *s: z.expand(*s)
+    n = (1 << 31) + 5
+    x = torch.zeros(2, 3, 1, 8)
+    for bad, text in [
+        (lambda: ops.cross_attention(wide(1, n, 1, 8), wide(1, 4, 1, 8), wide(1, 4, 1, 8)), "sizes up to"),
+        (lambda: ops.cross_attention(wide(1, 4, 1, 8), wide(1, n, 1, 8), wide(1, n, 1, 8)), "sizes up to"),
+        (lambda: ops.cross_attention(wide(n, 4, 1, 8), wide(n, 4, 1, 8), wide(n, 4, 1, 8)), "sizes up to"),
+        (lambda: ops.rotary(wide(1, n, 1, 2), f), "sizes up to"),
+        (lambda: ops.rotary(wide(1, 1, n, 2), f), "sizes up to"),
+        (lambda: ops.groupnorm_act(wide(1, n, 1), w, w, 1), "sizes up to"),
+        (lambda: ops.groupnorm_act(wide(n, 1, 1), w, w, 1), "sizes up to"),
+        (lambda: ops.groupnorm_act_bwd(wide(1, n, 1), wide(1, n, 1), w, w, torch.zeros(1, 1, 2), 1), "sizes up to"),
+        (lambda: ops.rotary(x, f, gain=1e39), "gain"),
+        (lambda: ops.rotary(x, f, gain=-math.inf), "gain"),
+        (lambda: ops.groupnorm_act(torch.zeros(2, 3, 8), torch.ones(8), torch.ones(8), 2, eps=1e39), "eps"),
+        (lambda: ops.cross_attention(x, x, x, scale=1e39), "scale"),
+    ]:
+        with pytest.raises(ops.StylerHipError, match=text):
+            bad()
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
