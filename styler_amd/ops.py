@@ -2025,7 +2025,9 @@ def cross_attention(q, k, v, lens=None, *, q_lens=None, mask=None, scale=None, o
     seen is never used; what is seen is finite.  q_lens int64 [B]: queries at or past it, like queries that see no key, give zeros
     and lse = -inf.
     lse (optional, fp32 [B, H, Lq]) receives the logarithm of the softmax's denominator, which cross_attention_bwd needs.
-    out (optional): the result's tensor, which shares no memory with the inputs."""
+    out (optional): the result's tensor, which shares no memory with the inputs.
+    The same call gives the same bits; an item by itself and the same item in a batch agree up to roundings only, as the batch decides
+    how keys are shared out (and, in fp32, by which instructions they are multiplied)."""
     name = "cross_attention"
     sizes, scale, lens, q_lens, mask, maskb = _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, True)
     device = q.device
@@ -2204,7 +2206,10 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
     [C], act one of ACT_NONE / ACT_RELU / ACT_SILU / ACT_GELU.  lens int64 [B]: the statistics cover the rows before it, rows at or
     past it give zeros and are not read.  stats (optional, fp32 [B, groups, 2]) receives mean and 1 / sqrt(var + eps) for
     groupnorm_act_bwd.  A NaN or an infinity in a group's rows makes the group NaN.  out (optional) may be x;
-    any other overlap with x is refused."""
+    any other overlap with x is refused.
+    16 channels a group with ReLU over all rows is also groupnorm_relu's case: that one is faster on long batches (48 x 1000 x 256 in
+    a graph, bf16 10.9 against 14.5 us, fp32 17.6 against 22.6; 16 x 60 x 320 4.5 against 4.4 to 5.5), this one cheaper to call
+    (7.7 us of the host against 10.5) and takes lengths."""
     name = "groupnorm_act"
     sizes, bf16, gamma, beta, lens = _gn_check(name, x, gamma, beta, groups, act, eps, lens, stats, out, "out")
     B, L, C, _ = sizes

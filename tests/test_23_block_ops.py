@@ -1335,6 +1335,31 @@ def test_block_operators_refuse_sizes_and_numbers_past_32_bits():
             bad()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D", [(40, 1, 900, 8, 2, 64), (16, 140, 520, 4, 4, 64), (24, 70, 300, 2, 1, 32)])
+def test_cross_attention_of_an_item_alone_and_in_a_batch(dev, B, Lq, Lk, H, G, D, dtype):
+    """The batch around an item decides how its keys are shared out (and, in fp32, by which instructions they are multiplied): its
+    results may change in the roundings, not by more."""
+    from styler_amd import ops
+    q, k, v, do = attention_case(dev, B, Lq, Lk, H, G, D, dtype, seed=61)
+    lens = torch.randint(1, Lk + 1, (B,), generator=torch.Generator().manual_seed(4))
+
+    def both(s):
+        n = lens[s].to(dev)
+        lse = torch.empty(len(n), H, Lq, device=dev)
+        out = ops.cross_attention(q[s], k[s], v[s], n, lse=lse)
+        return (out, *ops.cross_attention_bwd(q[s], k[s], v[s], out, do[s], lse, n))
+
+    whole = both(slice(0, B))
+    for b in (0, B // 2, B - 1):
+        s = slice(b, b + 1)
+        ref, tol = attention_oracle(q[s], k[s], v[s], do[s], lens[s], None, None, D ** -0.5, dtype)
+        for n, a, w, r, t in zip(("out", "dq", "dk", "dv"), both(s), whole, (ref[0], ref[2], ref[3], ref[4]), tol):
+            within(a.cpu(), r, t + 1e-30, n)
+            within(w[s].cpu(), r, t + 1e-30, n)
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
