@@ -339,9 +339,13 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& a, int s2) {
   return *reinterpret_cast<bf16x8*>(&v);
 }
 
-// acc[dt][32 features][32 lane rows] += tile(rows blk * 32 ..)^T . p      (p: accumulator registers of a 32 x 32 product.  bf16:
-// rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain; planes: split like the operands)
-template <typename T, int DT, int NP, int TS>
+// acc[dt][32 features][32 lane rows] += tile(rows blk * 32 ..)^T . p      (p: accumulator registers of a 32 x 32 product.  Planes:
+// split like the operands.  bf16: rounded to bf16 here, the one rounding between the two products of an fp32-accumulated chain.  It
+// is as large as the rounding of the result: out is 0.0023 off its 64-bit value (2-norm), 0.00165 of which are its own.  FINE adds
+// p's remainder as a second operand, and only the result's rounding is left; it is taken where the keys' bytes are the bound (few rows,
+// forward: 1500 keys 14.0 -> 14.1 us, 65537 keys 108.9 -> 110.0), not where it costs: 4 x 4096 x 4096 x 128 522 -> 705, training 8 x
+// 2048 x 1500 x 64 422 -> 458, 48 x 1000 x 133 x 64 70 -> 73, and their gradients would need the same of dS.)
+template <typename T, int DT, int NP, int TS, bool FINE = false>
 __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* tile, int blk, const f32x16& p, int lane) {
   constexpr int RB = stored(DT) * sizeof(T);
   const int li = lane & 31, lh = lane >> 5;
@@ -357,6 +361,14 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* til
         split8<>(v, pb);
       } else {
         pb[0] = pack8(p, s2);
+        if constexpr (FINE) {
+          const uint4 h = *reinterpret_cast<const uint4*>(&pb[0]);
+          const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+          f32x16 rest;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) rest[e] = p[s2 * 8 + e] - __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+          pb[1] = pack8(rest, 0);
+        }
       }
 #pragma unroll
       for (int dt = 0; dt < DT / 32; ++dt) {
@@ -374,7 +386,10 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DT / 32], const char* til
           a[k] = *reinterpret_cast<const bf16x8*>(&u);
         }
         if constexpr (NP == 3) mma_planes<false>(acc[dt], a, pb);
-        else acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], pb[0], acc[dt], 0, 0, 0);
+        else {
+          if constexpr (FINE) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], pb[1], acc[dt], 0, 0, 0);
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], pb[0], acc[dt], 0, 0, 0);
+        }
       }
     }
   } else {
@@ -675,7 +690,7 @@ __global__ __launch_bounds__(256, (waves_wanted<T, DT, KG, NP>(NP == 3 ? 3 : sto
       l += ls;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT, NP, TS>(o, tv, kg * NB + kb, s[kb], lane);
+      for (int kb = 0; kb < NB; ++kb) mma_cols<T, DT, NP, TS, KG == 4>(o, tv, kg * NB + kb, s[kb], lane);
       __builtin_amdgcn_s_setprio(0);
     }
     if (NBUF == 1 && t + 1 < t1) {

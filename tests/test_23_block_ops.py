@@ -1360,6 +1360,32 @@ def test_cross_attention_of_an_item_alone_and_in_a_batch(dev, B, Lq, Lk, H, G, D
             within(w[s].cpu(), r, t + 1e-30, n)
 
 
+@gpu
+@pytest.mark.parametrize("B,Lq,Lk,H,G,D", [(32, 1, 1500, 16, 4, 64), (2, 1, 8197, 8, 8, 128), (3, 5, 129, 6, 2, 96), (5, 2, 31, 8, 1, 40),
+                                           (40, 1, 700, 4, 4, 32), (2, 8, 5000, 4, 1, 80)])
+def test_cross_attention_tokens_are_rounded_once(dev, B, Lq, Lk, H, G, D):
+    """Up to 32 rows a key head, bf16: the probabilities keep 16 bits (two bf16 operands, 2^-17 left) between the two products, so
+    that the result is off by its own rounding and by 32-bit arithmetic."""
+    from styler_amd import ops
+    q, k, v, _ = attention_case(dev, B, Lq, Lk, H, G, D, torch.bfloat16, seed=71)
+    lens = torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(Lk))
+    lens[0] = Lk
+    out = ops.cross_attention(q, k, v, lens.to(dev)).cpu()
+    q, k, v = (t.cpu().double() for t in (q, k, v))
+    for b in range(B):
+        n = int(lens[b])
+        for h in range(H):
+            if n == 0:
+                assert not out[b, :, h].any()
+                continue
+            Q, K, V = q[b, :, h], k[b, :n, h // (H // G)], v[b, :n, h // (H // G)]
+            S = Q @ K.T * D ** -0.5
+            P = torch.softmax(S, -1)
+            lse = torch.logsumexp(S, 1)
+            e = (D + 4) * U32 * (Q.abs() @ K.abs().T * D ** -0.5).max() + 4 * U32 * (S.abs().max() + lse.abs().max()) + (n + 64) * U32
+            within(out[b, :, h], P @ V, half_step(torch.bfloat16) * (P @ V).abs() + (2.0 ** -17 + 2 * e) * (P @ V.abs()), (b, h))
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
