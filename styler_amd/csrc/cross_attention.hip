@@ -60,12 +60,6 @@ struct XArgs {
   float scale;
 };
 
-__device__ __forceinline__ int clamp_len(const int64_t* len, int b, int L) {
-  if (!len) return L;
-  const int64_t n = len[b];
-  return n < 0 ? 0 : (n > L ? L : (int)n);
-}
-
 // Launch slot -> logical block.  Workgroups go to the eight XCDs round robin, each with its own L2, and blocks that read the same
 // keys are neighbours in the logical order: runs of `chunk` logical blocks go to one XCD, run after run to the next.  (One eighth
 // of the blocks each would give an XCD whole items: with ragged lengths the XCD of the longest item then worked alone.)

@@ -33,12 +33,6 @@ struct GArgs {
   float eps;
 };
 
-__device__ __forceinline__ int gn_len(const int64_t* len, int b, int L) {
-  if (!len) return L;
-  const int64_t n = len[b];
-  return n < 0 ? 0 : (n > L ? L : (int)n);
-}
-
 // The kernels would be bound by their instructions with the library's erff and divisions (67 M values in 90 us leave 52
 // instructions a value): one v_exp_f32 and one v_rcp_f32 a value instead.
 __device__ __forceinline__ float sigmoid(float z) {
@@ -77,38 +71,10 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   return 1.f;
 }
 
-// V consecutive channels, kept as loaded
-template <bool B16, int V> struct Raw {
-  uint32_t w[B16 ? (V + 1) / 2 : V];
-  __device__ __forceinline__ void load(const void* base, int64_t idx) {
-    const char* p = reinterpret_cast<const char*>(base) + idx * (B16 ? 2 : 4);
-    constexpr int BY = V * (B16 ? 2 : 4);
-    if constexpr (BY == 16) { const uint4 u = *reinterpret_cast<const uint4*>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
-    else if constexpr (BY == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
-    else if constexpr (BY == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
-    else w[0] = *reinterpret_cast<const uint16_t*>(p);
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < (B16 ? (V + 1) / 2 : V); ++i) w[i] = 0;
-  }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (B16) return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-    else return __uint_as_float(w[i]);
-  }
-};
 template <bool B16, int V> __device__ __forceinline__ void put(void* base, int64_t idx, const float (&f)[V]) {
-  char* p = reinterpret_cast<char*>(base) + idx * (B16 ? 2 : 4);
-  constexpr int BY = V * (B16 ? 2 : 4);
-  if constexpr (B16 && V == 1) *reinterpret_cast<uint16_t*>(p) = (uint16_t)f32_to_bf16_bits(f[0]);
-  else {
-    uint32_t w[BY / 4];
-#pragma unroll
-    for (int i = 0; i < BY / 4; ++i) w[i] = B16 ? cvt_pk_bf16_rne(f[(2 * i) % V], f[(2 * i + 1) % V]) : __float_as_uint(f[i % V]);
-    if constexpr (BY == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else if constexpr (BY == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(p) = w[0];
-  }
+  Raw<B16, V> r;
+  r.set(f);
+  r.store(base, idx);
 }
 
 // K of each channel: the mean of two of the n rows (0 of none), the same for all of a column's threads
@@ -207,7 +173,7 @@ __global__ __launch_bounds__(T) void gn_slab_kernel(GArgs a) {
   const int c0 = nx % a.slabs * a.slab, tid = threadIdx.x, lane = tid & 63;
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv;
   const bool on = rl < RL;
-  const int n = gn_len(a.len, b, a.L), c = c0 + col * V;
+  const int n = clamp_len(a.len, b, a.L), c = c0 + col * V;
   float* red = sh;                                       // max(T V, slab)
   float* sa = sh + max(T * V, a.slab);                   // slab each
   float* sb = sa + a.slab;
@@ -348,7 +314,7 @@ __global__ __launch_bounds__(256) void gn_sums_kernel(GArgs a) {
   const int b = blockIdx.z, c0 = blockIdx.y * a.slab, tid = threadIdx.x;
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv, c = c0 + col * V;
   const bool on = rl < RL;
-  const int n = gn_len(a.len, b, a.L), t0 = blockIdx.x * a.rows, t1 = min(n, t0 + a.rows);
+  const int n = clamp_len(a.len, b, a.L), t0 = blockIdx.x * a.rows, t1 = min(n, t0 + a.rows);
   float* red = sh;
   float* sa = sh + T * V;
   float* sb = sa + a.slab;
@@ -434,7 +400,7 @@ template <bool BWD>
 __global__ __launch_bounds__(256) void gn_join_kernel(GArgs a, float* gw, float* pw) {
   __shared__ float red[2][256];
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int n = gn_len(a.len, b, a.L), live = (n + a.rows - 1) / a.rows;
+  const int n = clamp_len(a.len, b, a.L), live = (n + a.rows - 1) / a.rows;
   const int cl = min(a.cg, 256), RL = 256 / cl, r0 = tid / cl, c = tid - r0 * cl;
   const float* ws = a.ws + (int64_t)b * a.chunks * a.C * 2;
   const float count = (float)max(n, 1) * (float)a.cg;
@@ -497,7 +463,7 @@ __global__ __launch_bounds__(256) void gn_write_kernel(GArgs a, const float* gw)
   const int b = a.B - 1 - blockIdx.z, c0 = blockIdx.y * a.slab, tid = threadIdx.x;
   const int W = min(a.slab, a.C - c0), cv = W / V, RL = T / cv, rl = tid / cv, col = tid - rl * cv, c = c0 + col * V;
   if (rl >= RL) return;
-  const int n = gn_len(a.len, b, a.L), t0 = (a.chunks - 1 - (int)blockIdx.x) * a.rows, t1 = min(a.L, t0 + a.rows);
+  const int n = clamp_len(a.len, b, a.L), t0 = (a.chunks - 1 - (int)blockIdx.x) * a.rows, t1 = min(a.L, t0 + a.rows);
   float ga[V], be[V], R[V], S[V], m1[V], m2[V];          // h = R (x - S); forward: R includes gamma
 #pragma unroll
   for (int j = 0; j < V; ++j) {

@@ -30,38 +30,6 @@ struct RArgs {
 // i / d by a multiplication: m = floor(2^32 / d) + 1 is exact for i d < 2^32 (the host sees to it); d = 1 has m = 0
 __device__ __forceinline__ uint32_t div_magic(uint32_t i, uint32_t m) { return m ? __umulhi(i, m) : i; }
 
-// V consecutive elements of a bf16 or fp32 row, kept as loaded
-template <bool B16, int V> struct Raw {
-  static constexpr int BYTES = V * (B16 ? 2 : 4), NW = (BYTES + 3) / 4;
-  uint32_t w[NW];
-  __device__ __forceinline__ void load(const void* base, int64_t idx) {
-    const char* p = reinterpret_cast<const char*>(base) + idx * (B16 ? 2 : 4);
-    if constexpr (BYTES == 16) { const uint4 u = *reinterpret_cast<const uint4*>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
-    else if constexpr (BYTES == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
-    else if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
-    else w[0] = *reinterpret_cast<const uint16_t*>(p);
-  }
-  __device__ __forceinline__ void store(void* base, int64_t idx) const {
-    char* p = reinterpret_cast<char*>(base) + idx * (B16 ? 2 : 4);
-    if constexpr (BYTES == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
-  }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (B16) return __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-    else return __uint_as_float(w[i]);
-  }
-  __device__ __forceinline__ void set(const float (&f)[V]) {
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      if constexpr (!B16) w[i] = __float_as_uint(f[i]);
-      else if constexpr (V == 1) w[i] = f32_to_bf16_bits(f[0]);
-      else w[i] = cvt_pk_bf16_rne(f[2 * i], f[2 * i + 1]);
-    }
-  }
-};
-
 constexpr int UNROLL = 4;                                // items whose loads are in flight together
 // A block covers rpb rows (item, position).  An item is one slot of one head: V pairs (half layout; interleaved: the V / 2 pairs
 // of V consecutive features), or V features that pass through.  V: elements per access (interleaved and V = 1: the two elements
