@@ -1386,6 +1386,49 @@ def test_cross_attention_tokens_are_rounded_once(dev, B, Lq, Lk, H, G, D):
             within(out[b, :, h], P @ V, half_step(torch.bfloat16) * (P @ V).abs() + (2.0 ** -17 + 2 * e) * (P @ V.abs()), (b, h))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+def test_block_operators_with_gradients_in_a_graph(dev, dtype):
+    """Norm, rotary positions, attention and the gradients of all of them through the dispatcher, captured once and replayed with new
+    inputs and lengths; every replay equals the eager pass over leaves of its own."""
+    import styler_amd.torch_ops  # noqa: F401
+    from styler_amd import ops
+    B, Lq, Lk, H, G, D = 3, 70, 41, 4, 2, 64
+    gen = torch.Generator().manual_seed(77)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(dev)
+    shapes = [(B, Lq, H * D), (B, Lk, 2, G, D), (B, Lq, H, D)]
+    x, enc, dout = bufs = [r(*s) for s in shapes]
+    gamma, beta = (torch.randn(H * D, generator=gen).to(dev) for _ in range(2))
+    q_lens, lens = torch.tensor([70, 1, 33], device=dev), torch.tensor([41, 20, 7], device=dev)
+    freqs = ops.rotary_freqs(D, dev)
+
+    def step(x, enc, gamma, beta, dout):
+        x, enc, gamma, beta = leaves = [t.detach().requires_grad_() for t in (x, enc, gamma, beta)]
+        y, _ = torch.ops.styler.groupnorm_act(x, gamma, beta, 16, 6, 1e-5, q_lens)
+        q, k = torch.ops.styler.rotary(y.view(B, Lq, H, D), freqs), torch.ops.styler.rotary(enc[:, :, 0], freqs)
+        out = torch.ops.styler.cross_attention(q, k, enc[:, :, 1], lens, q_lens)[0]
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, enc, gamma, beta, dout)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, enc, gamma, beta, dout)
+    for turn in range(4):
+        for t in bufs:
+            t.copy_(torch.randn(t.shape, generator=gen).to(t.dtype))
+        q_lens.copy_(torch.randint(0, Lq + 1, (B,), generator=gen))
+        lens.copy_(torch.randint(0, Lk + 1, (B,), generator=gen))
+        want = [t.clone() for t in step(x.clone(), enc.clone(), gamma.clone(), beta.clone(), dout)]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), turn
+
+
 # ------------------------------------------------------------------------------------------------------------ the C entries
 def test_block_entry_points_refuse_before_any_launch():
     """Every refusal of the C entry points comes before a HIP call: these run without a GPU.  (Addresses are never followed.)"""
