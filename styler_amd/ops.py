@@ -1935,15 +1935,21 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
-def _shared(out, x):
-    """An element of `out` stands where one of `x` does.  (Slices of one buffer's rows may alternate without that.)"""
-    (a, a1), (b, b1) = _span(out), _span(x)
-    if a1 <= b or b1 <= a:
-        return False
-    try:
-        return np.shares_memory(np.asarray(_Layout(out)), np.asarray(_Layout(x)), max_work=100000)
-    except RuntimeError:                                     # (too many cases to look at)
-        return True
+def _shared(out, *inputs):
+    """An element of `out` stands where one of an input does.  (Slices of one buffer's rows may alternate without that.)"""
+    buf = out.untyped_storage().data_ptr()
+    for x in inputs:
+        if x.untyped_storage().data_ptr() != buf:            # (what most calls come to: half a us a tensor)
+            continue
+        (a, a1), (b, b1) = _span(out), _span(x)
+        if a1 <= b or b1 <= a:
+            continue
+        try:
+            if np.shares_memory(np.asarray(_Layout(out)), np.asarray(_Layout(x)), max_work=100000):
+                return True
+        except RuntimeError:                                 # (too many cases to look at)
+            return True
+    return False
 
 
 def _in_place(out, x):
@@ -2008,9 +2014,9 @@ def _xattn_check(name, q, k, v, out, lse, lens, q_lens, mask, scale, writes):
         _refuse(name, "lse must be contiguous")
     if out is not None:
         _like(name, out, "out", qs, q.dtype, device)
-        if writes and not (_rows_ok(qs, out.stride()) and _heads(out, 2 if bf16 else 4)[0] is out):
+        if writes and not ((out.is_contiguous() or _rows_ok(qs, out.stride())) and _heads(out, 2 if bf16 else 4)[0] is out):
             _refuse(name, "out must have contiguous features and distinct rows on 16 bytes")
-        if writes and out.numel() and (_shared(out, q) or _shared(out, k) or _shared(out, v)):
+        if writes and out.numel() and _shared(out, q, k, v):
             _refuse(name, "out shares memory with an input")
     if not q.is_cuda:
         _refuse(name, "there is no CPU form")
@@ -2132,7 +2138,7 @@ def rotary(x, freqs, pos=None, *, interleaved=False, gain=1.0, inverse=False, ou
             posb = pos.stride(0)
     if not -3e38 < gain < 3e38:
         _refuse(name, f"gain {gain}: a finite number expected")
-    if out is not None and not _rows_ok(_like(name, out, "out", shape, x.dtype, device).shape, out.stride()):
+    if out is not None and not (_like(name, out, "out", shape, x.dtype, device).is_contiguous() or _rows_ok(shape, out.stride())):
         _refuse(name, "out must have contiguous features and distinct rows")
     if out is not None and out.numel() and not _in_place(out, x) and _shared(out, x):
         _refuse(name, "out shares memory with x in another layout")
@@ -2219,7 +2225,7 @@ def groupnorm_act(x, gamma, beta, groups, act=ACT_SILU, *, eps=1e-5, lens=None, 
             return groupnorm_act(x, gamma, beta, groups, act, eps=eps, lens=lens, out=out, stats=stats)
     if out is None:
         out = _new(x)
-    elif not _rows_ok(out.shape, out.stride()):
+    elif not (out.is_contiguous() or _rows_ok(out.shape, out.stride())):
         _refuse(name, "out must have contiguous channels and distinct rows")
     if out.numel() == 0:
         if stats is not None:
