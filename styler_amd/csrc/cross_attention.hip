@@ -22,12 +22,15 @@
 // results a second launch joins.  fp32 with many rows: three bf16 planes (mma_planes).  Masks with many rows: xattn_order_kernel.
 // The backward is two walks, rows over keys (dq) and keys over rows (dk, dv); each rebuilds P, nothing is added by atomics.
 //
-// Bounds, as measured (us; TFLOP/s counts 4 and 10 flops a pair, head and feature, not the second P of the backward):
-//   forward 4 x 4096 x 4096, 16 heads of 128, bf16        527      1040 TFLOP/s: the matrix pipe at the clock this load leaves
-//   forward, 2 tokens, 65537 keys, 8 heads of 128, bf16   109      5.2 TB/s in the tiles (103), then the join
-//   forward, 32 tokens, 1500 keys, 4 key heads of 64      8.9 + 3.2 for 33 MB: start, two or three tiles a block, join
-//   training 8 x 2048 x 1500, 16 heads of 64, bf16        426      vector and matrix instructions (0.45 + 0.44 busy), masked keys left out
-//   training 8 x 1203 x 1001, 8 heads of 64, fp32         326      matrix pipe 0.53 .. 0.62 busy on six bf16 products for one
+// Bounds, as measured (us of a call, one after another, without a profiler, which adds a tenth to the matrix-bound ones; TFLOP/s counts 4
+// and 10 flops a pair, head and feature, not the second S and dP of the backward, 4 more):
+//   forward 4 x 4096 x 4096, 16 heads of 128, bf16        519      1060 TFLOP/s: the matrix pipe at the clock this load leaves
+//   forward, 2 tokens, 65537 keys, 8 heads of 128, bf16   110      5.2 TB/s in the tiles, then the join
+//   forward, 32 tokens, 1500 keys, 4 key heads of 64       14      two launches by the host; 9.8 + 4.0 of the device: start, two or three
+//                                                                  tiles a block (33 MB in all), join
+//   training 8 x 2048 x 1500, 16 heads of 64, bf16        417      vector and matrix instructions one after the other (0.45 + 0.44 busy)
+//   training 8 x 1203 x 1001, 8 heads of 64, fp32         321      six bf16 products for one (1142 / 6 = 190 TFLOP/s): those it forms, the
+//                                                                  second S and dP among them, take 230; waits at the tiles' barriers
 #include <type_traits>
 #include "common.h"
 
@@ -1078,7 +1081,11 @@ template <int N> __device__ __forceinline__ void add_from(f32x16 (&acc)[N], char
 // The block walks tiles of 64 query rows (32 of planes), head after head of the group; with KW = 2 two waves share the keys and each takes half of
 // a tile's rows.  S = Q K^T here, so the registers are 16 queries and their lse / delta come from LDS.  What an unseen key computes
 // stays in its own lane; zeros are stored for it.
-template <typename T, int DT, int NP> constexpr int DKV_UNROLL = stored(DT) * sizeof(T) * NP >= 256 ? 1 : 2;        // (twice the registers spill)
+// Registers: two blocks of rows in flight where a lane's K, V, dK and dV leave room for them.  With the waves asked for here the compiler
+// keeps 1 register of <64, 4 waves of keys>, 8 of <128, 4> and 25 of <128, 2> (bf16) in scratch; asking for a wave less frees them, and is
+// slower: backward 8 x 2048 x 1500 x 16 heads of 64 366 -> 374 us, 48 x 1000 x 133 x 4 x 64 62 -> 73, 4 x 2048 x 2048 x 16 / 4 x 128
+// 533 -> 550, 16 x 500 x 200 x 8 x 128 57 -> 67.
+template <typename T, int DT, int NP> constexpr int DKV_UNROLL = stored(DT) * sizeof(T) * NP >= 256 ? 1 : 2;
 template <typename T, int DT, int KW, int NP>
 __global__ __launch_bounds__(256, (stored(DT) * sizeof(T) * NP >= 512 ? 1 : stored(DT) * sizeof(T) * NP >= 256 ? 2 : 3)) void xattn_dkv_kernel(XArgs a) {
   typedef typename OutOf<T, NP>::type O;

@@ -5,8 +5,9 @@
 //   backward: dz = dy act'(z);  dbeta = sum dz, dgamma = sum dz xh;  with d = dz gamma and the group's means m1 = mean d,
 //   m2 = mean d xh:  dx = rstd (d - m1 - xh m2)
 //
-// Bound by memory.  Two forms (16 x 1000 x 320 bf16, fused: 11 us forward, 15 + 2 backward, one generation of blocks each; 8 x 16384 x
-// 512 fp32, split: 61 + 7 + 86 us forward, 119 + 7 + 137 backward, i.e. 5.1 TB/s over what the two passes move):
+// Two forms (kernel times of a trace).  8 x 16384 x 512 fp32, split: 62 + 8 + 85 us forward, 117 + 7 + 136 backward, bound by memory, 5.1
+// TB/s over what the two passes move.  16 x 1000 x 320 bf16, fused: 11 us forward, 15 + 2 to 4 backward, one generation of 160 blocks: 96
+// CUs have none, and on the others the vector unit is busy 0.62 and 0.76 of the time.
 //   * fused: a block owns a slab of whole groups of one item and keeps its values in registers between the statistics and the
 //     output, so x (and dy) is read once;
 //   * split (items too long for that, or too few of them): row chunks leave per-channel sums, a small launch joins them per
@@ -535,7 +536,7 @@ struct GPlan { bool fused; int v, slab, slabs, chunks, rows, it, T; };
 
 int gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
-// rows a thread of 1024 holds without spilling (the backward keeps x and dy)
+// rows a thread of 1024 holds without spilling (the backward keeps x as loaded and dz in 32 bits)
 constexpr int it_max(bool b16, int v, bool bwd) { return bwd ? (b16 && v == 8 ? 4 : 8) : 16; }
 
 GPlan gn_plan(int B, int L, int C, int G, int bf16, int v, bool bwd) {

@@ -19,7 +19,8 @@
 //     bits M for the combinations the model uses (one straight-line body each, the two rows' chains interleave across
 //     what used to be ~70 uniform branches per iteration); M < 0 is the same body driven by the run-time flags;
 //   * the dropout key schedule and thresholds are computed once per kernel.
-// Same expressions in the same order as before: the results are bit-identical to the round-2 kernel.
+// A row's channels are added in the order of wave_sum_up, and products that enter a sum as they stand elsewhere are rounded first
+// (mul_rounded): dx agrees bit for bit with the sixteen-lanes-per-row kernel's.
 enum { LNM_ALL16 = 1, LNM_DOT = 2, LNM_DROP = 4, LNM_INDROP = 8, LNM_LEN = 16, LNM_RELU = 32 };
 
 // Wave-wide sum from the nearest lanes to the farthest (xor 1, 2, 4, 8, 16, 32): the order in which the sixteen-lanes-per-row
