@@ -899,7 +899,8 @@ int styler_adam_step(float* p, const float* g, float* m, float* v, int64_t n, co
 
 /* Attention of queries [B, Lq, H, D] over keys / values [B, Lk, G, D] of another sequence, H % G == 0 (head h reads key head
  * h / (H / G)), D a multiple of 8 up to 128:  out = softmax(scale q k^T over the seen keys) v.  Key j of item b is seen iff
- * j < len[b] (len may be NULL) and mask[b * maskb + j] == 0 (mask may be NULL); what an unseen key's rows hold is not used.
+ * j < len[b] (len may be NULL) and mask[b * maskb + j] == 0 (mask may be NULL); what an unseen key's rows hold is not used, what
+ * a seen one's hold is finite.  `out` shares no memory with q, k, v.
  * Queries at or past q_len[b] (may be NULL) and queries that see no key give zeros and lse = -inf.  lse [B, H, Lq] (natural
  * logarithm of the softmax's denominator, scores included) may be NULL in the forward.  Strides (item, row, head) are in
  * elements, multiples of 16 bytes, features contiguous, 16-byte aligned bases; out / dq [B, Lq, H, D] and dk / dv
@@ -941,7 +942,8 @@ int styler_rotary(const styler_rotary_t* host_args, void* stream);
 
 /* Group norm over channels-last [B, L, C] with an activation (STYLER_ACT_NONE / RELU / SILU / GELU), C % G == 0: statistics of
  * group g over the C / G channels of the rows t < len[b] (len may be NULL), biased variance; rows at or past len[b] give zeros.
- * out = y; stats [B, G, 2] receives mean and 1 / sqrt(var + eps) (may be NULL in the forward).  The backward takes x, dy, stats
+ * A NaN or an infinity among a group's rows makes the group NaN.  out = y; stats [B, G, 2] receives mean and 1 / sqrt(var + eps)
+ * (may be NULL in the forward).  The backward takes x, dy, stats
  * and gives dx in `out` and dgamma, dbeta [C].  Strides (item, row) in elements, channels contiguous.  Deterministic. */
 typedef struct {
   const void *x, *dy;
